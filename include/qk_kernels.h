@@ -46,6 +46,8 @@ enum {
 
 /* dtype tags: crates/quantibbler-kernels/src/dtype.rs:99-129 (Dtype, NAMES). */
 enum { QK_F64 = 0, QK_F32 = 1, QK_BF16 = 2 };
+/* Storage of a key/value cache only (qk_kv_cache): INT8 codes with a float32 scale per row. */
+enum { QK_I8 = 3 };
 
 typedef struct qk_ctx qk_ctx;
 typedef struct qk_layer qk_layer;
@@ -791,6 +793,73 @@ qk_status qk_grouped_attention(qk_ctx *ctx, const qk_grouped_call *call);
 size_t qk_grouped_scratch(size_t tokens, size_t heads, size_t kv_heads, size_t vdim_stride, size_t n_splits);
 /* One portion of one sequence (bfloat16 projections, caches and output; strides up to 256). */
 qk_status qk_grouped_portion(qk_ctx *ctx, const qk_grouped_call *call);
+
+/* ------------------------------------------------------------------ key/value caches
+ * A cache of key and value rows per sequence slot in float32, bfloat16 or INT8, the attention of a step and
+ * of a prompt's portion over it, and the same with rows in front that all sequences share.  No reference
+ * counterpart (the reference's cache is float32 or bfloat16, engine/mod.rs:1189-1209; the INT8 rows follow its
+ * per-token quantiser, src/quantibbler/kernels/attention_sage.py:148-174).  The calls only launch kernels on
+ * the context's stream, which the tensors must be ordered with; device memory belongs to the caller; the
+ * device that is current before a call is current after it.  Arguments are checked on the host before
+ * anything is launched.
+ *
+ * QK_I8: a row x of head_dim values (a token's key, rotated, or value of one kv head) is held as
+ * scale = float32(max|x| / 127), 1 where that is zero, and the codes clip(rint(x / scale), -127, 127), ties to
+ * even, all in 64 bits.  A row that holds an infinity or NaN gets the scale NaN: what reads it is NaN, never a
+ * wrong number.  The value is code * scale. */
+typedef struct qk_kv_cache {
+    int32_t dtype;            /* QK_F32, QK_BF16 or QK_I8 */
+    void *k, *v;              /* [n_seq][n_kv_heads][rows][head_dim] */
+    float *k_scale, *v_scale; /* QK_I8: [n_seq][n_kv_heads][rows]; else null */
+    size_t n_seq, n_kv_heads, rows, head_dim;
+} qk_kv_cache;
+/* Checks a description, and makes what later calls on this context need (the error word): call it once,
+ * before any stream capture. */
+qk_status qk_cache_check(qk_ctx *ctx, const qk_kv_cache *cache);
+/* Rotates q and k as qk_rope_cache does and writes k, v into row positions[t] - first_position of slot
+ * seq_index[t].  q (null: none) [n_tokens][n_heads][head_dim] goes to q_out (q itself allowed); tokens are
+ * q_stride, q_out_stride, k_stride, v_stride values apart.  cos_sin [n_positions][head_dim/2][2].  A token
+ * whose row, slot or position does not exist is skipped (its q too) and reported by qk_gpu_synchronize
+ * (QK_ERR_VALUE).  Where several tokens of a call name one row, the last of them stays. */
+qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q, size_t q_stride, float *q_out,
+                          size_t q_out_stride, size_t n_heads, const float *k, size_t k_stride, const float *v,
+                          size_t v_stride, const float *cos_sin, size_t n_positions, const int32_t *positions,
+                          const int32_t *seq_index, size_t first_position, size_t n_tokens);
+/* The rows of the named tokens as values: k_out, v_out [n_tokens][n_kv_heads][head_dim] in out_dtype (QK_F32,
+ * or QK_BF16: rounded once).  A row that does not exist reads as zeros and is reported like in qk_cache_append. */
+qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *positions, const int32_t *seq_index,
+                        size_t first_position, size_t n_tokens, int32_t out_dtype, void *k_out, void *v_out);
+/* softmax(q k^T / sqrt(head_dim)) v for one query per sequence: sequence b (of batch <= cache->n_seq) sees
+ * rows 0 .. kv_len[b] - 1 of its slot (kv_len is clamped to 0 .. rows) and, with prefix_len > 0, the first
+ * prefix_len rows of slot prefix_seq of `prefix`, which are read once for all sequences.  The two caches agree
+ * in dtype, kv heads and head_dim; `prefix` may be the same cache.  A sequence that sees no row gets zeros.
+ * q [batch][n_heads][head_dim] (already rotated) and out, batch rows q_stride and out_stride values apart.
+ * scratch: qk_cache_attend_scratch bytes, nothing kept in it between calls; calls that may overlap on the
+ * device need one each.  head_dim up to 256; head_dim 64 and 128 with 16-byte aligned rows run on the tensor
+ * cores (all but float32 caches), others take a plain kernel. */
+qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, size_t prefix_seq,
+                          size_t prefix_len, const float *q, size_t q_stride, const int32_t *kv_len, size_t batch,
+                          size_t n_heads, void *scratch, float *out, size_t out_stride);
+size_t qk_cache_attend_scratch(const qk_kv_cache *cache, size_t prefix_len, size_t batch, size_t n_heads);
+/* The same for n_tokens consecutive tokens of one sequence whose rows first_row .. first_row + n_tokens - 1 have
+ * been appended: token t sees rows 0 .. first_row + t of slot seq, and the prefix. */
+qk_status qk_cache_portion(qk_ctx *ctx, const qk_kv_cache *cache, size_t seq, size_t first_row, const qk_kv_cache *prefix,
+                           size_t prefix_seq, size_t prefix_len, const float *q, size_t q_stride, size_t n_tokens,
+                           size_t n_heads, void *scratch, float *out, size_t out_stride);
+size_t qk_cache_portion_scratch(const qk_kv_cache *cache, size_t first_row, size_t prefix_len, size_t n_tokens,
+                                size_t n_heads);
+
+/* Log probabilities from logits x [n_tokens][vocab], rows `stride` values apart.  Per row:
+ * lse = ln sum_v e^x_v; logprob = x_target - lse; entropy = -sum_v p_v ln p_v (in nats); the n_top <= 32 largest
+ * entries as top_ids [n_tokens][n_top] (ties: the lowest id first) with their log probabilities.  An entry of
+ * -infinity has probability 0 and adds nothing to the entropy.  A row whose largest entry is -infinity or
+ * +infinity, or that holds a NaN, gives NaN throughout (its top_ids: -1).  targets may be null (no logprob);
+ * a negative target marks a row without a token: its logprob is 0; a target >= vocab gives NaN.  Any output
+ * may be null.  scratch: qk_log_probs_scratch bytes, nothing kept in it between calls. */
+qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t vocab, size_t stride,
+                       const int32_t *targets, size_t n_top, void *scratch, float *lse, float *logprob, float *entropy,
+                       float *top_logprob, int32_t *top_ids);
+size_t qk_log_probs_scratch(size_t n_tokens, size_t vocab, size_t n_top);
 
 /* Which GEMV kernel qk_layer_apply and the group calls use: 0 = sign-select SIMT, 1 = bit-sliced
  * INT8 tensor-core (default; many instances per launch run in the persistent streaming form, few and

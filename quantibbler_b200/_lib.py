@@ -15,6 +15,7 @@ from . import _build
 
 QK_OK, QK_ERR_VALUE, QK_ERR_INIT, QK_ERR_CUDA, QK_ERR_TIMEOUT, QK_ERR_ALLOC = range(6)
 QK_F64, QK_F32, QK_BF16 = 0, 1, 2
+QK_I8 = 3   # key/value caches only
 DTYPE_TAGS = {"float64": QK_F64, "float32": QK_F32, "bfloat16": QK_BF16}
 
 
@@ -176,6 +177,21 @@ _SIGNATURES = {
     "qk_window_attention": (c_int32, [c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t,
                                       c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_float, c_void_p,
                                       c_size_t]),
+    "qk_cache_check": (c_int32, [c_void_p, c_void_p]),
+    "qk_cache_append": (c_int32, [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_void_p,
+                                  c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t,
+                                  c_size_t]),
+    "qk_cache_read": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_int32, c_void_p,
+                                c_void_p]),
+    "qk_cache_attend": (c_int32, [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p,
+                                  c_size_t, c_size_t, c_void_p, c_void_p, c_size_t]),
+    "qk_cache_attend_scratch": (c_size_t, [c_void_p, c_size_t, c_size_t, c_size_t]),
+    "qk_cache_portion": (c_int32, [c_void_p, c_void_p, c_size_t, c_size_t, c_void_p, c_size_t, c_size_t, c_void_p,
+                                   c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t]),
+    "qk_cache_portion_scratch": (c_size_t, [c_void_p, c_size_t, c_size_t, c_size_t, c_size_t]),
+    "qk_log_probs": (c_int32, [c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p,
+                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "qk_log_probs_scratch": (c_size_t, [c_size_t, c_size_t, c_size_t]),
     "qk_set_wait_limit": (ctypes.c_uint32, [c_void_p, ctypes.c_uint32]),
     "qk_set_dependent_launch": (c_int32, [c_void_p, c_int32]),
 }

@@ -1,0 +1,442 @@
+// Key/value caches in float32, bfloat16 and INT8: appending with rotation and quantisation, reading back, the
+// attention of a step and of a prompt's portion, both with rows in front that all sequences share.
+#include <algorithm>
+#include <cmath>
+
+#include "qk_cache.h"
+#include "qk_decoder_dev.cuh"
+
+namespace {
+
+using qk::CacheView;
+
+// ------------------------------------------------------------------ append
+// x / scale, rounded to the nearest integer (ties to even) as 64-bit arithmetic does it: the 32-bit quotient is
+// off by less than 1e-4 (127 * 2^-22 from x and its division), so only next to a border is the division done in
+// 64 bits.
+__device__ __forceinline__ int quantise(double x, float scale, float inv) {
+    const float t = (float)x * inv;
+    if (fabsf(fabsf(t - truncf(t)) - 0.5f) > 1e-3f) return min(127, max(-127, __float2int_rn(t)));
+    return min(127, max(-127, __double2int_rn(x / (double)scale)));
+}
+
+// Whether a later token of the call names the same row.  All threads of the block take part.
+__device__ __forceinline__ bool superseded(const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index,
+                                           uint32_t tok, uint32_t n_tokens) {
+    const int pos = positions[tok], seq = seq_index[tok];
+    int later = 0;
+    for (uint32_t i = tok + 1 + threadIdx.x; i < n_tokens; i += blockDim.x)
+        later |= positions[i] == pos && seq_index[i] == seq;
+    return __syncthreads_or(later) != 0;
+}
+
+// One block per token and share of its rows; a warp per row (a head of q, k or v), a lane holds the pairs
+// i, i + d/2 it rotates.  What bounds it: a large prompt's bytes (q read and written in float32 are most of them).
+template <typename KV>  // float, uint16_t (bfloat16), int8_t
+__global__ void __launch_bounds__(256)
+append_kernel(CacheView c, const float *__restrict__ q, size_t q_stride, float *__restrict__ q_out, size_t q_out_stride,
+              uint32_t n_heads, const float *__restrict__ k, size_t k_stride, const float *__restrict__ v, size_t v_stride,
+              const float *__restrict__ cos_sin, uint32_t n_positions, const int32_t *__restrict__ positions,
+              const int32_t *__restrict__ seq_index, uint32_t first_position, uint32_t n_tokens, int *__restrict__ error) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    const uint32_t tok = blockIdx.x, half = c.d / 2, lane = threadIdx.x % 32;
+    const int64_t pos = positions[tok], seq = seq_index[tok], row = pos - (int64_t)first_position;
+    if (row < 0 || row >= (int64_t)c.rows || pos >= (int64_t)n_positions || seq < 0 || seq >= (int64_t)c.n_seq) {
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(error, 4);
+        return;
+    }
+    const bool hidden = superseded(positions, seq_index, tok, n_tokens);
+    const float *cs = cos_sin + (size_t)pos * c.d;
+    const uint32_t heads = q ? n_heads : 0, n_rows = heads + (hidden ? 0 : 2 * c.n_kv);
+    for (uint32_t r = blockIdx.y * (blockDim.x / 32) + threadIdx.x / 32; r < n_rows; r += gridDim.y * (blockDim.x / 32)) {
+        const bool is_q = r < heads, is_k = !is_q && r - heads < c.n_kv;
+        const uint32_t h = is_q ? r : is_k ? r - heads : r - heads - c.n_kv;
+        const float *src = is_q ? q + tok * q_stride + (size_t)h * c.d
+                                : (is_k ? k + tok * k_stride : v + tok * v_stride) + (size_t)h * c.d;
+        if (is_q) {
+            float *dst = q_out + tok * q_out_stride + (size_t)h * c.d;
+            for (uint32_t i = lane; i < half; i += 32) {
+                const float a = src[i], b = src[half + i], co = cs[2 * i], si = cs[2 * i + 1];
+                dst[i] = rope_first(a, b, co, si);
+                dst[half + i] = rope_second(a, b, co, si);
+            }
+            continue;
+        }
+        const size_t line = ((size_t)seq * c.n_kv + h) * c.rows + (size_t)row;
+        KV *dst = static_cast<KV *>(is_k ? c.k : c.v) + line * c.d;
+        if constexpr (sizeof(KV) != 1) {
+            for (uint32_t i = lane; i < half; i += 32) {
+                const float a = src[i], b = src[half + i], co = is_k ? cs[2 * i] : 1.f, si = is_k ? cs[2 * i + 1] : 0.f;
+                store_from_float<KV>(dst, i, is_k ? rope_first(a, b, co, si) : a);
+                store_from_float<KV>(dst, half + i, is_k ? rope_second(a, b, co, si) : b);
+            }
+        } else {
+            double x[2][4];  // (head_dim <= 256: four pairs a lane); products of two float32 are exact
+            double peak = 0.0;
+            bool finite = true;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t i = lane + 32 * e;
+                x[0][e] = x[1][e] = 0.0;
+                if (i >= half) continue;
+                const double a = src[i], b = src[half + i];
+                if (is_k) {
+                    const double co = cs[2 * i], si = cs[2 * i + 1];
+                    x[0][e] = fma(a, co, -(b * si));
+                    x[1][e] = fma(b, co, a * si);
+                } else {
+                    x[0][e] = a, x[1][e] = b;
+                }
+                finite = finite && fabs(x[0][e]) < INFINITY && fabs(x[1][e]) < INFINITY;
+                peak = fmax(peak, fmax(fabs(x[0][e]), fabs(x[1][e])));
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) peak = fmax(peak, __shfl_xor_sync(0xffffffffu, peak, off));
+            finite = __all_sync(0xffffffffu, finite);
+            float scale = (float)(peak / 127.0);
+            if (scale == 0.f) scale = 1.f;
+            const float inv = 1.f / scale;  // (infinite for the smallest scales: then every code takes the division)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t i = lane + 32 * e;
+                if (i >= half) continue;
+                dst[i] = (int8_t)(finite ? quantise(x[0][e], scale, inv) : 0);
+                dst[half + i] = (int8_t)(finite ? quantise(x[1][e], scale, inv) : 0);
+            }
+            if (lane == 0) (is_k ? c.k_scale : c.v_scale)[line] = finite ? scale : __int_as_float(0x7fffffff);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ reading back
+template <typename KV> __device__ __forceinline__ float value_at(const KV *p, size_t i, float) {
+    return load_as_float<KV>(p, i);
+}
+template <> __device__ __forceinline__ float value_at<int8_t>(const int8_t *p, size_t i, float scale) {
+    return (float)p[i] * scale;
+}
+
+template <typename KV, typename Out>
+__global__ void __launch_bounds__(256)
+read_kernel(CacheView c, const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index, uint32_t first_position,
+            uint32_t n_tokens, Out *__restrict__ k_out, Out *__restrict__ v_out, int *__restrict__ error) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    const uint32_t lane = threadIdx.x % 32;
+    const size_t r = (size_t)blockIdx.x * 8 + threadIdx.x / 32;  // (token, kv head, k or v)
+    if (r >= (size_t)n_tokens * c.n_kv * 2) return;
+    const bool is_v = r % 2;
+    const uint32_t h = (uint32_t)(r / 2 % c.n_kv), tok = (uint32_t)(r / 2 / c.n_kv);
+    const int64_t row = (int64_t)positions[tok] - (int64_t)first_position, seq = seq_index[tok];
+    const bool there = row >= 0 && row < (int64_t)c.rows && seq >= 0 && seq < (int64_t)c.n_seq;
+    if (!there && lane == 0) atomicOr(error, 4);
+    const size_t line = there ? ((size_t)seq * c.n_kv + h) * c.rows + (size_t)row : 0;
+    const KV *src = static_cast<const KV *>(is_v ? c.v : c.k) + line * c.d;
+    const float scale = sizeof(KV) == 1 && there ? (is_v ? c.v_scale : c.k_scale)[line] : 1.f;
+    Out *dst = (is_v ? v_out : k_out) + ((size_t)tok * c.n_kv + h) * c.d;
+    for (uint32_t i = lane; i < c.d; i += 32) store_from_float<Out>(dst, i, there ? value_at<KV>(src, i, scale) : 0.f);
+}
+
+// ------------------------------------------------------------------ attention, plain form
+// Any dtype and head size: a warp per (query row, head), the lanes share the channels, one pass with the running
+// maximum and sum.  What the fast kernels cannot hold runs here.
+template <typename KV>
+__global__ void __launch_bounds__(128)
+attend_plain_kernel(CacheView c, CacheView p, qk::AttendArgs a) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    const size_t row = (size_t)blockIdx.x * 4 + threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x % 32, d = c.d;
+    if (row >= (size_t)a.n_queries * a.n_heads) return;
+    const uint32_t t = (uint32_t)(row / a.n_heads), head = (uint32_t)(row % a.n_heads), kvh = head / (a.n_heads / c.n_kv);
+    const float *qr = a.q + t * a.q_stride + (size_t)head * d;
+    const float scale = 1.0f / sqrtf((float)d);
+    float qv[8], o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t i = lane + 32 * e;
+        qv[e] = i < d ? qr[i] * scale : 0.f;
+        o[e] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    auto span = [&](const CacheView &s, size_t slot, uint32_t n) {
+        const size_t line0 = (slot * s.n_kv + kvh) * s.rows;
+        const KV *kb = static_cast<const KV *>(s.k) + line0 * d, *vb = static_cast<const KV *>(s.v) + line0 * d;
+        for (uint32_t j = 0; j < n; ++j) {
+            const float ks = sizeof(KV) == 1 ? s.k_scale[line0 + j] : 1.f, vs = sizeof(KV) == 1 ? s.v_scale[line0 + j] : 1.f;
+            float dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t i = lane + 32 * e;
+                if (i < d) dot = fmaf(qv[e], value_at<KV>(kb, (size_t)j * d + i, 1.f), dot);
+            }
+            for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+            const float x = dot * ks, m_new = fmaxf(m, x), alpha = m_new == -INFINITY ? 1.f : expf(m - m_new);
+            const float w = x == -INFINITY ? 0.f : expf(x - m_new);
+            l = l * alpha + w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t i = lane + 32 * e;
+                if (i < d) o[e] = o[e] * alpha + w * vs * value_at<KV>(vb, (size_t)j * d + i, 1.f);
+            }
+            m = m_new;
+        }
+    };
+    if (a.prefix_len) span(p, a.prefix_seq, a.prefix_len);
+    if (a.kv_len) span(c, t, (uint32_t)min(max(a.kv_len[t], 0), (int)c.rows));
+    else span(c, a.seq, a.first_row + t + 1);
+    float *dst = a.out + t * a.out_stride + (size_t)head * d;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t i = lane + 32 * e;
+        if (i < d) dst[i] = l == 0.f ? 0.f : o[e] / l;
+    }
+}
+
+// ------------------------------------------------------------------ host side
+using qk::DeviceGuard;
+
+qk_status check_cache(const qk_kv_cache *c, const char *what) {
+    if (!c) return qk::fail(QK_ERR_VALUE, "%s is null", what);
+    if (c->dtype != QK_F32 && c->dtype != QK_BF16 && c->dtype != QK_I8)
+        return qk::fail(QK_ERR_VALUE, "%s: dtype must be float32, bfloat16 or int8, got tag %d", what, c->dtype);
+    if (c->n_seq == 0 || c->n_kv_heads == 0 || c->rows == 0 || c->head_dim == 0)
+        return qk::fail(QK_ERR_VALUE, "%s is empty: %zu slots, %zu kv heads, %zu rows, head_dim %zu", what, c->n_seq,
+                        c->n_kv_heads, c->rows, c->head_dim);
+    if (c->head_dim > 256 || c->head_dim % 2)
+        return qk::fail(QK_ERR_VALUE, "%s: head_dim must be even and at most 256, got %zu", what, c->head_dim);
+    if (c->rows > 0x7fffffffull || c->n_seq > 0x7fffffffull || c->n_kv_heads > 65535)
+        return qk::fail(QK_ERR_VALUE, "%s: at most 2^31 - 1 rows and slots and 65535 kv heads, got %zu, %zu, %zu", what, c->rows,
+                        c->n_seq, c->n_kv_heads);
+    if (!c->k || !c->v) return qk::fail(QK_ERR_VALUE, "%s: k or v is null", what);
+    if (c->dtype == QK_I8 && (!c->k_scale || !c->v_scale))
+        return qk::fail(QK_ERR_VALUE, "%s: an int8 cache needs k_scale and v_scale", what);
+    return QK_OK;
+}
+
+CacheView view(const qk_kv_cache *c) {
+    CacheView v{};
+    if (c) {
+        v.k = c->k, v.v = c->v, v.k_scale = c->k_scale, v.v_scale = c->v_scale;
+        v.rows = (uint32_t)c->rows, v.n_seq = (uint32_t)c->n_seq, v.n_kv = (uint32_t)c->n_kv_heads, v.d = (uint32_t)c->head_dim;
+        v.dtype = c->dtype;
+    }
+    return v;
+}
+
+// The prefix of an attention call fits the cache it stands in front of.
+qk_status check_prefix(const qk_kv_cache *c, const qk_kv_cache *p, size_t prefix_seq, size_t prefix_len) {
+    if (prefix_len == 0) return QK_OK;
+    qk_status st = check_cache(p, "prefix");
+    if (st != QK_OK) return st;
+    if (p->dtype != c->dtype || p->n_kv_heads != c->n_kv_heads || p->head_dim != c->head_dim)
+        return qk::fail(QK_ERR_VALUE, "prefix and cache must agree in dtype, kv heads and head_dim: tags %d, %d; %zu, %zu; %zu, %zu",
+                        p->dtype, c->dtype, p->n_kv_heads, c->n_kv_heads, p->head_dim, c->head_dim);
+    if (prefix_seq >= p->n_seq || prefix_len > p->rows)
+        return qk::fail(QK_ERR_VALUE, "prefix: %zu rows of slot %zu do not lie in %zu slots of %zu rows", prefix_len, prefix_seq,
+                        p->n_seq, p->rows);
+    return QK_OK;
+}
+
+qk_status check_heads(const qk_kv_cache *c, size_t n_heads, size_t n_tokens) {
+    if (n_heads == 0 || n_heads % c->n_kv_heads != 0)
+        return qk::fail(QK_ERR_VALUE, "n_kv_heads must divide n_heads: n_heads=%zu, n_kv_heads=%zu", n_heads, c->n_kv_heads);
+    if (n_heads > 65535 || n_tokens > (1u << 24) || n_tokens * n_heads > 0x7fffffffull)
+        return qk::fail(QK_ERR_VALUE, "%zu tokens of %zu heads are more than one call takes", n_tokens, n_heads);
+    return QK_OK;
+}
+
+// A token's row of `width` values, `stride` to the next.
+qk_status check_rows(const char *what, const void *p, size_t stride, size_t width) {
+    if (!p) return qk::fail(QK_ERR_VALUE, "%s is null", what);
+    if (stride < width) return qk::fail(QK_ERR_VALUE, "%s: rows of %zu values cannot be %zu apart", what, width, stride);
+    return QK_OK;
+}
+
+qk_status enter(qk_ctx *ctx, qk_ctx **c) {
+    qk_status st = qk::resolve_ctx(ctx, c);
+    if (st != QK_OK) return st;
+    QK_CUDA(cudaSetDevice((*c)->device));
+    return QK_OK;
+}
+
+// The error word, which must exist before a capture begins.
+qk_status ready_error_word(qk_ctx *c) {
+    if (!c->d_err.ptr && qk::capturing(c))
+        return qk::fail(QK_ERR_VALUE, "qk_cache_check has to be called on this context before a stream capture");
+    return qk::error_word(c);
+}
+
+#define QK_PDL(c, kernel, grid, block, smem, ...) \
+    (void)qk::launch_pdl((c)->pdl, kernel, grid, block, smem, (c)->stream, __VA_ARGS__)
+
+qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, const qk::AttendArgs &a) {
+    qk_ctx *c;
+    DeviceGuard guard;
+    qk_status st = enter(ctx, &c);
+    if (st != QK_OK) return st;
+    std::lock_guard<std::mutex> lock(c->mu);
+    const CacheView own = view(cache), pre = view(a.prefix_len ? prefix : nullptr);
+    const unsigned blocks = (unsigned)qk::ceil_div((size_t)a.n_queries * a.n_heads, 4);
+    if (own.dtype == QK_I8) QK_PDL(c, attend_plain_kernel<int8_t>, dim3(blocks), dim3(128), 0, own, pre, a);
+    else if (own.dtype == QK_BF16) QK_PDL(c, attend_plain_kernel<uint16_t>, dim3(blocks), dim3(128), 0, own, pre, a);
+    else QK_PDL(c, attend_plain_kernel<float>, dim3(blocks), dim3(128), 0, own, pre, a);
+    QK_CUDA(cudaGetLastError());
+    c->launches++;
+    return QK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+qk_status qk_cache_check(qk_ctx *ctx, const qk_kv_cache *cache) {
+    qk_status st = check_cache(cache, "cache");
+    if (st != QK_OK) return st;
+    qk_ctx *c;
+    DeviceGuard guard;
+    if ((st = enter(ctx, &c)) != QK_OK) return st;
+    std::lock_guard<std::mutex> lock(c->mu);
+    return ready_error_word(c);
+}
+
+qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q, size_t q_stride, float *q_out,
+                          size_t q_out_stride, size_t n_heads, const float *k, size_t k_stride, const float *v,
+                          size_t v_stride, const float *cos_sin, size_t n_positions, const int32_t *positions,
+                          const int32_t *seq_index, size_t first_position, size_t n_tokens) {
+    qk_status st = check_cache(cache, "cache");
+    if (st != QK_OK) return st;
+    const size_t d = cache->head_dim, kv_width = cache->n_kv_heads * d;
+    if (q) {
+        if ((st = check_heads(cache, n_heads, n_tokens)) != QK_OK) return st;
+        if ((st = check_rows("q", q, q_stride, n_heads * d)) != QK_OK) return st;
+        if ((st = check_rows("q_out", q_out, q_out_stride, n_heads * d)) != QK_OK) return st;
+    } else if ((st = check_heads(cache, cache->n_kv_heads, n_tokens)) != QK_OK) {
+        return st;
+    }
+    if ((st = check_rows("k", k, k_stride, kv_width)) != QK_OK) return st;
+    if ((st = check_rows("v", v, v_stride, kv_width)) != QK_OK) return st;
+    if (!cos_sin || !positions || !seq_index) return qk::fail(QK_ERR_VALUE, "cos_sin, positions or seq_index is null");
+    if (first_position > 0x7fffffffull || n_positions > 0x7fffffffull)
+        return qk::fail(QK_ERR_VALUE, "positions are 32-bit: first_position %zu, n_positions %zu", first_position, n_positions);
+    qk_ctx *c;
+    DeviceGuard guard;
+    if ((st = enter(ctx, &c)) != QK_OK) return st;
+    if (n_tokens == 0) return QK_OK;
+    std::lock_guard<std::mutex> lock(c->mu);
+    if ((st = ready_error_word(c)) != QK_OK) return st;
+    const size_t rows = (q ? n_heads : 0) + 2 * cache->n_kv_heads;
+    const size_t most = qk::ceil_div(rows, 8), want = qk::ceil_div((size_t)c->sm_count * 4, n_tokens);
+    const dim3 grid((unsigned)n_tokens, (unsigned)std::min(most, want));
+    const CacheView cv = view(cache);
+    int *err = (int *)c->d_err.ptr;
+#define QK_APPEND(KV)                                                                                                          \
+    QK_PDL(c, append_kernel<KV>, grid, dim3(256), 0, cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, v, \
+           v_stride, cos_sin, (uint32_t)n_positions, positions, seq_index, (uint32_t)first_position, (uint32_t)n_tokens, err)
+    if (cv.dtype == QK_I8) QK_APPEND(int8_t);
+    else if (cv.dtype == QK_BF16) QK_APPEND(uint16_t);
+    else QK_APPEND(float);
+#undef QK_APPEND
+    QK_CUDA(cudaGetLastError());
+    c->launches++;
+    c->err_armed = true;
+    return QK_OK;
+}
+
+qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *positions, const int32_t *seq_index,
+                        size_t first_position, size_t n_tokens, int32_t out_dtype, void *k_out, void *v_out) {
+    qk_status st = check_cache(cache, "cache");
+    if (st != QK_OK) return st;
+    if ((st = check_heads(cache, cache->n_kv_heads, n_tokens)) != QK_OK) return st;
+    if (!positions || !seq_index || !k_out || !v_out)
+        return qk::fail(QK_ERR_VALUE, "positions, seq_index, k_out or v_out is null");
+    if (out_dtype != QK_F32 && out_dtype != QK_BF16)
+        return qk::fail(QK_ERR_VALUE, "rows are read as float32 or bfloat16, got tag %d", out_dtype);
+    if (first_position > 0x7fffffffull) return qk::fail(QK_ERR_VALUE, "positions are 32-bit: first_position %zu", first_position);
+    qk_ctx *c;
+    DeviceGuard guard;
+    if ((st = enter(ctx, &c)) != QK_OK) return st;
+    if (n_tokens == 0) return QK_OK;
+    std::lock_guard<std::mutex> lock(c->mu);
+    if ((st = ready_error_word(c)) != QK_OK) return st;
+    const unsigned blocks = (unsigned)qk::ceil_div(n_tokens * cache->n_kv_heads * 2, 8);
+    const CacheView cv = view(cache);
+    int *err = (int *)c->d_err.ptr;
+#define QK_READ(KV, Out)                                                                                                  \
+    QK_PDL(c, (read_kernel<KV, Out>), dim3(blocks), dim3(256), 0, cv, positions, seq_index, (uint32_t)first_position, \
+           (uint32_t)n_tokens, (Out *)k_out, (Out *)v_out, err)
+#define QK_READ_TO(Out)                                \
+    do {                                               \
+        if (cv.dtype == QK_I8) QK_READ(int8_t, Out);   \
+        else if (cv.dtype == QK_BF16) QK_READ(uint16_t, Out); \
+        else QK_READ(float, Out);                      \
+    } while (0)
+    if (out_dtype == QK_F32) QK_READ_TO(float);
+    else QK_READ_TO(uint16_t);
+#undef QK_READ_TO
+#undef QK_READ
+    QK_CUDA(cudaGetLastError());
+    c->launches++;
+    c->err_armed = true;
+    return QK_OK;
+}
+
+size_t qk_cache_attend_scratch(const qk_kv_cache *cache, size_t prefix_len, size_t batch, size_t n_heads) {
+    (void)cache, (void)prefix_len, (void)batch, (void)n_heads;
+    return 0;
+}
+
+qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, size_t prefix_seq,
+                          size_t prefix_len, const float *q, size_t q_stride, const int32_t *kv_len, size_t batch,
+                          size_t n_heads, void *scratch, float *out, size_t out_stride) {
+    qk_status st = check_cache(cache, "cache");
+    if (st != QK_OK) return st;
+    if ((st = check_prefix(cache, prefix, prefix_seq, prefix_len)) != QK_OK) return st;
+    if ((st = check_heads(cache, n_heads, batch)) != QK_OK) return st;
+    if (batch > cache->n_seq) return qk::fail(QK_ERR_VALUE, "%zu sequences, but the cache has %zu slots", batch, cache->n_seq);
+    if ((st = check_rows("q", q, q_stride, n_heads * cache->head_dim)) != QK_OK) return st;
+    if ((st = check_rows("out", out, out_stride, n_heads * cache->head_dim)) != QK_OK) return st;
+    if (!kv_len) return qk::fail(QK_ERR_VALUE, "kv_len is null");
+    if (!scratch && qk_cache_attend_scratch(cache, prefix_len, batch, n_heads))
+        return qk::fail(QK_ERR_VALUE, "scratch is null");
+    if (batch == 0) return QK_OK;
+    qk::AttendArgs a{};
+    a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride, a.kv_len = kv_len;
+    a.n_queries = (uint32_t)batch, a.n_heads = (uint32_t)n_heads;
+    a.prefix_len = (uint32_t)prefix_len, a.prefix_seq = prefix_seq;
+    a.scratch = (float *)scratch;
+    return attend(ctx, cache, prefix, a);
+}
+
+size_t qk_cache_portion_scratch(const qk_kv_cache *cache, size_t first_row, size_t prefix_len, size_t n_tokens,
+                                size_t n_heads) {
+    (void)cache, (void)first_row, (void)prefix_len, (void)n_tokens, (void)n_heads;
+    return 0;
+}
+
+qk_status qk_cache_portion(qk_ctx *ctx, const qk_kv_cache *cache, size_t seq, size_t first_row, const qk_kv_cache *prefix,
+                           size_t prefix_seq, size_t prefix_len, const float *q, size_t q_stride, size_t n_tokens,
+                           size_t n_heads, void *scratch, float *out, size_t out_stride) {
+    qk_status st = check_cache(cache, "cache");
+    if (st != QK_OK) return st;
+    if ((st = check_prefix(cache, prefix, prefix_seq, prefix_len)) != QK_OK) return st;
+    if ((st = check_heads(cache, n_heads, n_tokens)) != QK_OK) return st;
+    if (seq >= cache->n_seq) return qk::fail(QK_ERR_VALUE, "slot %zu outside the cache of %zu slots", seq, cache->n_seq);
+    if (first_row > cache->rows || n_tokens > cache->rows - first_row)
+        return qk::fail(QK_ERR_VALUE, "%zu tokens from row %zu on do not fit the cache of %zu rows", n_tokens, first_row, cache->rows);
+    if ((st = check_rows("q", q, q_stride, n_heads * cache->head_dim)) != QK_OK) return st;
+    if ((st = check_rows("out", out, out_stride, n_heads * cache->head_dim)) != QK_OK) return st;
+    if (!scratch && qk_cache_portion_scratch(cache, first_row, prefix_len, n_tokens, n_heads))
+        return qk::fail(QK_ERR_VALUE, "scratch is null");
+    if (n_tokens == 0) return QK_OK;
+    qk::AttendArgs a{};
+    a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride;
+    a.n_queries = (uint32_t)n_tokens, a.n_heads = (uint32_t)n_heads;
+    a.seq = seq, a.first_row = (uint32_t)first_row;
+    a.prefix_len = (uint32_t)prefix_len, a.prefix_seq = prefix_seq;
+    a.scratch = (float *)scratch;
+    return attend(ctx, cache, prefix, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,29 @@
+// What the kernels over key/value caches share: the cache as the device sees it, the arguments of an attention call.
+#pragma once
+
+#include "qk_common.h"
+
+namespace qk {
+
+struct CacheView {
+    void *k, *v;               // [n_seq][n_kv][rows][d]
+    float *k_scale, *v_scale;  // INT8: [n_seq][n_kv][rows]
+    uint32_t rows, n_seq, n_kv, d;
+    int32_t dtype;
+};
+
+struct AttendArgs {
+    const float *q;
+    size_t q_stride;
+    float *out;
+    size_t out_stride;
+    const int32_t *kv_len;     // one query per sequence: its rows; null: a portion, query t sees rows 0 .. first_row + t of `seq`
+    uint32_t n_queries, n_heads;
+    size_t seq;
+    uint32_t first_row;
+    uint32_t prefix_len;       // rows of the prefix's slot prefix_seq, seen by every query
+    size_t prefix_seq;
+    float *scratch;
+};
+
+}  // namespace qk

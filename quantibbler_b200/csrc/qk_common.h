@@ -152,6 +152,16 @@ cudaError_t launch_pdl(bool allow_overlap, void (*kernel)(KArgs...), dim3 grid, 
 }
 #endif
 
+// Puts the device that was current back at the end of a call.
+struct DeviceGuard {
+    int before = -1;
+    DeviceGuard() {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)cudaSetDevice(before);
+    }
+};
 // Returns the context to use for a call: `ctx` itself, or the process-wide default on
 // device 0 (created on first use) when `ctx` is null.
 qk_status resolve_ctx(qk_ctx *ctx, qk_ctx **out);

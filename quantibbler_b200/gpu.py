@@ -54,14 +54,15 @@ class GpuContext:
     ``gpu_init_hint()`` embedded.  Safe to share between host threads.
     """
 
-    def __init__(self, handle):
+    def __init__(self, handle, device_index: int = 0):
         self._h = handle
+        self.device_index = int(device_index)
 
     @classmethod
     def init_at(cls, device_index: int) -> "GpuContext":
         h = ctypes.c_void_p()
         check(_lib.lib().qk_gpu_init_at(int(device_index), ctypes.byref(h)))
-        return cls(h)
+        return cls(h, device_index)
 
     @classmethod
     def init(cls) -> "GpuContext":

@@ -1,0 +1,61 @@
+"""Log probabilities of given tokens, with the entropy of their distributions and the most probable entries."""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+from . import _lib
+from ._lib import KernelError, check
+from .cache import check_tensor, ordered
+from .gpu import GpuContext
+
+MAX_TOP = 32
+
+
+class LogProbs(NamedTuple):
+    """Per row of logits, on the device: ``lse`` (ln of the sum of exponentials), ``logprob`` of the target (None
+    without targets), ``entropy`` in nats, and the ``top`` most probable entries, ``top_ids`` (int32, ties: the
+    lowest id first) and ``top_logprob``."""
+    lse: object
+    logprob: object
+    entropy: object
+    top_logprob: object
+    top_ids: object
+
+
+def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
+    """``logits`` float32 ``[rows, vocab]``, rows possibly apart; ``targets`` int32 ``[rows]`` or None, a negative
+    one marks a row without a token (its logprob is 0).  A row that holds a NaN or +infinity, or nothing above
+    -infinity, gives NaN (its ids: -1); entries of -infinity are impossible ones.  Runs on the context's stream,
+    ordered with torch's current one."""
+    import torch
+    if logits.dim() != 2:
+        raise KernelError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    if logits.device.type != "cuda" or logits.device.index != ctx.device_index:
+        raise KernelError(f"logits are on {logits.device}, the context on cuda:{ctx.device_index}")
+    check_tensor("logits", logits, torch.float32, logits.device)
+    n, vocab = (int(v) for v in logits.shape)
+    if logits.stride(1) != 1 and vocab > 1:
+        raise KernelError(f"a row of logits must be contiguous, got strides {logits.stride()}")
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise KernelError(f"top must lie in 0 .. {min(MAX_TOP, vocab)}, got {top}")
+    if targets is not None:
+        check_tensor("targets", targets, torch.int32, logits.device, (n,))
+        if not targets.is_contiguous():
+            raise KernelError("targets must be contiguous")
+    dev, f32 = logits.device, torch.float32
+    # (one allocation for the float outputs: lse, entropy, logprob, top_logprob)
+    flat = torch.empty(n * (3 + top), dtype=f32, device=dev)
+    lse, entropy, logprob = flat[:n], flat[n:2 * n], flat[2 * n:3 * n]
+    top_logprob, top_ids = flat[3 * n:].view(n, top), torch.empty((n, top), dtype=torch.int32, device=dev)
+    lib = _lib.lib()
+    if n:
+        size = lib.qk_log_probs_scratch(n, vocab, top)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        with ordered(ctx, dev):
+            check(lib.qk_log_probs(ctx.handle, logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab,
+                                   None if targets is None else targets.data_ptr(), top,
+                                   None if scratch is None else scratch.data_ptr(), lse.data_ptr(),
+                                   None if targets is None else logprob.data_ptr(), entropy.data_ptr(),
+                                   top_logprob.data_ptr() if top else None, top_ids.data_ptr() if top else None))
+    return LogProbs(lse, None if targets is None else logprob, entropy, top_logprob, top_ids)
