@@ -4,11 +4,9 @@
 #include <cmath>
 
 #include "qk_cache.h"
-#include "qk_decoder_dev.cuh"
+#include "qk_cache_attend.cuh"
 
 namespace {
-
-using qk::CacheView;
 
 // ------------------------------------------------------------------ append
 // x / scale, rounded to the nearest integer (ties to even) as 64-bit arithmetic does it: the 32-bit quotient is
@@ -194,6 +192,109 @@ attend_plain_kernel(CacheView c, CacheView p, qk::AttendArgs a) {
     }
 }
 
+// ------------------------------------------------------------------ attention of few query rows
+// How a call is dealt out: blocks over the prefix first (all queries of a kv head in rows of eight, splits of the
+// prefix), then blocks over the sequences' own rows.  A split of a sequence's rows is the same part of every
+// sequence, so that unequal lengths keep all blocks at work.
+struct Plan {
+    uint32_t prefix_subs, prefix_splits, prefix_chunk, prefix_blocks;
+    uint32_t own_subs, own_splits, own_rows;  // own_rows: query rows of a block
+    uint32_t n_slots;                         // partial results per (query, head); 1: none, the output is written
+};
+
+template <bool kI8, int D>
+__global__ void __launch_bounds__(128, kI8 ? 3 : 2)
+attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    extern __shared__ __align__(16) uint8_t attend_smem[];
+    const uint32_t group = a.n_heads / c.n_kv, row_bytes = kI8 ? D : 2 * D;
+    Span s;
+    uint32_t id = blockIdx.x, kvh;
+    const CacheView *src;
+    size_t line;
+    if (id < pl.prefix_blocks) {
+        src = &p;
+        const uint32_t sub = id % pl.prefix_subs, split = id / pl.prefix_subs % pl.prefix_splits;
+        kvh = id / pl.prefix_subs / pl.prefix_splits;
+        line = (a.prefix_seq * p.n_kv + kvh) * p.rows;
+        s.begin = (int)(split * pl.prefix_chunk);
+        s.end = (int)min(a.prefix_len, (split + 1) * pl.prefix_chunk);
+        s.first_row = sub * 8;
+        s.n_rows = min(8u, a.n_queries * group - s.first_row);
+        s.slot = split;
+    } else {
+        id -= pl.prefix_blocks;
+        src = &c;
+        const uint32_t sub = id % pl.own_subs;
+        kvh = id / pl.own_subs % c.n_kv;
+        const uint32_t split = id / pl.own_subs / c.n_kv % pl.own_splits, b = id / pl.own_subs / c.n_kv / pl.own_splits;
+        line = ((size_t)b * c.n_kv + kvh) * c.rows;
+        const uint32_t len = (uint32_t)min(max(a.kv_len[b], 0), (int)c.rows);
+        const uint32_t chunk = ((len + pl.own_splits - 1) / pl.own_splits + 63) / 64 * 64;
+        s.begin = (int)min(len, split * chunk);
+        s.end = (int)min(len, (split + 1) * chunk);
+        s.first_row = b * group + sub * pl.own_rows;
+        s.n_rows = min(pl.own_rows, group - sub * pl.own_rows);
+        s.slot = pl.prefix_splits + split;
+    }
+    s.k = static_cast<const uint8_t *>(src->k) + line * row_bytes;
+    s.v = static_cast<const uint8_t *>(src->v) + line * row_bytes;
+    s.k_scale = kI8 ? src->k_scale + line : nullptr;
+    s.v_scale = kI8 ? src->v_scale + line : nullptr;
+    if (s.n_rows > 4) attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+    else attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+}
+
+// Partial results {maximum (log2 units), sum, output[d]} of a (query, head) joined.  A block of 128 threads each.
+constexpr uint32_t kMaxSlots = 256;
+
+__global__ void __launch_bounds__(128)
+join_kernel(const float *__restrict__ partial, qk::AttendArgs a, uint32_t n_slots, uint32_t d) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    __shared__ float weight[kMaxSlots], red[8];
+    const uint32_t query = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads, warp = threadIdx.x / 32;
+    const float *p = partial + (size_t)blockIdx.x * n_slots * (d + 2);
+    float m[kMaxSlots / 128], l[kMaxSlots / 128], top = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlots / 128; ++i) {
+        const uint32_t s = threadIdx.x + 128 * i;
+        m[i] = s < n_slots ? p[(size_t)s * (d + 2)] : -INFINITY;
+        l[i] = s < n_slots ? p[(size_t)s * (d + 2) + 1] : 0.f;
+        top = fmaxf(top, m[i]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (threadIdx.x % 32 == 0) red[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlots / 128; ++i) {
+        const uint32_t s = threadIdx.x + 128 * i;
+        // (a span without keys has the sum 0; a NaN stays)
+        const float w = m[i] == -INFINITY ? (l[i] == 0.f ? 0.f : 1.f) : ex2(m[i] - top);
+        if (s < n_slots) weight[s] = w;
+        sum = fmaf(l[i], w, sum);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (threadIdx.x % 32 == 0) red[4 + warp] = sum;
+    __syncthreads();
+    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (uint32_t c = threadIdx.x; c < d; c += 128) {
+        float v = 0.f;
+#pragma unroll 8
+        for (uint32_t s = 0; s < n_slots; ++s) {
+            const float w = weight[s];
+            if (w != 0.f) v = fmaf(p[(size_t)s * (d + 2) + 2 + c], w, v);
+        }
+        a.out[query * a.out_stride + (size_t)head * d + c] = v * inv;
+    }
+}
+
 // ------------------------------------------------------------------ host side
 using qk::DeviceGuard;
 
@@ -271,6 +372,54 @@ qk_status ready_error_word(qk_ctx *c) {
 #define QK_PDL(c, kernel, grid, block, smem, ...) \
     (void)qk::launch_pdl((c)->pdl, kernel, grid, block, smem, (c)->stream, __VA_ARGS__)
 
+// Whether attend_rows_kernel takes the shape.  (Rows on 16-byte boundaries are a matter of the pointers, below.)
+bool takes_rows(const qk_kv_cache *c) { return c->dtype != QK_F32 && (c->head_dim == 64 || c->head_dim == 128); }
+bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+bool aligned_rows(const CacheView &v) { return aligned(v.k) && aligned(v.v); }
+
+constexpr size_t kWantBlocks = 148 * 9, kMinChunk = 128;
+
+Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_heads) {
+    Plan pl{};
+    const size_t group = n_heads / c->n_kv_heads;
+    auto splits = [](size_t blocks, size_t rows) {
+        const size_t most = std::min<size_t>(128, qk::ceil_div(rows, kMinChunk));
+        return (uint32_t)std::max<size_t>(1, std::min(most, qk::ceil_div(kWantBlocks, blocks)));
+    };
+    if (prefix_len) {
+        pl.prefix_subs = (uint32_t)qk::ceil_div(batch * group, 8);
+        pl.prefix_splits = splits(pl.prefix_subs * c->n_kv_heads, prefix_len);
+        pl.prefix_chunk = (uint32_t)(qk::ceil_div(qk::ceil_div(prefix_len, pl.prefix_splits), 64) * 64);
+        pl.prefix_blocks = (uint32_t)(pl.prefix_subs * pl.prefix_splits * c->n_kv_heads);
+    }
+    pl.own_rows = (uint32_t)std::min<size_t>(group, 8);
+    pl.own_subs = (uint32_t)qk::ceil_div(group, pl.own_rows);
+    pl.own_splits = splits(batch * c->n_kv_heads * pl.own_subs, c->rows);
+    pl.n_slots = pl.prefix_splits + pl.own_splits;
+    return pl;
+}
+
+size_t partial_bytes(size_t queries, size_t n_heads, size_t slots, size_t d) {
+    return slots > 1 ? queries * n_heads * slots * (d + 2) * sizeof(float) : 0;
+}
+
+template <bool kI8, int D>
+qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, const qk::AttendArgs &a, const Plan &pl) {
+    constexpr size_t smem = AttendShape<kI8, D>::kSmem;
+    qk_status st = qk::allow_smem(c, attend_rows_kernel<kI8, D>, smem);
+    if (st != QK_OK) return st;
+    const unsigned blocks = pl.prefix_blocks + a.n_queries * own.n_kv * pl.own_subs * pl.own_splits;
+    QK_PDL(c, (attend_rows_kernel<kI8, D>), dim3(blocks), dim3(128), smem, own, pre, a, pl);
+    QK_CUDA(cudaGetLastError());
+    c->launches++;
+    if (pl.n_slots > 1) {
+        QK_PDL(c, join_kernel, dim3(a.n_queries * a.n_heads), dim3(128), 0, (const float *)a.scratch, a, pl.n_slots, own.d);
+        QK_CUDA(cudaGetLastError());
+        c->launches++;
+    }
+    return QK_OK;
+}
+
 qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, const qk::AttendArgs &a) {
     qk_ctx *c;
     DeviceGuard guard;
@@ -278,6 +427,13 @@ qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefi
     if (st != QK_OK) return st;
     std::lock_guard<std::mutex> lock(c->mu);
     const CacheView own = view(cache), pre = view(a.prefix_len ? prefix : nullptr);
+    if (a.kv_len && takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0 &&
+        (!a.scratch || aligned(a.scratch))) {
+        const Plan pl = plan_rows(cache, a.prefix_len, a.n_queries, a.n_heads);
+        if (own.dtype == QK_I8)
+            return own.d == 128 ? launch_rows<true, 128>(c, own, pre, a, pl) : launch_rows<true, 64>(c, own, pre, a, pl);
+        return own.d == 128 ? launch_rows<false, 128>(c, own, pre, a, pl) : launch_rows<false, 64>(c, own, pre, a, pl);
+    }
     const unsigned blocks = (unsigned)qk::ceil_div((size_t)a.n_queries * a.n_heads, 4);
     if (own.dtype == QK_I8) QK_PDL(c, attend_plain_kernel<int8_t>, dim3(blocks), dim3(128), 0, own, pre, a);
     else if (own.dtype == QK_BF16) QK_PDL(c, attend_plain_kernel<uint16_t>, dim3(blocks), dim3(128), 0, own, pre, a);
@@ -383,8 +539,8 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
 }
 
 size_t qk_cache_attend_scratch(const qk_kv_cache *cache, size_t prefix_len, size_t batch, size_t n_heads) {
-    (void)cache, (void)prefix_len, (void)batch, (void)n_heads;
-    return 0;
+    if (!cache || cache->n_kv_heads == 0 || n_heads < cache->n_kv_heads || !batch || !takes_rows(cache)) return 0;
+    return partial_bytes(batch, n_heads, plan_rows(cache, prefix_len, batch, n_heads).n_slots, cache->head_dim);
 }
 
 qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, size_t prefix_seq,

@@ -1,0 +1,429 @@
+// Attention of few query rows over INT8 and bfloat16 cache rows (a step of a batch; a prefix for small batches).
+//
+// Up to eight query rows that read the same kv head go through a span of keys together; four warps of a block
+// take 16 keys at a time in turn, each through a ring of its own in shared memory (cp.async), with a running
+// maximum and sum per row.  The keys are the M side of the scores' product and the channels that of the output's,
+// (query row, term) the N side: a pair of accumulator columns is one row's leading and second term, so a thread
+// (g, t) holds the scores of keys g and g + 8 for row t and, later, channels of the same row t; the weights turn
+// into the second product's B fragment by one transposition of an 8 x 8 matrix (movmatrix).
+//
+// Exactness.  INT8: the codes are the A operand of the integer product as they lie; q is 23-bit fixed point in
+// three 8-bit digits, so a score is exact but for q's rounding (2^-22 of its largest entry) and one float32
+// rounding.  The weights times the value scales are two float16 terms (22 bits), scaled to 2^14; codes as float16
+// are exact.  The scales are taken relative to a power of two at their running maximum E, so nothing leaves
+// float16's range.  bfloat16: q and the weights are three bfloat16 terms.  A step's output product starts from
+// zero and is added to the running sum by float32 arithmetic: the tensor core truncates.
+//
+// What bounds it: the cache's bytes.
+#pragma once
+
+#include "qk_cache.h"
+#include "qk_mma.cuh"
+
+namespace {
+
+using qk::CacheView;
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kWeightScale = 16384.f;  // weights enter the float16 product times this
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ int exponent_of(float magnitude) {  // clamped to -100 .. 126
+    return min(126, max(-100, (int)(__float_as_uint(magnitude) >> 23) - 127));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {  // an 8 x 8 matrix of 16-bit values
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void copy4(void *smem, const void *gmem, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem),
+                 "r"(bytes)
+                 : "memory");
+}
+// {hi, lo} of a weight as two float16 in one word, hi below.
+__device__ __forceinline__ uint32_t weight_terms(float w) {
+    uint32_t hi, r;
+    float back;
+    asm("{\n .reg .b16 h;\n cvt.rn.f16.f32 h, %2;\n cvt.f32.f16 %1, h;\n mov.b32 %0, {h, h};\n}" : "=r"(hi), "=f"(back) : "f"(w));
+    asm("{\n .reg .b16 l, h, x;\n mov.b32 {h, x}, %1;\n cvt.rn.f16.f32 l, %2;\n mov.b32 %0, {h, l};\n}"
+        : "=r"(r)
+        : "r"(hi), "f"(w - back));
+    return r;
+}
+// Codes of byte `i` of two words (biased by 128) as a pair of float16: 1024 + u is the bit pattern 0x6400 | u.
+__device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b, int i) {
+    uint32_t w = __byte_perm(a, b, (4 + i) << 4 | i);  // bytes 0 and 1; then 16 bits apart
+    w = __byte_perm(w, 0x64646464u, 0x4140);
+    uint32_t r;
+    asm("{\n .reg .b32 c;\n mov.b32 c, 0x64806480;\n sub.rn.f16x2 %0, %1, c;\n}" : "=r"(r) : "r"(w));
+    return r;
+}
+
+// What a block works on: its query rows and its span of keys.
+struct Span {
+    const void *k, *v;              // the kv head's rows, from row 0
+    const float *k_scale, *v_scale;
+    int begin, end;                 // rows
+    uint32_t first_row, n_rows;     // query rows: row r is query (first_row + r) / group, head (first_row + r) % group of the kv head
+    uint32_t slot;                  // where the partial result goes
+};
+
+template <bool kI8, int D>
+struct AttendShape {
+    static constexpr int kRowBytes = kI8 ? D : 2 * D, kPieces = kRowBytes / 16;
+    static constexpr int kStageBytes = 2 * 16 * kRowBytes + (kI8 ? 128 : 0);
+    static constexpr int kStages = kI8 ? 4 : 3;
+    static constexpr int kWarpBytes = kStages * kStageBytes;
+    static constexpr int kSmem = 4 * kWarpBytes;
+    static_assert(kWarpBytes >= (8 * D + 16) * 4, "a warp's results lie in its ring");
+    // (pieces of 16 bytes of a row change places so that fragment loads meet no bank twice)
+    __device__ static uint32_t swizzle(uint32_t row, uint32_t piece) {
+        return row * kRowBytes + ((piece ^ (kPieces >= 8 ? row & 7 : (row >> 1) & (kPieces - 1))) << 4);
+    }
+};
+
+// kTiles: column tiles of query rows, four rows each.
+template <bool kI8, int D, int kTiles>
+__device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &a, uint32_t kvh, uint32_t n_kv, uint32_t n_slots,
+                                            uint8_t *smem) {
+    using Shape = AttendShape<kI8, D>;
+    constexpr int kRowBytes = Shape::kRowBytes, kPieces = Shape::kPieces, kStages = Shape::kStages;
+    constexpr int kQTiles = kTiles + 1;                              // column tiles of q: (first, second) term per row, then the thirds
+    constexpr int kSteps = D / (kI8 ? 32 : 16);                      // of the scores' contraction
+    constexpr int kOut = D / 16;                                     // channel tiles
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+    const uint32_t group = a.n_heads / n_kv;
+    uint8_t *ring = smem + warp * Shape::kWarpBytes;
+    const uint8_t *kb = static_cast<const uint8_t *>(s.k), *vb = static_cast<const uint8_t *>(s.v);
+
+    auto fetch = [&](int j, int stage) {
+        uint8_t *dst = ring + stage * Shape::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < 16 * kPieces / 32; ++i) {
+            const uint32_t idx = lane + 32 * i, key = idx / kPieces, piece = idx % kPieces;
+            const bool live = j + (int)key < s.end;
+            const size_t at = (size_t)(live ? j + key : s.end - 1) * kRowBytes + piece * 16;
+            const uint32_t to = Shape::swizzle(key, piece);
+            copy16(dst + to, kb + at, live ? 16u : 0u);
+            copy16(dst + 16 * kRowBytes + to, vb + at, live ? 16u : 0u);
+        }
+        if (kI8) {
+            const uint32_t key = lane % 16;
+            const bool live = j + (int)key < s.end;
+            copy4(dst + 2 * 16 * kRowBytes + lane * 4, (lane < 16 ? s.k_scale : s.v_scale) + (live ? j + key : s.end - 1),
+                  live ? 4u : 0u);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    constexpr int kStride = 64;
+    const int j_first = s.begin + 16 * (int)warp;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+        if (j_first + i * kStride < s.end) fetch(j_first + i * kStride, i);
+
+    // ---- q as B fragments.  Column g of tile n: tile n < kTiles: row 4 n + g / 2, term g % 2; the last: thirds
+    uint32_t qf[kQTiles][kSteps][2];
+    float f[kTiles];  // what turns a score's sum into log2 units, row 4 n + t
+    const float unit = kLog2E / sqrtf((float)D);
+    auto q_row = [&](uint32_t r) {
+        const uint32_t row = s.first_row + min(r, s.n_rows - 1);
+        return a.q + (row / group) * a.q_stride + (size_t)(kvh * group + row % group) * D;
+    };
+#pragma unroll
+    for (int n = 0; n < kQTiles; ++n) {
+        const bool third = n >= kTiles;
+        const uint32_t r = third ? 4 * (g % 2) + g / 2 : 4 * n + g / 2;
+        const int term = third ? 2 : (int)(g % 2);
+        const bool live = r < s.n_rows && r < 4 * kTiles;
+        const float *src = q_row(r);
+        if (kI8) {
+            float x[D / 4];
+            float peak = 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {  // lane t: pieces of 16 channels 2t, 2t + 1 (D 128), t (D 64)
+                const uint32_t c = (D == 128 ? 2 * t : t) * 16 + i * 4;
+                const float4 v4 = *reinterpret_cast<const float4 *>(src + c);
+                x[4 * i] = v4.x, x[4 * i + 1] = v4.y, x[4 * i + 2] = v4.z, x[4 * i + 3] = v4.w;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                peak = fmaxf(peak, fabsf(x[i]));
+                finite = finite && fabsf(x[i]) < INFINITY;
+            }
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+            const int e = exponent_of(peak);
+            const float mul = pow2(21 - e);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    int v = live ? __float2int_rn(x[4 * i + b] * mul) : 0;
+                    const int d0 = (int)(int8_t)v;
+                    v = (v - d0) >> 8;
+                    const int d1 = (int)(int8_t)v;
+                    const int d2 = (v - d1) >> 8;
+                    word |= (uint32_t)((term == 0 ? d2 : term == 1 ? d1 : d0) & 0xff) << (8 * b);
+                }
+                qf[n][i / 2][i % 2] = word;
+            }
+            // row 4 n + t's factor: from the lanes of column 2 t
+            unsigned ok = __ballot_sync(0xffffffffu, finite);
+            if (!third) {
+                const int e_t = __shfl_sync(0xffffffffu, e, 8 * t);
+                f[n < kTiles ? n : 0] = (ok >> (8 * t) & 0xf) == 0xf ? pow2(e_t - 21) * unit : __int_as_float(0x7fffffff);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {  // pieces of 8 channels: 2t, 2t + 1, then 8 further on
+                const uint32_t c = (2 * t + (i % 2) + 8 * (i / 2)) * 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 v4 = *reinterpret_cast<const float4 *>(src + c + 4 * h);
+                    uint32_t w0[3], w1[3];
+                    split3(live ? v4.x : 0.f, live ? v4.y : 0.f, w0);
+                    split3(live ? v4.z : 0.f, live ? v4.w : 0.f, w1);
+                    qf[n][2 * i + h][0] = term == 0 ? w0[0] : term == 1 ? w0[1] : w0[2];
+                    qf[n][2 * i + h][1] = term == 0 ? w1[0] : term == 1 ? w1[1] : w1[2];
+                }
+            }
+            if (!third) f[n < kTiles ? n : 0] = unit;
+        }
+    }
+
+    float o[kTiles][kOut][2], m[kTiles], l[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) o[n][i][0] = o[n][i][1] = 0.f;
+    }
+    int e_max = -100;  // exponent of the largest value scale so far
+
+    int stage = 0;
+    for (int j = j_first; j < s.end; j += kStride, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        if (j + (kStages - 1) * kStride < s.end) {
+            fetch(j + (kStages - 1) * kStride, (stage + kStages - 1) % kStages);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        } else if (kStages > 3 && j + 2 * kStride < s.end) {
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+        } else if (j + kStride < s.end) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncwarp();
+        const uint8_t *kt = ring + stage * Shape::kStageBytes, *vt = kt + 16 * kRowBytes;
+
+        // ---- scores of keys g and g + 8
+        float x[kTiles][2];
+        float vs[2];
+        if (kI8) {
+            int acc[kQTiles][4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const uint32_t piece = D == 128 ? 2 * t + i : t;
+                const uint4 lo = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g, piece));
+                const uint4 hi = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g + 8, piece));
+                const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+                for (int n = 0; n < kQTiles; ++n) {
+                    mma_s8(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
+                    mma_s8(acc[n], a1, qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
+                }
+            }
+            const float *sc = reinterpret_cast<const float *>(kt + 2 * 16 * kRowBytes);
+            vs[0] = sc[16 + g], vs[1] = sc[24 + g];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // (thirds: columns 2 t and 2 t + 1 of the last tile are rows t and 4 + t)
+                    const int low = acc[n][2 * h + 1] * 256 + acc[kTiles][2 * h + n];
+                    x[n][h] = fmaf((float)acc[n][2 * h], 65536.f, (float)low) * f[n] * sc[8 * h + g];
+                }
+        } else {
+            float acc[kQTiles][4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const uint32_t piece = 2 * t + (i % 2) + 8 * (i / 2);
+                const uint4 lo = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g, piece));
+                const uint4 hi = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g + 8, piece));
+                const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+                for (int n = 0; n < kQTiles; ++n) {
+                    mma16(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
+                    mma16(acc[n], a1, qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
+                }
+            }
+            vs[0] = vs[1] = 1.f;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    x[n][h] = (acc[n][2 * h] + (acc[n][2 * h + 1] + acc[kTiles][2 * h + n])) * f[n];
+        }
+        if (j + 16 > s.end) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (j + (int)g + 8 * h >= s.end) x[n][h] = -INFINITY;
+        }
+        // ---- the value scales' common power of two
+        float shrink = 1.f, vmul = 1.f;
+        if (kI8) {
+            const uint32_t bits = max(__float_as_uint(fabsf(vs[0])), __float_as_uint(fabsf(vs[1])));
+            const int e_new = max(e_max, min(125, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, bits)))));
+            shrink = pow2(max(-126, e_max - e_new));
+            e_max = e_new;
+            vmul = pow2(-1 - e_new);
+            vs[0] *= vmul, vs[1] *= vmul;
+        }
+        // ---- running maximum and sum, weights as terms
+        uint32_t pf[kI8 ? kTiles : kQTiles][2];
+        float alpha[kTiles];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            float mx = fmaxf(x[n][0], x[n][1]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m[n], mx), base = m_new == -INFINITY ? 0.f : m_new;
+            alpha[n] = ex2(m[n] - base);
+            m[n] = m_new;
+            const float p0 = ex2(x[n][0] - base), p1 = ex2(x[n][1] - base);
+            l[n] = fmaf(l[n], alpha[n], p0 + p1);
+            alpha[n] *= shrink;
+            if (kI8) {
+                pf[n][0] = transposed(weight_terms(p0 * vs[0] * kWeightScale));
+                pf[n][1] = transposed(weight_terms(p1 * vs[1] * kWeightScale));
+            } else {
+                uint32_t w[3];
+                split3(p0, p1, w);  // (key g below, key g + 8 above)
+                pf[n][0] = transposed(__byte_perm(w[0], w[1], 0x5410));
+                pf[n][1] = transposed(__byte_perm(w[0], w[1], 0x7632));
+                if (n == 0) x[0][0] = __uint_as_float(w[2]);
+                else x[0][1] = __uint_as_float(w[2]);
+            }
+        }
+        if (!kI8) {  // thirds of rows t and 4 + t side by side
+            const uint32_t w0 = __float_as_uint(x[0][0]), w1 = kTiles > 1 ? __float_as_uint(x[0][1]) : 0u;
+            pf[kQTiles - 1][0] = transposed(__byte_perm(w0, w1, 0x5410));
+            pf[kQTiles - 1][1] = transposed(__byte_perm(w0, w1, 0x7632));
+        }
+        // ---- output: channels are the M side
+        if (kI8) {
+            uint32_t vw[4][D / 32];  // keys 2t, 2t + 1, 2t + 8, 2t + 9: channels (D / 8) g ..
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t key = 2 * t + (r & 1) + 8 * (r >> 1);
+                if constexpr (D == 128) {
+                    const uint4 v4 = *reinterpret_cast<const uint4 *>(vt + Shape::swizzle(key, g));
+                    vw[r][0] = v4.x, vw[r][1] = v4.y, vw[r][2] = v4.z, vw[r][3] = v4.w;
+                } else {
+                    const uint2 v2 = *reinterpret_cast<const uint2 *>(vt + Shape::swizzle(key, g / 2) + 8 * (g % 2));
+                    vw[r][0] = v2.x, vw[r][1] = v2.y;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) vw[r][i] ^= 0x80808080u;
+            }
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {  // rows g, g + 8 of tile i: channels (D / 8) g + 2 i, + 1
+                const int w = i / 2, b = 2 * (i % 2);
+                const uint32_t af[4] = {code_pair(vw[0][w], vw[1][w], b), code_pair(vw[0][w], vw[1][w], b + 1),
+                                        code_pair(vw[2][w], vw[3][w], b), code_pair(vw[2][w], vw[3][w], b + 1)};
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(c, af, pf[n][0], pf[n][1]);
+                    o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + c[1]);
+                    o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + c[3]);
+                }
+            }
+        } else {
+            const uint32_t v_addr = (uint32_t)__cvta_generic_to_shared(vt);
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {  // rows g, g + 8 of tile i: channels 16 i + g, 16 i + 8 + g
+                uint32_t af[4];
+                const uint32_t key = (lane & 7) + 8 * (lane >> 4), piece = 2 * i + ((lane >> 3) & 1);
+                ldsm4_trans(af, v_addr + Shape::swizzle(key, piece));
+                float third[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16(third, af, pf[kQTiles - 1][0], pf[kQTiles - 1][1]);
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16(c, af, pf[n][0], pf[n][1]);
+                    o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + (c[1] + third[n]));
+                    o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + (c[3] + third[2 + n]));
+                }
+            }
+        }
+        __syncwarp();  // the stage may be filled again
+    }
+
+    // ---- the block's warps join: [row][D] outputs, then maxima and sums, each in its warp's ring
+    const float undo = kI8 ? pow2(min(127, e_max + 1)) * (1.f / kWeightScale) : 1.f;
+    float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+        const uint32_t r = 4 * n + t;
+        if (g == 0) mine[8 * D + r] = m[n], mine[8 * D + 8 + r] = l[n];
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                mine[r * D + (kI8 ? (D / 8) * g + 2 * i + h : 16 * i + 8 * h + g)] = o[n][i][h] * undo;
+    }
+    __syncthreads();
+    for (uint32_t at = threadIdx.x; at < s.n_rows * D; at += 128) {
+        const uint32_t r = at / D, c = at % D;
+        float mw[4], top = -INFINITY, sum = 0.f, val = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            mw[w] = reinterpret_cast<const float *>(smem + w * Shape::kWarpBytes)[8 * D + r];
+            top = fmaxf(top, mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float *src = reinterpret_cast<const float *>(smem + w * Shape::kWarpBytes);
+            // (a warp without keys has nothing; NaN sums stay)
+            const float weight = mw[w] == -INFINITY ? (src[8 * D + 8 + r] == 0.f ? 0.f : 1.f) : ex2(mw[w] - top);
+            sum = fmaf(src[8 * D + 8 + r], weight, sum);
+            val = fmaf(src[r * D + c], weight, val);
+        }
+        const uint32_t row = s.first_row + r, query = row / group, head = kvh * group + row % group;
+        if (n_slots == 1) {
+            a.out[query * a.out_stride + (size_t)head * D + c] = sum == 0.f ? 0.f : val / sum;
+        } else {
+            float *p = a.scratch + (((size_t)query * a.n_heads + head) * n_slots + s.slot) * (D + 2);
+            p[2 + c] = val;
+            if (c == 0) p[0] = top, p[1] = sum;
+        }
+    }
+}
+
+}  // namespace
