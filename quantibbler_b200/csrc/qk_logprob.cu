@@ -1,93 +1,323 @@
 // Log probabilities, entropy and the most probable entries from logits.
+//
+// One pass over a row: every thread keeps a running maximum m, the sum S of e^(x - m) and T of (x - m) e^(x - m);
+// then lse = m + ln S, ln p = (x - m) - ln S, entropy = ln S - T / S (both terms are positive: nothing cancels).
+// The most probable entries are 64-bit keys of (value, index) whose order is the wanted one, held by a warp, lane i
+// the i-th best; lists are sorted and merged by bitonic networks across the warp.
+//
+// What bounds it: the logits' bytes.  A row is cut into slices where there are fewer rows than blocks fit the
+// device; a second kernel joins the slices of a row.
+#include <algorithm>
 #include <cmath>
 
 #include "qk_common.h"
 
 namespace {
 
-constexpr uint32_t kMaxTop = 32;
+constexpr uint32_t kMaxTop = 32, kThreads = 256, kWarps = kThreads / 32;
+constexpr uint32_t kMinSlice = 2048;   // entries a block takes at least
+constexpr uint32_t kHeld = 8;          // vectors of four entries that a thread keeps in registers
+constexpr uint32_t kCandidates = 256;  // places for entries that may be among the best of a slice
+constexpr uint32_t kWantBlocks = 148 * 8;
+constexpr float kLog2E = 1.4426950408889634f;
 
 struct LogProbArgs {
     const float *logits;
     size_t stride;
-    uint32_t n_tokens, vocab, n_top;
+    uint32_t n_tokens, vocab, n_top, n_slices, slice;
     const int32_t *targets;
     float *lse, *logprob, *entropy, *top_logprob;
     int32_t *top_ids;
+    float *stats;    // [n_tokens][n_slices][4]: m, S, T; where n_slices > 1
+    uint64_t *keys;  // [n_tokens][n_slices][32]; where also n_top > 0
 };
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // An order on (value, index) as one number: larger is better, the lowest index first among equals (0 and -0 are).
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
     const uint32_t u = __float_as_uint(x + 0.f);
     return ((uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | (0xffffffffu - index);
 }
-
-__device__ __forceinline__ float block_reduce(float v, bool is_max, float *red) {
-    for (int off = 16; off > 0; off >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, v, off);
-        v = is_max ? fmaxf(v, o) : v + o;
-    }
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = red[0];
-    for (uint32_t w = 1; w < blockDim.x / 32; ++w) v = is_max ? fmaxf(v, red[w]) : v + red[w];
-    __syncthreads();
-    return v;
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-__global__ void __launch_bounds__(256)
-log_probs_plain_kernel(LogProbArgs a) {
+// Lane i keeps the larger (keep_max) or smaller of its and its partner's key.
+__device__ __forceinline__ uint64_t exchanged(uint64_t key, int partner_bit, bool keep_max) {
+    const uint64_t other = __shfl_xor_sync(0xffffffffu, key, partner_bit);
+    return (key > other) == keep_max ? key : other;
+}
+// 32 keys in falling order over the lanes.
+__device__ __forceinline__ uint64_t sorted(uint64_t key, uint32_t lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int bit = size / 2; bit > 0; bit /= 2)
+            key = exchanged(key, bit, ((lane & bit) == 0) == ((lane & size) == 0 || size == 32));
+    return key;
+}
+// The best 32 of two lists in falling order, in falling order: the larger of a and the reversed b is a bitonic sequence.
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b, uint32_t lane) {
+    const uint64_t r = __shfl_xor_sync(0xffffffffu, b, 31);
+    uint64_t key = a > r ? a : r;
+#pragma unroll
+    for (int bit = 16; bit > 0; bit /= 2) key = exchanged(key, bit, (lane & bit) == 0);
+    return key;
+}
+
+struct Stats {  // m, S = sum e^(x - m), T = sum (x - m) e^(x - m)
+    float m, s, t;
+};
+// Two disjoint parts of a row as one.
+__device__ __forceinline__ Stats joined(Stats a, Stats b) {
+    const float m = fmaxf(a.m, b.m);
+    if (!(m > -INFINITY)) return {m, a.s + b.s, a.t + b.t};  // (nothing possible in either; a NaN stays)
+    const float da = a.m - m, db = b.m - m, wa = ex2(da * kLog2E), wb = ex2(db * kLog2E);
+    Stats r{m, a.s * wa + b.s * wb, 0.f};
+    r.t = (wa > 0.f ? wa * (a.t + da * a.s) : 0.f) + (wb > 0.f ? wb * (b.t + db * b.s) : 0.f);
+    return r;
+}
+
+// A row's results from its statistics and its best entries (held by the lanes of one warp).
+__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, Stats st, uint64_t best, uint32_t lane) {
+    const float *x = a.logits + row * a.stride;
+    const float nan = __int_as_float(0x7fffffff);
+    // (an infinity makes the sums NaN, a NaN too)
+    const bool ok = st.m > -INFINITY && st.s < INFINITY && st.t > -INFINITY;
+    const float ln = logf(st.s);
+    if (lane == 0) {
+        if (a.lse) a.lse[row] = ok ? st.m + ln : nan;
+        if (a.entropy) a.entropy[row] = ok ? ln - st.t / st.s : nan;
+        if (a.logprob) {
+            const int32_t id = a.targets[row];
+            a.logprob[row] = id < 0 ? 0.f : !ok || (uint32_t)id >= a.vocab ? nan : (x[id] - st.m) - ln;
+        }
+    }
+    if (lane < a.n_top) {
+        const size_t at = (size_t)row * a.n_top + lane;
+        if (a.top_ids) a.top_ids[at] = ok ? (int32_t)key_index(best) : -1;
+        if (a.top_logprob) a.top_logprob[at] = ok ? (key_value(best) - st.m) - ln : nan;
+    }
+}
+
+// A thread's statistics of values in registers; the block's in shared memory.
+__device__ __forceinline__ void share(Stats st, Stats *part) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+        st = joined(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, off), __shfl_xor_sync(0xffffffffu, st.s, off),
+                              __shfl_xor_sync(0xffffffffu, st.t, off)});
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = st;
+}
+__device__ __forceinline__ Stats of_block(const Stats *part) {
+    Stats st = part[0];
+    for (uint32_t w = 1; w < kWarps; ++w) st = joined(st, part[w]);
+    return st;
+}
+
+// Where a slice's 16-byte vectors lie: up to three single entries in front, up to three behind.
+struct Extent {
+    uint32_t lo, hi, head, vectors, tail;
+    __device__ __forceinline__ Extent(const float *x, const LogProbArgs &a, uint32_t slice) {
+        lo = slice * a.slice, hi = min(a.vocab, lo + a.slice);
+        head = min(hi - lo, (uint32_t)((16 - ((uintptr_t)(x + lo) & 15)) & 15) / 4);
+        vectors = (hi - lo - head) / 4, tail = hi - lo - head - 4 * vectors;
+    }
+    // The single entry of this thread (threads 0 .. 2 and 8 .. 10), or none.
+    __device__ __forceinline__ uint32_t single() const {
+        return threadIdx.x < head ? lo + threadIdx.x
+                                  : threadIdx.x >= 8 && threadIdx.x - 8 < tail ? hi - tail + threadIdx.x - 8 : 0xffffffffu;
+    }
+};
+
+// Statistics alone: a slice of any length per block, streamed.
+__global__ void __launch_bounds__(kThreads)
+log_probs_kernel(LogProbArgs a) {
     qk::pdl_launch();
     qk::pdl_wait();
-    __shared__ float red[8];
-    __shared__ unsigned long long best;
-    const uint32_t t = blockIdx.x;
-    const float *x = a.logits + t * a.stride;
-    float m = -INFINITY, bad = 0.f;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += 256) {
-        m = fmaxf(m, x[i]);
-        if (!(x[i] < INFINITY)) bad = 1.f;
+    __shared__ Stats part[kWarps];
+    const uint32_t row = blockIdx.x / a.n_slices, slice = blockIdx.x % a.n_slices;
+    const float *x = a.logits + row * a.stride;
+    const Extent ext(x, a, slice);
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    auto take = [&](float v0, float v1, float v2, float v3) {
+        const float top = fmaxf(fmaxf(v0, v1), fmaxf(v2, v3));
+        if (top > m) {
+            if (m > -INFINITY) {
+                const float d = m - top, w = ex2(d * kLog2E);
+                t = w > 0.f ? w * fmaf(d, s, t) : 0.f;
+                s *= w;
+            }
+            m = top;
+        }
+        const float base = m > -INFINITY ? m : 0.f;
+        const float v[4] = {v0, v1, v2, v3};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (the difference first: its rounding counts for this entry alone)
+            const float d = v[e] - base, w = ex2(d * kLog2E);
+            s += w;
+            t = w == 0.f ? t : fmaf(d, w, t);
+        }
+    };
+    const float4 *xv = reinterpret_cast<const float4 *>(x + ext.lo + ext.head);
+    constexpr uint32_t kAhead = 4;
+    uint32_t i = threadIdx.x;
+    for (; i + (kAhead - 1) * kThreads < ext.vectors; i += kAhead * kThreads) {
+        float4 v[kAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) v[u] = __ldg(xv + i + u * kThreads);
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) take(v[u].x, v[u].y, v[u].z, v[u].w);
     }
-    m = block_reduce(m, true, red);
-    bad = block_reduce(bad, true, red);
-    float s = 0.f, w = 0.f;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += 256) {
-        const float y = x[i] - m, e = expf(y);
-        s += e;
-        w += e == 0.f ? 0.f : y * e;
+    for (; i < ext.vectors; i += kThreads) {
+        const float4 v = __ldg(xv + i);
+        take(v.x, v.y, v.z, v.w);
     }
-    s = block_reduce(s, false, red);
-    w = block_reduce(w, false, red);
-    const float nan = __int_as_float(0x7fffffff);
-    const bool ok = bad == 0.f && m > -INFINITY;
-    const float ln = logf(s);
-    if (threadIdx.x == 0) {
-        if (a.lse) a.lse[t] = ok ? m + ln : nan;
-        if (a.entropy) a.entropy[t] = ok ? ln - w / s : nan;
-        if (a.logprob) {
-            const int32_t id = a.targets ? a.targets[t] : -1;
-            a.logprob[t] = id < 0 ? 0.f : !ok || (uint32_t)id >= a.vocab ? nan : (x[id] - m) - ln;
+    const uint32_t single = ext.single();
+    if (single != 0xffffffffu) take(x[single], -INFINITY, -INFINITY, -INFINITY);
+    share(Stats{m, s, t}, part);
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const Stats st = of_block(part);
+    if (a.n_slices == 1) finish(a, row, st, 0, threadIdx.x);
+    else if (threadIdx.x == 0) *reinterpret_cast<float4 *>(a.stats + (size_t)blockIdx.x * 4) = make_float4(st.m, st.s, st.t, 0.f);
+}
+
+// With the most probable entries: a slice of at most 32 entries a thread (and a single one) stays in registers.  The
+// n_top-th largest of a warp's 32 thread maxima is no better than the slice's n_top-th entry; the best such bound of
+// the warps leaves a few dozen candidates, which one warp sorts.  (Sorting whatever beats a running last place,
+// warp by warp, took 93 us on 64 rows of 128256 with 20 places.)
+__global__ void __launch_bounds__(kThreads)
+log_probs_top_kernel(LogProbArgs a) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    __shared__ Stats part[kWarps];
+    __shared__ uint64_t bound_of[kWarps], candidates[kCandidates];
+    __shared__ uint64_t best_of[kWarps][32];
+    __shared__ uint32_t n_candidates;
+    const uint32_t row = blockIdx.x / a.n_slices, slice = blockIdx.x % a.n_slices;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float *x = a.logits + row * a.stride;
+    const Extent ext(x, a, slice);
+    const float4 *xv = reinterpret_cast<const float4 *>(x + ext.lo + ext.head);
+    const uint32_t first = ext.lo + ext.head, single = ext.single();
+    if (threadIdx.x == 0) n_candidates = 0;
+    float v[kHeld * 4 + 1];
+#pragma unroll
+    for (uint32_t u = 0; u < kHeld; ++u) {
+        const uint32_t i = threadIdx.x + u * kThreads;
+        const float4 w = i < ext.vectors ? __ldg(xv + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        v[4 * u] = w.x, v[4 * u + 1] = w.y, v[4 * u + 2] = w.z, v[4 * u + 3] = w.w;
+    }
+    v[kHeld * 4] = single != 0xffffffffu ? x[single] : -INFINITY;
+    // (entries past the slice are -infinity too, but `there` tells them apart)
+    auto index_of = [&](uint32_t i) { return i == kHeld * 4 ? single : first + 4 * (threadIdx.x + i / 4 * kThreads) + i % 4; };
+    auto there = [&](uint32_t i) { return i == kHeld * 4 ? single != 0xffffffffu : threadIdx.x + i / 4 * kThreads < ext.vectors; };
+    float m = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i <= kHeld * 4; ++i) m = fmaxf(m, v[i]);
+    float s = 0.f, t = 0.f;
+    const float base = m > -INFINITY ? m : 0.f;
+    uint64_t mine = 0;  // the thread's best entry (its lowest index is taken: the single one may lie in front of or behind the others)
+#pragma unroll
+    for (uint32_t i = 0; i <= kHeld * 4; ++i) {
+        const float d = v[i] - base, w = ex2(d * kLog2E);
+        s += w;
+        t = w == 0.f ? t : fmaf(d, w, t);
+        if (v[i] == m && there(i)) {
+            const uint64_t key = rank_key(v[i], index_of(i));
+            mine = key > mine ? key : mine;
         }
     }
-    uint64_t below = ~0ull;
-    for (uint32_t j = 0; j < a.n_top; ++j) {
-        if (threadIdx.x == 0) best = 0;
-        __syncthreads();
-        uint64_t mine = 0;
-        for (uint32_t i = threadIdx.x; i < a.vocab; i += 256) {
-            const uint64_t key = rank_key(x[i], i);
-            if (key < below && key > mine) mine = key;
+    share(Stats{m, s, t}, part);
+    mine = sorted(mine, lane);
+    const uint64_t mark = __shfl_sync(0xffffffffu, mine, a.n_top - 1);
+    if (lane == 0) bound_of[warp] = mark;
+    __syncthreads();
+    uint64_t bound = bound_of[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWarps; ++w) bound = bound_of[w] > bound ? bound_of[w] : bound;
+    const float bound_value = bound ? key_value(bound) : -INFINITY;
+    const uint32_t bound_index = bound ? key_index(bound) : 0xffffffffu;
+    auto enters = [&](uint32_t i) { return v[i] >= bound_value && there(i) && (v[i] > bound_value || index_of(i) <= bound_index); };
+    if (m >= bound_value) {
+#pragma unroll
+        for (uint32_t i = 0; i <= kHeld * 4; ++i)
+            if (enters(i)) {
+                const uint32_t at = atomicAdd(&n_candidates, 1u);
+                if (at < kCandidates) candidates[at] = rank_key(v[i], index_of(i));
+            }
+    }
+    __syncthreads();
+    const uint32_t n = n_candidates;
+    uint64_t best = 0;
+    if (n > kCandidates) {  // too many for the list: every warp sorts its own, then they join
+        for (uint32_t i = 0; i <= kHeld * 4; ++i) {
+            uint64_t key = 0;
+#pragma unroll
+            for (uint32_t e = 0; e <= kHeld * 4; ++e)
+                if (e == i && enters(e)) key = rank_key(v[e], index_of(e));
+            if (__any_sync(0xffffffffu, key != 0)) best = merged(best, sorted(key, lane), lane);
         }
-        atomicMax(&best, (unsigned long long)mine);
-        __syncthreads();
-        below = best;
-        if (threadIdx.x == 0) {
-            const uint32_t id = 0xffffffffu - (uint32_t)below;
-            if (a.top_ids) a.top_ids[(size_t)t * a.n_top + j] = ok ? (int32_t)id : -1;
-            if (a.top_logprob) a.top_logprob[(size_t)t * a.n_top + j] = ok ? (x[id] - m) - ln : nan;
-        }
+        best_of[warp][lane] = best;
         __syncthreads();
     }
+    if (warp != 0) return;
+    if (n > kCandidates) {
+        for (uint32_t w = 1; w < kWarps; ++w) best = merged(best, best_of[w][lane], lane);
+    } else {
+        for (uint32_t i = 0; i < n; i += 32) best = merged(best, sorted(i + lane < n ? candidates[i + lane] : 0ull, lane), lane);
+    }
+    const Stats st = of_block(part);
+    if (a.n_slices == 1) {
+        finish(a, row, st, best, lane);
+        return;
+    }
+    if (lane == 0) *reinterpret_cast<float4 *>(a.stats + (size_t)blockIdx.x * 4) = make_float4(st.m, st.s, st.t, 0.f);
+    a.keys[(size_t)blockIdx.x * 32 + lane] = best;
+}
+
+// The slices of a row, one block each row.
+template <bool kTop>
+__global__ void __launch_bounds__(kThreads)
+log_probs_join_kernel(LogProbArgs a) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    __shared__ Stats part[kWarps];
+    __shared__ uint64_t best_of[kTop ? kWarps : 1][32];
+    const uint32_t row = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    Stats st{-INFINITY, 0.f, 0.f};
+    for (uint32_t i = threadIdx.x; i < a.n_slices; i += kThreads) {
+        const float4 v = *reinterpret_cast<const float4 *>(a.stats + ((size_t)row * a.n_slices + i) * 4);
+        st = joined(st, Stats{v.x, v.y, v.z});
+    }
+    share(st, part);
+    uint64_t best = 0;
+    if constexpr (kTop) {
+        for (uint32_t i = warp; i < a.n_slices; i += kWarps)
+            best = merged(best, a.keys[((size_t)row * a.n_slices + i) * 32 + lane], lane);
+        best_of[warp][lane] = best;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    st = of_block(part);
+    if constexpr (kTop)
+        for (uint32_t w = 1; w < kWarps; ++w) best = merged(best, best_of[w][lane], lane);
+    finish(a, row, st, best, lane);
+}
+
+// How many slices a row is cut into, and their length (a multiple of four entries).
+void slices(size_t n_tokens, size_t vocab, size_t n_top, uint32_t *n, uint32_t *length) {
+    const size_t most = qk::ceil_div(vocab, kMinSlice), want = std::max<size_t>(1, kWantBlocks / std::max<size_t>(1, n_tokens));
+    size_t len = (qk::ceil_div(vocab, std::min(most, want)) + 3) / 4 * 4;
+    if (n_top) len = std::min<size_t>(len, kThreads * kHeld * 4);  // (what stays in registers)
+    *length = (uint32_t)len;
+    *n = (uint32_t)qk::ceil_div(vocab, len);
 }
 
 }  // namespace
@@ -95,8 +325,10 @@ log_probs_plain_kernel(LogProbArgs a) {
 extern "C" {
 
 size_t qk_log_probs_scratch(size_t n_tokens, size_t vocab, size_t n_top) {
-    (void)n_tokens, (void)vocab, (void)n_top;
-    return 0;
+    if (!n_tokens || !vocab) return 0;
+    uint32_t n, length;
+    slices(n_tokens, vocab, n_top, &n, &length);
+    return n == 1 ? 0 : n_tokens * n * (16 + (n_top ? 256 : 0));
 }
 
 qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t vocab, size_t stride,
@@ -108,8 +340,10 @@ qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t
         return qk::fail(QK_ERR_VALUE, "n_top must be at most %u and the vocabulary of %zu, got %zu", kMaxTop, vocab, n_top);
     if (n_tokens > (1u << 24)) return qk::fail(QK_ERR_VALUE, "%zu rows are more than one call takes", n_tokens);
     if (!logits) return qk::fail(QK_ERR_VALUE, "logits is null");
+    if ((uintptr_t)logits % sizeof(float)) return qk::fail(QK_ERR_VALUE, "logits lie on no float boundary");
     if (logprob && !targets) return qk::fail(QK_ERR_VALUE, "logprob needs targets");
-    if (!scratch && qk_log_probs_scratch(n_tokens, vocab, n_top)) return qk::fail(QK_ERR_VALUE, "scratch is null");
+    const size_t need = qk_log_probs_scratch(n_tokens, vocab, n_top);
+    if (need && (!scratch || (uintptr_t)scratch % 16)) return qk::fail(QK_ERR_VALUE, "scratch is null or on no 16-byte boundary");
     if (n_tokens == 0) return QK_OK;
     qk_ctx *c;
     qk::DeviceGuard guard;
@@ -120,10 +354,18 @@ qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t
     LogProbArgs a{};
     a.logits = logits, a.stride = stride, a.n_tokens = (uint32_t)n_tokens, a.vocab = (uint32_t)vocab, a.n_top = (uint32_t)n_top;
     a.targets = targets, a.lse = lse, a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob, a.top_ids = top_ids;
-    (void)qk::launch_pdl(c->pdl, log_probs_plain_kernel, dim3((unsigned)n_tokens), dim3(256), 0, c->stream, a);
-    QK_CUDA(cudaGetLastError());
-    c->launches++;
-    return QK_OK;
+    slices(n_tokens, vocab, n_top, &a.n_slices, &a.slice);
+    a.keys = static_cast<uint64_t *>(scratch);
+    a.stats = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + (n_top ? n_tokens * a.n_slices * 256 : 0));
+    auto go = [&](auto kernel, unsigned blocks) -> qk_status {
+        (void)qk::launch_pdl(c->pdl, kernel, dim3(blocks), dim3(kThreads), 0, c->stream, a);
+        QK_CUDA(cudaGetLastError());
+        c->launches++;
+        return QK_OK;
+    };
+    st = go(n_top ? log_probs_top_kernel : log_probs_kernel, (unsigned)(n_tokens * a.n_slices));
+    if (st != QK_OK || a.n_slices == 1) return st;
+    return go(n_top ? log_probs_join_kernel<true> : log_probs_join_kernel<false>, (unsigned)n_tokens);
 }
 
 }  // extern "C"
