@@ -4,14 +4,14 @@ a prefix that all sequences share.
 
 A ``KvCache`` names torch tensors; every method is C-ABI calls (``qk_cache_*``) that only launch kernels, so
 that a step can be captured in a CUDA graph.  Work runs on the context's stream and is ordered with torch's
-current stream on both sides; outputs and workspaces come from torch's allocator, per call, so that two
-captured graphs share none.
+current stream on both sides.  A captured call has a workspace of its graph's; eager calls share the context's.
 """
 
 from __future__ import annotations
 
 import contextlib
 import ctypes
+import threading
 
 from . import _lib
 from ._lib import QK_BF16, QK_F32, QK_I8, KernelError, check
@@ -39,17 +39,40 @@ def _joined(torch, handle, current):
 
 
 _alone = contextlib.nullcontext()
+_growing = threading.Lock()
+
+
+def _raw_stream(torch):
+    """Device index -> handle of torch's current stream (a tenth of the cost of the stream object)."""
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def ordered(ctx: GpuContext, device):
     """A context manager around calls on ``ctx`` whose tensors belong to torch's current stream."""
     import torch
-    current = torch.cuda.current_stream(device)
-    handle = ctx.stream
-    if handle == (current.cuda_stream or 1):   # (the legacy default stream is 0 to torch, 1 to the context)
+    handle = ctx.stream_handle
+    # (the legacy default stream is 0 to torch, 1 to the context)
+    if handle == (_raw_stream(torch)(device.index) or 1):
         return _alone
-    return _joined(torch, handle, current)
+    return _joined(torch, handle, torch.cuda.current_stream(device))
 
+
+def workspace(ctx: GpuContext, size: int, device):
+    """Device memory of ``size`` bytes for one call on ``ctx``: the context's own, grown and kept (calls on a context
+    follow one another on its stream), but inside a stream capture a tensor of the graph's."""
+    import torch
+    if not size:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    kept = ctx.workspaces    # (the ones outgrown stay: work in flight may use them)
+    if not kept or kept[-1].numel() < size:
+        with _growing:
+            if not kept or kept[-1].numel() < size:
+                grown = torch.empty(max(size, 1 << 20, 2 * kept[-1].numel() if kept else 0), dtype=torch.uint8, device=device)
+                kept.append(grown)
+    return kept[-1]
 
 
 def check_tensor(what: str, t, dtype, device, shape=None) -> None:
@@ -70,7 +93,7 @@ class KvCache:
 
     def __init__(self, ctx: GpuContext, k, v, k_scale=None, v_scale=None, first_position: int = 0):
         import torch
-        self._torch, self.ctx = torch, ctx
+        self._torch, self._f32, self.ctx = torch, torch.float32, ctx
         names = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.int8: "int8"}
         if k.dtype not in names:
             raise KernelError(f"a cache holds float32, bfloat16 or int8, got {str(k.dtype).replace('torch.', '')}")
@@ -121,8 +144,11 @@ class KvCache:
 
     def _rows(self, what: str, t, heads: int | None, tokens: int | None = None):
         """A float32 ``[tokens, heads, head_dim]`` whose tokens may lie apart; its tokens and their distance."""
-        check_tensor(what, t, self._torch.float32, self.device)
-        d = self.head_dim
+        d, shape = self.head_dim, t.shape
+        if (t.dtype is self._f32 and t.device == self.device and len(shape) == 3 and shape[2] == d
+                and (heads is None or shape[1] == heads) and (tokens is None or shape[0] == tokens) and t.is_contiguous()):
+            return shape[0], shape[1] * d
+        check_tensor(what, t, self._f32, self.device)
         if t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads) or \
                 (tokens is not None and t.shape[0] != tokens):
             want = ("tokens" if tokens is None else tokens, "heads" if heads is None else heads, d)
@@ -204,9 +230,6 @@ class KvCache:
             raise KernelError(f"prefix_len and prefix_seq must not be negative, got {prefix_len}, {prefix_seq}")
         return prefix._ref
 
-    def _scratch(self, size: int):
-        return self._torch.empty(size, dtype=self._torch.uint8, device=self.device) if size else None
-
     def attend(self, q, kv_len, prefix: "KvCache | None" = None, prefix_len: int = 0, prefix_seq: int = 0, out=None):
         """softmax(q k^T / sqrt(head_dim)) v with one query per sequence: ``q`` ``[batch, heads, head_dim]``
         (rotated), sequence b sees the first ``kv_len[b]`` rows of slot b (int32, on the device) and the first
@@ -221,7 +244,7 @@ class KvCache:
         out, out_stride = self._out(out, n, heads)
         lib = _lib.lib()
         if n:
-            scratch = self._scratch(lib.qk_cache_attend_scratch(self._ref, prefix_len, n, heads))
+            scratch = workspace(self.ctx, lib.qk_cache_attend_scratch(self._ref, prefix_len, n, heads), self.device)
             with ordered(self.ctx, self.device):
                 check(lib.qk_cache_attend(self.ctx.handle, self._ref, ref, prefix_seq, prefix_len, q.data_ptr(), q_stride,
                                           kv_len.data_ptr(), n, heads, None if scratch is None else scratch.data_ptr(),
@@ -243,7 +266,8 @@ class KvCache:
         out, out_stride = self._out(out, n, heads)
         lib = _lib.lib()
         if n:
-            scratch = self._scratch(lib.qk_cache_portion_scratch(self._ref, row, prefix_len, n, heads))
+            scratch = workspace(self.ctx, lib.qk_cache_portion_scratch(self._ref, row, prefix_len, n, heads),
+                                self.device)
             with ordered(self.ctx, self.device):
                 check(lib.qk_cache_portion(self.ctx.handle, self._ref, seq, row, ref, prefix_seq, prefix_len, q.data_ptr(),
                                            q_stride, n, heads, None if scratch is None else scratch.data_ptr(),

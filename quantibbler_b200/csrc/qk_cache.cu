@@ -2,6 +2,7 @@
 // attention of a step and of a prompt's portion, both with rows in front that all sequences share.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "qk_cache.h"
 #include "qk_cache_attend.cuh"
@@ -28,82 +29,142 @@ __device__ __forceinline__ bool superseded(const int32_t *__restrict__ positions
     return __syncthreads_or(later) != 0;
 }
 
-// One block per token and share of its rows; a warp per row (a head of q, k or v), a lane holds the pairs
-// i, i + d/2 it rotates.  What bounds it: a large prompt's bytes (q read and written in float32 are most of them).
-template <typename KV>  // float, uint16_t (bfloat16), int8_t
+// The largest of the lanes' non-negative numbers (their bits are in their order).
+__device__ __forceinline__ double warp_peak(double x) {
+    const uint32_t hi = (uint32_t)__double2hiint(x), top = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, hi == top ? (uint32_t)__double2loint(x) : 0u);
+    return __hiloint2double((int)top, (int)lo);
+}
+
+// n consecutive values.
+template <int kN, typename T>
+__device__ __forceinline__ void load_n(const T *p, T (&v)[kN]) {
+    using V = std::conditional_t<kN * sizeof(T) == 16, uint4, std::conditional_t<kN * sizeof(T) == 8, uint2, uint32_t>>;
+    *reinterpret_cast<V *>(v) = *reinterpret_cast<const V *>(p);
+}
+
+// One block per token and share of its rows; a warp per row (a head of q, k or v) at a time.  A lane rotates pairs
+// (i, i + d/2) and keeps their angles for all rows of the token.  kPairs > 0: a lane has kPairs neighbouring pairs and
+// loads them as vectors; 0: any even head size, addresses of any alignment.
+// What bounds it: a long prompt's bytes (q read and written in float32 are most of them); a step's few rows are latency.
+template <typename KV, int kPairs>  // KV: float, uint16_t (bfloat16), int8_t
 __global__ void __launch_bounds__(256)
-append_kernel(CacheView c, const float *__restrict__ q, size_t q_stride, float *__restrict__ q_out, size_t q_out_stride,
+append_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t q_out_stride,
               uint32_t n_heads, const float *__restrict__ k, size_t k_stride, const float *__restrict__ v, size_t v_stride,
               const float *__restrict__ cos_sin, uint32_t n_positions, const int32_t *__restrict__ positions,
               const int32_t *__restrict__ seq_index, uint32_t first_position, uint32_t n_tokens, int *__restrict__ error) {
     qk::pdl_launch();
     qk::pdl_wait();
-    const uint32_t tok = blockIdx.x, half = c.d / 2, lane = threadIdx.x % 32;
+    constexpr int kMine = kPairs ? kPairs : 4;  // pairs of a lane (head_dim <= 256)
+    const uint32_t tok = blockIdx.x, half = c.d / 2, lane = threadIdx.x % 32, warps = gridDim.y * (blockDim.x / 32);
+    const uint32_t warp = blockIdx.y * (blockDim.x / 32) + threadIdx.x / 32;
     const int64_t pos = positions[tok], seq = seq_index[tok], row = pos - (int64_t)first_position;
     if (row < 0 || row >= (int64_t)c.rows || pos >= (int64_t)n_positions || seq < 0 || seq >= (int64_t)c.n_seq) {
         if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(error, 4);
         return;
     }
-    const bool hidden = superseded(positions, seq_index, tok, n_tokens);
-    const float *cs = cos_sin + (size_t)pos * c.d;
-    const uint32_t heads = q ? n_heads : 0, n_rows = heads + (hidden ? 0 : 2 * c.n_kv);
-    for (uint32_t r = blockIdx.y * (blockDim.x / 32) + threadIdx.x / 32; r < n_rows; r += gridDim.y * (blockDim.x / 32)) {
-        const bool is_q = r < heads, is_k = !is_q && r - heads < c.n_kv;
-        const uint32_t h = is_q ? r : is_k ? r - heads : r - heads - c.n_kv;
-        const float *src = is_q ? q + tok * q_stride + (size_t)h * c.d
-                                : (is_k ? k + tok * k_stride : v + tok * v_stride) + (size_t)h * c.d;
-        if (is_q) {
-            float *dst = q_out + tok * q_out_stride + (size_t)h * c.d;
-            for (uint32_t i = lane; i < half; i += 32) {
-                const float a = src[i], b = src[half + i], co = cs[2 * i], si = cs[2 * i + 1];
-                dst[i] = rope_first(a, b, co, si);
-                dst[half + i] = rope_second(a, b, co, si);
+    auto pair_of = [&](int e) { return kPairs ? lane * kPairs + e : lane + 32 * e; };
+    auto load_pairs = [&](const float *src, float (&a)[kMine], float (&b)[kMine]) {
+        if constexpr (kPairs > 0) {
+            load_n<kPairs>(src + lane * kPairs, a);
+            load_n<kPairs>(src + half + lane * kPairs, b);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kMine; ++e) {
+                const uint32_t i = pair_of(e);
+                a[e] = i < half ? src[i] : 0.f, b[e] = i < half ? src[half + i] : 0.f;
             }
-            continue;
         }
+    };
+    auto store_pairs = [&](auto *dst, const auto &a, const auto &b) {
+        using T = std::remove_reference_t<decltype(*dst)>;
+        if constexpr (kPairs > 0 && (kPairs * sizeof(T) == 2 || kPairs * sizeof(T) == 4 || kPairs * sizeof(T) >= 8)) {
+            using V = std::conditional_t<kPairs * sizeof(T) == 16, uint4,
+                                         std::conditional_t<kPairs * sizeof(T) == 8, uint2,
+                                                            std::conditional_t<kPairs * sizeof(T) == 4, uint32_t, uint16_t>>>;
+            *reinterpret_cast<V *>(dst + lane * kPairs) = *reinterpret_cast<const V *>(a);
+            *reinterpret_cast<V *>(dst + half + lane * kPairs) = *reinterpret_cast<const V *>(b);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kMine; ++e) {
+                const uint32_t i = pair_of(e);
+                if (i < half) dst[i] = a[e], dst[half + i] = b[e];
+            }
+        }
+    };
+    float co[kMine], si[kMine];
+    {
+        const float *cs = cos_sin + (size_t)pos * c.d;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) {
+            const uint32_t i = pair_of(e);
+            const float2 t = i < half ? make_float2(cs[2 * i], cs[2 * i + 1]) : make_float2(1.f, 0.f);
+            co[e] = t.x, si[e] = t.y;
+        }
+    }
+    if (q) {
+        constexpr uint32_t kRows = 2;  // rows in flight
+        for (uint32_t h0 = warp; h0 < n_heads; h0 += kRows * warps) {
+            alignas(16) float a[kRows][kMine], b[kRows][kMine];
+#pragma unroll
+            for (uint32_t u = 0; u < kRows; ++u)
+                if (h0 + u * warps < n_heads) load_pairs(q + tok * q_stride + (size_t)(h0 + u * warps) * c.d, a[u], b[u]);
+#pragma unroll
+            for (uint32_t u = 0; u < kRows; ++u) {
+                if (h0 + u * warps >= n_heads) break;
+                alignas(16) float x[kMine], y[kMine];
+#pragma unroll
+                for (int e = 0; e < kMine; ++e) {
+                    x[e] = rope_first(a[u][e], b[u][e], co[e], si[e]);
+                    y[e] = rope_second(a[u][e], b[u][e], co[e], si[e]);
+                }
+                store_pairs(q_out + tok * q_out_stride + (size_t)(h0 + u * warps) * c.d, x, y);
+            }
+        }
+    }
+    if (superseded(positions, seq_index, tok, n_tokens)) return;
+    // (the warps that had fewer rows of q first)
+    for (uint32_t r = warps - 1 - warp; r < 2 * c.n_kv; r += warps) {
+        const bool is_k = r < c.n_kv;
+        const uint32_t h = is_k ? r : r - c.n_kv;
+        alignas(16) float a[kMine], b[kMine];
+        load_pairs((is_k ? k + tok * k_stride : v + tok * v_stride) + (size_t)h * c.d, a, b);
         const size_t line = ((size_t)seq * c.n_kv + h) * c.rows + (size_t)row;
         KV *dst = static_cast<KV *>(is_k ? c.k : c.v) + line * c.d;
+        alignas(16) KV x[kMine], y[kMine];
         if constexpr (sizeof(KV) != 1) {
-            for (uint32_t i = lane; i < half; i += 32) {
-                const float a = src[i], b = src[half + i], co = is_k ? cs[2 * i] : 1.f, si = is_k ? cs[2 * i + 1] : 0.f;
-                store_from_float<KV>(dst, i, is_k ? rope_first(a, b, co, si) : a);
-                store_from_float<KV>(dst, half + i, is_k ? rope_second(a, b, co, si) : b);
+#pragma unroll
+            for (int e = 0; e < kMine; ++e) {
+                store_from_float<KV>(x, e, is_k ? rope_first(a[e], b[e], co[e], si[e]) : a[e]);
+                store_from_float<KV>(y, e, is_k ? rope_second(a[e], b[e], co[e], si[e]) : b[e]);
             }
         } else {
-            double x[2][4];  // (head_dim <= 256: four pairs a lane); products of two float32 are exact
-            double peak = 0.0;
+            // In 64 bits, where products of two float32 are exact.
+            double p[kMine], s[kMine], peak = 0.0;
             bool finite = true;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t i = lane + 32 * e;
-                x[0][e] = x[1][e] = 0.0;
-                if (i >= half) continue;
-                const double a = src[i], b = src[half + i];
+            for (int e = 0; e < kMine; ++e) {
+                p[e] = a[e], s[e] = b[e];
                 if (is_k) {
-                    const double co = cs[2 * i], si = cs[2 * i + 1];
-                    x[0][e] = fma(a, co, -(b * si));
-                    x[1][e] = fma(b, co, a * si);
-                } else {
-                    x[0][e] = a, x[1][e] = b;
+                    const double x0 = p[e], y0 = s[e];
+                    p[e] = fma(x0, (double)co[e], -(y0 * (double)si[e]));
+                    s[e] = fma(y0, (double)co[e], x0 * (double)si[e]);
                 }
-                finite = finite && fabs(x[0][e]) < INFINITY && fabs(x[1][e]) < INFINITY;
-                peak = fmax(peak, fmax(fabs(x[0][e]), fabs(x[1][e])));
+                finite = finite && fabs(p[e]) < INFINITY && fabs(s[e]) < INFINITY;
+                peak = fmax(peak, fmax(fabs(p[e]), fabs(s[e])));
             }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) peak = fmax(peak, __shfl_xor_sync(0xffffffffu, peak, off));
             finite = __all_sync(0xffffffffu, finite);
-            float scale = (float)(peak / 127.0);
+            float scale = (float)(warp_peak(peak) / 127.0);
             if (scale == 0.f) scale = 1.f;
             const float inv = 1.f / scale;  // (infinite for the smallest scales: then every code takes the division)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t i = lane + 32 * e;
-                if (i >= half) continue;
-                dst[i] = (int8_t)(finite ? quantise(x[0][e], scale, inv) : 0);
-                dst[half + i] = (int8_t)(finite ? quantise(x[1][e], scale, inv) : 0);
+            for (int e = 0; e < kMine; ++e) {
+                x[e] = (int8_t)(finite ? quantise(p[e], scale, inv) : 0);
+                y[e] = (int8_t)(finite ? quantise(s[e], scale, inv) : 0);
             }
             if (lane == 0) (is_k ? c.k_scale : c.v_scale)[line] = finite ? scale : __int_as_float(0x7fffffff);
         }
+        store_pairs(dst, x, y);
     }
 }
 
@@ -115,17 +176,18 @@ template <> __device__ __forceinline__ float value_at<int8_t>(const int8_t *p, s
     return (float)p[i] * scale;
 }
 
-template <typename KV, typename Out>
+// A warp per row.  kVec: head sizes of whole groups of four values per lane, on 16-byte boundaries.
+template <typename KV, typename Out, bool kVec>
 __global__ void __launch_bounds__(256)
 read_kernel(CacheView c, const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index, uint32_t first_position,
             uint32_t n_tokens, Out *__restrict__ k_out, Out *__restrict__ v_out, int *__restrict__ error) {
     qk::pdl_launch();
     qk::pdl_wait();
     const uint32_t lane = threadIdx.x % 32;
-    const size_t r = (size_t)blockIdx.x * 8 + threadIdx.x / 32;  // (token, kv head, k or v)
+    const size_t r = (size_t)blockIdx.x * 8 + threadIdx.x / 32;  // (token, k or v, kv head)
     if (r >= (size_t)n_tokens * c.n_kv * 2) return;
-    const bool is_v = r % 2;
-    const uint32_t h = (uint32_t)(r / 2 % c.n_kv), tok = (uint32_t)(r / 2 / c.n_kv);
+    const uint32_t h = (uint32_t)(r % c.n_kv), tok = (uint32_t)(r / c.n_kv / 2);
+    const bool is_v = r / c.n_kv % 2;
     const int64_t row = (int64_t)positions[tok] - (int64_t)first_position, seq = seq_index[tok];
     const bool there = row >= 0 && row < (int64_t)c.rows && seq >= 0 && seq < (int64_t)c.n_seq;
     if (!there && lane == 0) atomicOr(error, 4);
@@ -133,7 +195,19 @@ read_kernel(CacheView c, const int32_t *__restrict__ positions, const int32_t *_
     const KV *src = static_cast<const KV *>(is_v ? c.v : c.k) + line * c.d;
     const float scale = sizeof(KV) == 1 && there ? (is_v ? c.v_scale : c.k_scale)[line] : 1.f;
     Out *dst = (is_v ? v_out : k_out) + ((size_t)tok * c.n_kv + h) * c.d;
-    for (uint32_t i = lane; i < c.d; i += 32) store_from_float<Out>(dst, i, there ? value_at<KV>(src, i, scale) : 0.f);
+    if constexpr (kVec) {
+        for (uint32_t i = 4 * lane; i < c.d; i += 128) {
+            alignas(16) KV x[4];
+            alignas(16) Out y[4];
+            if (there) load_n<4>(src + i, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_from_float<Out>(y, e, there ? value_at<KV>(x, e, scale) : 0.f);
+            if constexpr (sizeof(Out) == 4) *reinterpret_cast<uint4 *>(dst + i) = *reinterpret_cast<const uint4 *>(y);
+            else *reinterpret_cast<uint2 *>(dst + i) = *reinterpret_cast<const uint2 *>(y);
+        }
+    } else {
+        for (uint32_t i = lane; i < c.d; i += 32) store_from_float<Out>(dst, i, there ? value_at<KV>(src, i, scale) : 0.f);
+    }
 }
 
 // ------------------------------------------------------------------ attention, plain form
@@ -287,10 +361,7 @@ join_kernel(const float *__restrict__ partial, qk::AttendArgs a, uint32_t n_slot
     for (uint32_t c = threadIdx.x; c < d; c += 128) {
         float v = 0.f;
 #pragma unroll 8
-        for (uint32_t s = 0; s < n_slots; ++s) {
-            const float w = weight[s];
-            if (w != 0.f) v = fmaf(p[(size_t)s * (d + 2) + 2 + c], w, v);
-        }
+        for (uint32_t s = 0; s < n_slots; ++s) v = fmaf(p[(size_t)s * (d + 2) + 2 + c], weight[s], v);
         a.out[query * a.out_stride + (size_t)head * d + c] = v * inv;
     }
 }
@@ -487,12 +558,23 @@ qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q,
     const dim3 grid((unsigned)n_tokens, (unsigned)std::min(most, want));
     const CacheView cv = view(cache);
     int *err = (int *)c->d_err.ptr;
-#define QK_APPEND(KV)                                                                                                          \
-    QK_PDL(c, append_kernel<KV>, grid, dim3(256), 0, cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, v, \
-           v_stride, cos_sin, (uint32_t)n_positions, positions, seq_index, (uint32_t)first_position, (uint32_t)n_tokens, err)
+    // (a row's vectors lie on their boundaries where the tensors' addresses and strides do)
+    const size_t mask = ((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cv.k | (uintptr_t)cv.v) |
+                        (q ? (q_stride | q_out_stride) * 4 : 0) | (k_stride | v_stride) * 4;
+    const int pairs = mask % 16 ? 0 : d == 128 ? 2 : d == 256 ? 4 : 0;
+#define QK_APPEND_N(KV, N)                                                                                                  \
+    QK_PDL(c, (append_kernel<KV, N>), grid, dim3(256), 0, cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, \
+           v, v_stride, cos_sin, (uint32_t)n_positions, positions, seq_index, (uint32_t)first_position, (uint32_t)n_tokens, err)
+#define QK_APPEND(KV)                          \
+    do {                                       \
+        if (pairs == 2) QK_APPEND_N(KV, 2);    \
+        else if (pairs == 4) QK_APPEND_N(KV, 4); \
+        else QK_APPEND_N(KV, 0);               \
+    } while (0)
     if (cv.dtype == QK_I8) QK_APPEND(int8_t);
     else if (cv.dtype == QK_BF16) QK_APPEND(uint16_t);
     else QK_APPEND(float);
+#undef QK_APPEND_N
 #undef QK_APPEND
     QK_CUDA(cudaGetLastError());
     c->launches++;
@@ -519,9 +601,15 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
     const unsigned blocks = (unsigned)qk::ceil_div(n_tokens * cache->n_kv_heads * 2, 8);
     const CacheView cv = view(cache);
     int *err = (int *)c->d_err.ptr;
-#define QK_READ(KV, Out)                                                                                                  \
-    QK_PDL(c, (read_kernel<KV, Out>), dim3(blocks), dim3(256), 0, cv, positions, seq_index, (uint32_t)first_position, \
+    const bool vec = cv.d % 4 == 0 && (((uintptr_t)cv.k | (uintptr_t)cv.v | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0;
+#define QK_READ_V(KV, Out, V)                                                                                             \
+    QK_PDL(c, (read_kernel<KV, Out, V>), dim3(blocks), dim3(256), 0, cv, positions, seq_index, (uint32_t)first_position, \
            (uint32_t)n_tokens, (Out *)k_out, (Out *)v_out, err)
+#define QK_READ(KV, Out)                     \
+    do {                                     \
+        if (vec) QK_READ_V(KV, Out, true);   \
+        else QK_READ_V(KV, Out, false);      \
+    } while (0)
 #define QK_READ_TO(Out)                                \
     do {                                               \
         if (cv.dtype == QK_I8) QK_READ(int8_t, Out);   \
@@ -532,6 +620,7 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
     else QK_READ_TO(uint16_t);
 #undef QK_READ_TO
 #undef QK_READ
+#undef QK_READ_V
     QK_CUDA(cudaGetLastError());
     c->launches++;
     c->err_armed = true;

@@ -92,11 +92,16 @@ struct AttendShape {
     static constexpr int kStageBytes = 2 * 16 * kRowBytes + (kI8 ? 128 : 0);
     static constexpr int kStages = kI8 ? 4 : 3;
     static constexpr int kWarpBytes = kStages * kStageBytes;
-    static constexpr int kSmem = 4 * kWarpBytes;
+    static constexpr int kQPitch = kRowBytes + 16;                     // bytes of one term of a query row
+    static constexpr int kSmem = 4 * kWarpBytes + 8 * 3 * kQPitch + 32;
     static_assert(kWarpBytes >= (8 * D + 16) * 4, "a warp's results lie in its ring");
     // (pieces of 16 bytes of a row change places so that fragment loads meet no bank twice)
     __device__ static uint32_t swizzle(uint32_t row, uint32_t piece) {
         return row * kRowBytes + ((piece ^ (kPieces >= 8 ? row & 7 : (row >> 1) & (kPieces - 1))) << 4);
+    }
+    // The i-th piece of a row that lane t feeds to the scores' product (any order of the channels will do).
+    __device__ static uint32_t piece_of(uint32_t t, int i) {
+        return kI8 ? (D == 128 ? 2 * t + i : t) : 2 * t + (i % 2) + 8 * (i / 2);
     }
 };
 
@@ -139,76 +144,67 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
     for (int i = 0; i < kStages - 1; ++i)
         if (j_first + i * kStride < s.end) fetch(j_first + i * kStride, i);
 
-    // ---- q as B fragments.  Column g of tile n: tile n < kTiles: row 4 n + g / 2, term g % 2; the last: thirds
-    uint32_t qf[kQTiles][kSteps][2];
-    float f[kTiles];  // what turns a score's sum into log2 units, row 4 n + t
+    // ---- q's terms, a warp per row: lines of [row][term] in shared memory
+    uint8_t *q_lines = smem + 4 * Shape::kWarpBytes;
+    float *q_factor = reinterpret_cast<float *>(q_lines + 8 * 3 * Shape::kQPitch);  // what turns a row's sums into log2 units
     const float unit = kLog2E / sqrtf((float)D);
-    auto q_row = [&](uint32_t r) {
-        const uint32_t row = s.first_row + min(r, s.n_rows - 1);
-        return a.q + (row / group) * a.q_stride + (size_t)(kvh * group + row % group) * D;
-    };
+    for (uint32_t r = warp; r < 4 * kTiles; r += 4) {
+        constexpr uint32_t kLanes = D / 4;  // lanes with four channels each
+        const uint32_t row = s.first_row + min(r, s.n_rows - 1), c = 4 * (lane % kLanes);
+        float4 x = *reinterpret_cast<const float4 *>(a.q + (row / group) * a.q_stride +
+                                                     (size_t)(kvh * group + row % group) * D + c);
+        if (r >= s.n_rows) x = make_float4(0.f, 0.f, 0.f, 0.f);
+        uint8_t *line = q_lines + r * 3 * Shape::kQPitch;
+        if (kI8) {
+            const uint32_t bits = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
+                                      max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
+            const uint32_t peak = __reduce_max_sync(0xffffffffu, bits);  // (an infinity or NaN is larger than any number)
+            const int e = exponent_of(__uint_as_float(peak));
+            const float mul = pow2(21 - e);
+            const float v4[4] = {x.x, x.y, x.z, x.w};
+            uint32_t word[3] = {0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                // v = 65536 d2 + 256 d1 + d0, digits in -128 .. 127: the bytes of v + 0x8080, the lower two less 128
+                const uint32_t v = (uint32_t)(__float2int_rn(v4[b] * mul) + 0x8080);
+                word[0] |= (v >> 16 & 0xff) << (8 * b);
+                word[1] |= ((v >> 8 & 0xff) ^ 0x80) << (8 * b);
+                word[2] |= ((v & 0xff) ^ 0x80) << (8 * b);
+            }
+            if (lane < kLanes) {
+#pragma unroll
+                for (int term = 0; term < 3; ++term) *reinterpret_cast<uint32_t *>(line + term * Shape::kQPitch + c) = word[term];
+            }
+            if (lane == 0) q_factor[r] = peak < 0x7f800000u ? pow2(e - 21) * unit : __int_as_float(0x7fffffff);
+        } else {
+            uint32_t w0[3], w1[3];
+            split3(x.x, x.y, w0);
+            split3(x.z, x.w, w1);
+            if (lane < kLanes) {
+#pragma unroll
+                for (int term = 0; term < 3; ++term)
+                    *reinterpret_cast<uint2 *>(line + term * Shape::kQPitch + 2 * c) = make_uint2(w0[term], w1[term]);
+            }
+            if (lane == 0) q_factor[r] = unit;
+        }
+    }
+    __syncthreads();
+    // ---- as B fragments.  Column g of tile n: tile n < kTiles: row 4 n + g / 2, term g % 2; the last: third terms of
+    // rows g / 2 and 4 + g / 2 side by side
+    uint32_t qf[kQTiles][kSteps][2];
+    float f[kTiles];
 #pragma unroll
     for (int n = 0; n < kQTiles; ++n) {
-        const bool third = n >= kTiles;
-        const uint32_t r = third ? 4 * (g % 2) + g / 2 : 4 * n + g / 2;
-        const int term = third ? 2 : (int)(g % 2);
-        const bool live = r < s.n_rows && r < 4 * kTiles;
-        const float *src = q_row(r);
-        if (kI8) {
-            float x[D / 4];
-            float peak = 0.f;
-            bool finite = true;
+        const uint32_t r = n >= kTiles ? 4 * (g % 2) + g / 2 : 4 * n + g / 2, term = n >= kTiles ? 2 : g % 2;
+        const uint8_t *line = q_lines + (r * 3 + term) * Shape::kQPitch;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {  // lane t: pieces of 16 channels 2t, 2t + 1 (D 128), t (D 64)
-                const uint32_t c = (D == 128 ? 2 * t : t) * 16 + i * 4;
-                const float4 v4 = *reinterpret_cast<const float4 *>(src + c);
-                x[4 * i] = v4.x, x[4 * i + 1] = v4.y, x[4 * i + 2] = v4.z, x[4 * i + 3] = v4.w;
-            }
-#pragma unroll
-            for (int i = 0; i < D / 4; ++i) {
-                peak = fmaxf(peak, fabsf(x[i]));
-                finite = finite && fabsf(x[i]) < INFINITY;
-            }
-            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-            const int e = exponent_of(peak);
-            const float mul = pow2(21 - e);
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                uint32_t word = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    int v = live ? __float2int_rn(x[4 * i + b] * mul) : 0;
-                    const int d0 = (int)(int8_t)v;
-                    v = (v - d0) >> 8;
-                    const int d1 = (int)(int8_t)v;
-                    const int d2 = (v - d1) >> 8;
-                    word |= (uint32_t)((term == 0 ? d2 : term == 1 ? d1 : d0) & 0xff) << (8 * b);
-                }
-                qf[n][i / 2][i % 2] = word;
-            }
-            // row 4 n + t's factor: from the lanes of column 2 t
-            unsigned ok = __ballot_sync(0xffffffffu, finite);
-            if (!third) {
-                const int e_t = __shfl_sync(0xffffffffu, e, 8 * t);
-                f[n < kTiles ? n : 0] = (ok >> (8 * t) & 0xf) == 0xf ? pow2(e_t - 21) * unit : __int_as_float(0x7fffffff);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {  // pieces of 8 channels: 2t, 2t + 1, then 8 further on
-                const uint32_t c = (2 * t + (i % 2) + 8 * (i / 2)) * 8;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 v4 = *reinterpret_cast<const float4 *>(src + c + 4 * h);
-                    uint32_t w0[3], w1[3];
-                    split3(live ? v4.x : 0.f, live ? v4.y : 0.f, w0);
-                    split3(live ? v4.z : 0.f, live ? v4.w : 0.f, w1);
-                    qf[n][2 * i + h][0] = term == 0 ? w0[0] : term == 1 ? w0[1] : w0[2];
-                    qf[n][2 * i + h][1] = term == 0 ? w1[0] : term == 1 ? w1[1] : w1[2];
-                }
-            }
-            if (!third) f[n < kTiles ? n : 0] = unit;
+        for (int i = 0; i < kSteps / 2; ++i) {
+            uint4 w = *reinterpret_cast<const uint4 *>(line + 16 * Shape::piece_of(t, i));
+            if (kTiles == 1 && n == 1 && g % 2) w = make_uint4(0u, 0u, 0u, 0u);
+            qf[n][2 * i][0] = w.x, qf[n][2 * i][1] = w.y;
+            qf[n][2 * i + 1][0] = w.z, qf[n][2 * i + 1][1] = w.w;
         }
+        if (n < kTiles) f[n < kTiles ? n : 0] = q_factor[4 * n + t];
     }
 
     float o[kTiles][kOut][2], m[kTiles], l[kTiles];
@@ -242,7 +238,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
             int acc[kQTiles][4] = {};
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
-                const uint32_t piece = D == 128 ? 2 * t + i : t;
+                const uint32_t piece = Shape::piece_of(t, i);
                 const uint4 lo = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g, piece));
                 const uint4 hi = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g + 8, piece));
                 const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
@@ -266,7 +262,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
             float acc[kQTiles][4] = {};
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                const uint32_t piece = 2 * t + (i % 2) + 8 * (i / 2);
+                const uint32_t piece = Shape::piece_of(t, i);
                 const uint4 lo = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g, piece));
                 const uint4 hi = *reinterpret_cast<const uint4 *>(kt + Shape::swizzle(g + 8, piece));
                 const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};

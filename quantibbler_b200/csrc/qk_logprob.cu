@@ -189,15 +189,15 @@ log_probs_kernel(LogProbArgs a) {
 }
 
 // With the most probable entries: a slice of at most 32 entries a thread (and a single one) stays in registers.  The
-// n_top-th largest of a warp's 32 thread maxima is no better than the slice's n_top-th entry; the best such bound of
-// the warps leaves a few dozen candidates, which one warp sorts.  (Sorting whatever beats a running last place,
-// warp by warp, took 93 us on 64 rows of 128256 with 20 places.)
+// n_top-th of the 256 threads' best entries is no better than the slice's n_top-th entry: what is as good as that, a
+// few more than n_top entries, one warp sorts.  (64 rows of 128256, 20 places: whatever beats a running last place
+// sorted warp by warp 93 us; the bound from each warp's 32 threads 44.)
 __global__ void __launch_bounds__(kThreads)
 log_probs_top_kernel(LogProbArgs a) {
     qk::pdl_launch();
     qk::pdl_wait();
     __shared__ Stats part[kWarps];
-    __shared__ uint64_t bound_of[kWarps], candidates[kCandidates];
+    __shared__ uint64_t bound_key, candidates[kCandidates];
     __shared__ uint64_t best_of[kWarps][32];
     __shared__ uint32_t n_candidates;
     const uint32_t row = blockIdx.x / a.n_slices, slice = blockIdx.x % a.n_slices;
@@ -223,25 +223,29 @@ log_probs_top_kernel(LogProbArgs a) {
     for (uint32_t i = 0; i <= kHeld * 4; ++i) m = fmaxf(m, v[i]);
     float s = 0.f, t = 0.f;
     const float base = m > -INFINITY ? m : 0.f;
-    uint64_t mine = 0;  // the thread's best entry (its lowest index is taken: the single one may lie in front of or behind the others)
+    uint32_t at = 0xffffffffu;  // the lowest index of the thread's best value
 #pragma unroll
-    for (uint32_t i = 0; i <= kHeld * 4; ++i) {
+    for (int i = kHeld * 4; i >= 0; --i) {
         const float d = v[i] - base, w = ex2(d * kLog2E);
         s += w;
         t = w == 0.f ? t : fmaf(d, w, t);
-        if (v[i] == m && there(i)) {
-            const uint64_t key = rank_key(v[i], index_of(i));
-            mine = key > mine ? key : mine;
+        if (v[i] == m && there(i)) at = min(at, index_of(i));
+    }
+    // the threads' best entries, sorted: the n_top-th of them is no better than the slice's n_top-th entry
+    uint64_t list = sorted(at != 0xffffffffu ? rank_key(m, at) : 0ull, lane);
+    best_of[warp][lane] = list;
+    share(Stats{m, s, t}, part);
+#pragma unroll
+    for (uint32_t half = kWarps / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (warp < half) {
+            list = merged(list, best_of[warp + half][lane], lane);
+            best_of[warp][lane] = list;
         }
     }
-    share(Stats{m, s, t}, part);
-    mine = sorted(mine, lane);
-    const uint64_t mark = __shfl_sync(0xffffffffu, mine, a.n_top - 1);
-    if (lane == 0) bound_of[warp] = mark;
+    if (warp == 0 && lane == a.n_top - 1) bound_key = list;
     __syncthreads();
-    uint64_t bound = bound_of[0];
-#pragma unroll
-    for (uint32_t w = 1; w < kWarps; ++w) bound = bound_of[w] > bound ? bound_of[w] : bound;
+    const uint64_t bound = bound_key;
     const float bound_value = bound ? key_value(bound) : -INFINITY;
     const uint32_t bound_index = bound ? key_index(bound) : 0xffffffffu;
     auto enters = [&](uint32_t i) { return v[i] >= bound_value && there(i) && (v[i] > bound_value || index_of(i) <= bound_index); };

@@ -57,6 +57,8 @@ class GpuContext:
     def __init__(self, handle, device_index: int = 0):
         self._h = handle
         self.device_index = int(device_index)
+        self._stream_handle = None   # (known once asked for; set_stream is the only way to change it)
+        self.workspaces = []         # device memory of eager calls (cache.workspace)
 
     @classmethod
     def init_at(cls, device_index: int) -> "GpuContext":
@@ -90,6 +92,13 @@ class GpuContext:
     def stream(self) -> int:
         return int(_lib.lib().qk_gpu_stream(self._h) or 0)
 
+    @property
+    def stream_handle(self) -> int:
+        """``stream`` without a library call."""
+        if self._stream_handle is None:
+            self._stream_handle = self.stream
+        return self._stream_handle
+
     def set_stream(self, cuda_stream: int | None) -> None:
         """Launch on a caller-owned stream; ``None`` restores the context's own stream.
         The legacy default stream has the numeric handle 0, which the C ABI reads as
@@ -98,6 +107,7 @@ class GpuContext:
             handle = 0
         else:
             handle = int(cuda_stream) or 1
+        self._stream_handle = None
         check(_lib.lib().qk_gpu_set_stream(self._h, ctypes.c_void_p(handle)))
 
     def container_to_rows(self, stream, n_rows: int, r: int, transposed: bool = False) -> np.ndarray:

@@ -6,7 +6,7 @@ from typing import NamedTuple
 
 from . import _lib
 from ._lib import KernelError, check
-from .cache import check_tensor, ordered
+from .cache import check_tensor, ordered, workspace
 from .gpu import GpuContext
 
 MAX_TOP = 32
@@ -50,8 +50,7 @@ def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
     top_logprob, top_ids = flat[3 * n:].view(n, top), torch.empty((n, top), dtype=torch.int32, device=dev)
     lib = _lib.lib()
     if n:
-        size = lib.qk_log_probs_scratch(n, vocab, top)
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        scratch = workspace(ctx, lib.qk_log_probs_scratch(n, vocab, top), dev)
         with ordered(ctx, dev):
             check(lib.qk_log_probs(ctx.handle, logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab,
                                    None if targets is None else targets.data_ptr(), top,
