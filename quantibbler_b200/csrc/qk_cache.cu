@@ -276,8 +276,9 @@ struct Plan {
     uint32_t n_slots;                         // partial results per (query, head); 1: none, the output is written
 };
 
-template <bool kI8, int D>
-__global__ void __launch_bounds__(128, kI8 ? 3 : 2)
+// kMost: column tiles of four query rows that a block needs at most.
+template <bool kI8, int D, int kMost>
+__global__ void __launch_bounds__(128, kI8 ? (kMost == 1 ? 4 : 3) : 2)
 attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     qk::pdl_launch();
     qk::pdl_wait();
@@ -316,26 +317,37 @@ attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     s.v = static_cast<const uint8_t *>(src->v) + line * row_bytes;
     s.k_scale = kI8 ? src->k_scale + line : nullptr;
     s.v_scale = kI8 ? src->v_scale + line : nullptr;
-    if (s.n_rows > 4) attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
-    else attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+    if constexpr (kMost > 1) {
+        if (s.n_rows > 4) {
+            attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+            return;
+        }
+    }
+    attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
 }
 
-// Partial results {maximum (log2 units), sum, output[d]} of a (query, head) joined.  A block of 128 threads each.
+// Partial results of a (query, head) joined: outputs [slot][D], then {maximum (log2 units), sum} [slot] of all rows.
+// A block of four warps each; D / 4 lanes take a slot's output, four channels a lane.
 constexpr uint32_t kMaxSlots = 256;
 
+template <int D>
 __global__ void __launch_bounds__(128)
-join_kernel(const float *__restrict__ partial, qk::AttendArgs a, uint32_t n_slots, uint32_t d) {
+join_kernel(qk::AttendArgs a, uint32_t n_slots) {
     qk::pdl_launch();
     qk::pdl_wait();
     __shared__ float weight[kMaxSlots], red[8];
+    __shared__ __align__(16) float part[128 / (D / 4)][D];
+    constexpr uint32_t kLanes = D / 4, kSide = 128 / kLanes;  // slots side by side
     const uint32_t query = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads, warp = threadIdx.x / 32;
-    const float *p = partial + (size_t)blockIdx.x * n_slots * (d + 2);
+    const float *outs = a.scratch + (size_t)blockIdx.x * n_slots * D;
+    const float2 *stats = reinterpret_cast<const float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * n_slots * D) +
+                          (size_t)blockIdx.x * n_slots;
     float m[kMaxSlots / 128], l[kMaxSlots / 128], top = -INFINITY;
 #pragma unroll
     for (uint32_t i = 0; i < kMaxSlots / 128; ++i) {
         const uint32_t s = threadIdx.x + 128 * i;
-        m[i] = s < n_slots ? p[(size_t)s * (d + 2)] : -INFINITY;
-        l[i] = s < n_slots ? p[(size_t)s * (d + 2) + 1] : 0.f;
+        const float2 st = s < n_slots ? stats[s] : make_float2(-INFINITY, 0.f);
+        m[i] = st.x, l[i] = st.y;
         top = fmaxf(top, m[i]);
     }
 #pragma unroll
@@ -357,12 +369,21 @@ join_kernel(const float *__restrict__ partial, qk::AttendArgs a, uint32_t n_slot
     if (threadIdx.x % 32 == 0) red[4 + warp] = sum;
     __syncthreads();
     sum = (red[4] + red[5]) + (red[6] + red[7]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (uint32_t c = threadIdx.x; c < d; c += 128) {
-        float v = 0.f;
-#pragma unroll 8
-        for (uint32_t s = 0; s < n_slots; ++s) v = fmaf(p[(size_t)s * (d + 2) + 2 + c], weight[s], v);
-        a.out[query * a.out_stride + (size_t)head * d + c] = v * inv;
+    const uint32_t side = threadIdx.x / kLanes, c = 4 * (threadIdx.x % kLanes);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (uint32_t s = side; s < n_slots; s += kSide) {
+        const float4 x = *reinterpret_cast<const float4 *>(outs + (size_t)s * D + c);
+        const float w = weight[s];
+        v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
+    }
+    *reinterpret_cast<float4 *>(&part[side][c]) = v;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float x = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < kSide; ++i) x += part[i][threadIdx.x];
+        a.out[query * a.out_stride + (size_t)head * D + threadIdx.x] = sum == 0.f ? 0.f : x / sum;
     }
 }
 
@@ -426,6 +447,12 @@ qk_status check_rows(const char *what, const void *p, size_t stride, size_t widt
     return QK_OK;
 }
 
+qk_status check_scratch(const void *scratch, size_t need) {
+    if (need && (!scratch || (uintptr_t)scratch % 16))
+        return qk::fail(QK_ERR_VALUE, "scratch is null or on no 16-byte boundary (%zu bytes are needed)", need);
+    return QK_OK;
+}
+
 qk_status enter(qk_ctx *ctx, qk_ctx **c) {
     qk_status st = qk::resolve_ctx(ctx, c);
     if (st != QK_OK) return st;
@@ -448,7 +475,7 @@ bool takes_rows(const qk_kv_cache *c) { return c->dtype != QK_F32 && (c->head_di
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned_rows(const CacheView &v) { return aligned(v.k) && aligned(v.v); }
 
-constexpr size_t kWantBlocks = 148 * 9, kMinChunk = 128;
+constexpr size_t kWantBlocks = 148 * 8, kMinChunk = 128;
 
 Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_heads) {
     Plan pl{};
@@ -474,21 +501,26 @@ size_t partial_bytes(size_t queries, size_t n_heads, size_t slots, size_t d) {
     return slots > 1 ? queries * n_heads * slots * (d + 2) * sizeof(float) : 0;
 }
 
-template <bool kI8, int D>
+template <bool kI8, int D, int kMost>
 qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, const qk::AttendArgs &a, const Plan &pl) {
     constexpr size_t smem = AttendShape<kI8, D>::kSmem;
-    qk_status st = qk::allow_smem(c, attend_rows_kernel<kI8, D>, smem);
+    qk_status st = qk::allow_smem(c, attend_rows_kernel<kI8, D, kMost>, smem);
     if (st != QK_OK) return st;
     const unsigned blocks = pl.prefix_blocks + a.n_queries * own.n_kv * pl.own_subs * pl.own_splits;
-    QK_PDL(c, (attend_rows_kernel<kI8, D>), dim3(blocks), dim3(128), smem, own, pre, a, pl);
+    QK_PDL(c, (attend_rows_kernel<kI8, D, kMost>), dim3(blocks), dim3(128), smem, own, pre, a, pl);
     QK_CUDA(cudaGetLastError());
     c->launches++;
     if (pl.n_slots > 1) {
-        QK_PDL(c, join_kernel, dim3(a.n_queries * a.n_heads), dim3(128), 0, (const float *)a.scratch, a, pl.n_slots, own.d);
+        QK_PDL(c, join_kernel<D>, dim3(a.n_queries * a.n_heads), dim3(128), 0, a, pl.n_slots);
         QK_CUDA(cudaGetLastError());
         c->launches++;
     }
     return QK_OK;
+}
+template <bool kI8, int D>
+qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, const qk::AttendArgs &a, const Plan &pl) {
+    const uint32_t rows = a.prefix_len ? std::max(pl.own_rows, std::min(8u, a.n_queries * (a.n_heads / own.n_kv))) : pl.own_rows;
+    return rows > 4 ? launch_rows<kI8, D, 2>(c, own, pre, a, pl) : launch_rows<kI8, D, 1>(c, own, pre, a, pl);
 }
 
 qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, const qk::AttendArgs &a) {
@@ -498,8 +530,7 @@ qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefi
     if (st != QK_OK) return st;
     std::lock_guard<std::mutex> lock(c->mu);
     const CacheView own = view(cache), pre = view(a.prefix_len ? prefix : nullptr);
-    if (a.kv_len && takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0 &&
-        (!a.scratch || aligned(a.scratch))) {
+    if (a.kv_len && takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0) {
         const Plan pl = plan_rows(cache, a.prefix_len, a.n_queries, a.n_heads);
         if (own.dtype == QK_I8)
             return own.d == 128 ? launch_rows<true, 128>(c, own, pre, a, pl) : launch_rows<true, 64>(c, own, pre, a, pl);
@@ -643,8 +674,7 @@ qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cac
     if ((st = check_rows("q", q, q_stride, n_heads * cache->head_dim)) != QK_OK) return st;
     if ((st = check_rows("out", out, out_stride, n_heads * cache->head_dim)) != QK_OK) return st;
     if (!kv_len) return qk::fail(QK_ERR_VALUE, "kv_len is null");
-    if (!scratch && qk_cache_attend_scratch(cache, prefix_len, batch, n_heads))
-        return qk::fail(QK_ERR_VALUE, "scratch is null");
+    if ((st = check_scratch(scratch, qk_cache_attend_scratch(cache, prefix_len, batch, n_heads))) != QK_OK) return st;
     if (batch == 0) return QK_OK;
     qk::AttendArgs a{};
     a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride, a.kv_len = kv_len;
@@ -672,8 +702,7 @@ qk_status qk_cache_portion(qk_ctx *ctx, const qk_kv_cache *cache, size_t seq, si
         return qk::fail(QK_ERR_VALUE, "%zu tokens from row %zu on do not fit the cache of %zu rows", n_tokens, first_row, cache->rows);
     if ((st = check_rows("q", q, q_stride, n_heads * cache->head_dim)) != QK_OK) return st;
     if ((st = check_rows("out", out, out_stride, n_heads * cache->head_dim)) != QK_OK) return st;
-    if (!scratch && qk_cache_portion_scratch(cache, first_row, prefix_len, n_tokens, n_heads))
-        return qk::fail(QK_ERR_VALUE, "scratch is null");
+    if ((st = check_scratch(scratch, qk_cache_portion_scratch(cache, first_row, prefix_len, n_tokens, n_heads))) != QK_OK) return st;
     if (n_tokens == 0) return QK_OK;
     qk::AttendArgs a{};
     a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride;

@@ -47,16 +47,36 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// Products that begin from zero.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void copy4(void *smem, const void *gmem, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem),
                  "r"(bytes)
                  : "memory");
+}
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16_to(uint32_t smem, const void *gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void copy16_some(uint32_t smem, const void *gmem, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
 }
 // {hi, lo} of a weight as two float16 in one word, hi below.
 __device__ __forceinline__ uint32_t weight_terms(float w) {
@@ -90,7 +110,7 @@ template <bool kI8, int D>
 struct AttendShape {
     static constexpr int kRowBytes = kI8 ? D : 2 * D, kPieces = kRowBytes / 16;
     static constexpr int kStageBytes = 2 * 16 * kRowBytes + (kI8 ? 128 : 0);
-    static constexpr int kStages = kI8 ? 4 : 3;
+    static constexpr int kStages = kI8 && D == 64 ? 4 : 3;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kQPitch = kRowBytes + 16;                     // bytes of one term of a query row
     static constexpr int kSmem = 4 * kWarpBytes + 8 * 3 * kQPitch + 32;
@@ -119,22 +139,37 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
     uint8_t *ring = smem + warp * Shape::kWarpBytes;
     const uint8_t *kb = static_cast<const uint8_t *>(s.k), *vb = static_cast<const uint8_t *>(s.v);
 
-    auto fetch = [&](int j, int stage) {
-        uint8_t *dst = ring + stage * Shape::kStageBytes;
+    // A step's rows lie one behind the other: a lane's pieces are 512 bytes apart, and their places in the stage are
+    // two swizzled ones, eight rows apart.
+    constexpr int kCopies = 16 * kPieces / 32, kFresh = kPieces / 4;
+    uint32_t place[kFresh];
 #pragma unroll
-        for (int i = 0; i < 16 * kPieces / 32; ++i) {
-            const uint32_t idx = lane + 32 * i, key = idx / kPieces, piece = idx % kPieces;
-            const bool live = j + (int)key < s.end;
-            const size_t at = (size_t)(live ? j + key : s.end - 1) * kRowBytes + piece * 16;
-            const uint32_t to = Shape::swizzle(key, piece);
-            copy16(dst + to, kb + at, live ? 16u : 0u);
-            copy16(dst + 16 * kRowBytes + to, vb + at, live ? 16u : 0u);
-        }
-        if (kI8) {
-            const uint32_t key = lane % 16;
-            const bool live = j + (int)key < s.end;
-            copy4(dst + 2 * 16 * kRowBytes + lane * 4, (lane < 16 ? s.k_scale : s.v_scale) + (live ? j + key : s.end - 1),
-                  live ? 4u : 0u);
+    for (int i = 0; i < kFresh; ++i) place[i] = smem_addr(ring) + Shape::swizzle((lane + 32 * i) / kPieces, lane % kPieces);
+    const uint8_t *k_lane = kb + lane * 16, *v_lane = vb + lane * 16;
+    const float *s_lane = kI8 ? (lane < 16 ? s.k_scale : s.v_scale) + lane % 16 : nullptr;
+    auto fetch = [&](int j, int stage) {
+        const uint32_t at = stage * Shape::kStageBytes;
+        const uint8_t *ks = k_lane + (size_t)j * kRowBytes, *vs = v_lane + (size_t)j * kRowBytes;
+        if (j + 16 <= s.end) {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const uint32_t to = place[i % kFresh] + at + i / kFresh * 8 * kRowBytes;
+                copy16_to(to, ks + i * 512);
+                copy16_to(to + 16 * kRowBytes, vs + i * 512);
+            }
+            if (kI8) copy4(ring + at + 2 * 16 * kRowBytes + lane * 4, s_lane + j, 4u);
+        } else {  // rows past the end are zeros
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const bool live = j + (int)((lane + 32 * i) / kPieces) < s.end;
+                const uint32_t to = place[i % kFresh] + at + i / kFresh * 8 * kRowBytes;
+                copy16_some(to, live ? ks + i * 512 : kb, live ? 16u : 0u);
+                copy16_some(to + 16 * kRowBytes, live ? vs + i * 512 : vb, live ? 16u : 0u);
+            }
+            if (kI8) {
+                const bool live = j + (int)(lane % 16) < s.end;
+                copy4(ring + at + 2 * 16 * kRowBytes + lane * 4, live ? s_lane + j : s.k_scale, live ? 4u : 0u);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -235,7 +270,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
         float x[kTiles][2];
         float vs[2];
         if (kI8) {
-            int acc[kQTiles][4] = {};
+            int acc[kQTiles][4];
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
                 const uint32_t piece = Shape::piece_of(t, i);
@@ -244,7 +279,8 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                 const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
                 for (int n = 0; n < kQTiles; ++n) {
-                    mma_s8(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
+                    if (i == 0) mma_s8_first(acc[n], a0, qf[n][0][0], qf[n][0][1]);
+                    else mma_s8(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
                     mma_s8(acc[n], a1, qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
                 }
             }
@@ -259,7 +295,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                     x[n][h] = fmaf((float)acc[n][2 * h], 65536.f, (float)low) * f[n] * sc[8 * h + g];
                 }
         } else {
-            float acc[kQTiles][4] = {};
+            float acc[kQTiles][4];
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
                 const uint32_t piece = Shape::piece_of(t, i);
@@ -268,7 +304,8 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                 const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
                 for (int n = 0; n < kQTiles; ++n) {
-                    mma16(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
+                    if (i == 0) mma_bf16_first(acc[n], a0, qf[n][0][0], qf[n][0][1]);
+                    else mma16(acc[n], a0, qf[n][2 * i][0], qf[n][2 * i][1]);
                     mma16(acc[n], a1, qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
                 }
             }
@@ -351,8 +388,8 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                                         code_pair(vw[2][w], vw[3][w], b), code_pair(vw[2][w], vw[3][w], b + 1)};
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(c, af, pf[n][0], pf[n][1]);
+                    float c[4];
+                    mma_f16_first(c, af, pf[n][0], pf[n][1]);
                     o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + c[1]);
                     o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + c[3]);
                 }
@@ -364,12 +401,12 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                 uint32_t af[4];
                 const uint32_t key = (lane & 7) + 8 * (lane >> 4), piece = 2 * i + ((lane >> 3) & 1);
                 ldsm4_trans(af, v_addr + Shape::swizzle(key, piece));
-                float third[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16(third, af, pf[kQTiles - 1][0], pf[kQTiles - 1][1]);
+                float third[4];
+                mma_bf16_first(third, af, pf[kQTiles - 1][0], pf[kQTiles - 1][1]);
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16(c, af, pf[n][0], pf[n][1]);
+                    float c[4];
+                    mma_bf16_first(c, af, pf[n][0], pf[n][1]);
                     o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + (c[1] + third[n]));
                     o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + (c[3] + third[2 + n]));
                 }
@@ -415,9 +452,11 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
         if (n_slots == 1) {
             a.out[query * a.out_stride + (size_t)head * D + c] = sum == 0.f ? 0.f : val / sum;
         } else {
-            float *p = a.scratch + (((size_t)query * a.n_heads + head) * n_slots + s.slot) * (D + 2);
-            p[2 + c] = val;
-            if (c == 0) p[0] = top, p[1] = sum;
+            const size_t at_slot = ((size_t)query * a.n_heads + head) * n_slots + s.slot;
+            a.scratch[at_slot * D + c] = val;
+            if (c == 0)
+                *reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * n_slots * D + 2 * at_slot) =
+                    make_float2(top, sum);
         }
     }
 }

@@ -37,6 +37,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// x, at least -10000 (where ex2 gives 0, and 0 times it is 0); a NaN stays.
+__device__ __forceinline__ float floored(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(-10000.f));
+    return y;
+}
 // An order on (value, index) as one number: larger is better, the lowest index first among equals (0 and -0 are).
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
     const uint32_t u = __float_as_uint(x + 0.f);
@@ -159,9 +165,9 @@ log_probs_kernel(LogProbArgs a) {
         const float v[4] = {v0, v1, v2, v3};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // (the difference first: its rounding counts for this entry alone)
-            const float d = v[e] - base, w = ex2(d * kLog2E);
+            const float d = floored(v[e] - base), w = ex2(d * kLog2E);
             s += w;
-            t = w == 0.f ? t : fmaf(d, w, t);
+            t = fmaf(d, w, t);
         }
     };
     const float4 *xv = reinterpret_cast<const float4 *>(x + ext.lo + ext.head);
@@ -223,14 +229,21 @@ log_probs_top_kernel(LogProbArgs a) {
     for (uint32_t i = 0; i <= kHeld * 4; ++i) m = fmaxf(m, v[i]);
     float s = 0.f, t = 0.f;
     const float base = m > -INFINITY ? m : 0.f;
-    uint32_t at = 0xffffffffu;  // the lowest index of the thread's best value
+    uint32_t which = kHeld * 4;  // the first of the thread's entries that has its best value
 #pragma unroll
-    for (int i = kHeld * 4; i >= 0; --i) {
-        const float d = v[i] - base, w = ex2(d * kLog2E);
+    for (int i = kHeld * 4 - 1; i >= 0; --i) {
+        const float d = floored(v[i] - base), w = ex2(d * kLog2E);
         s += w;
-        t = w == 0.f ? t : fmaf(d, w, t);
-        if (v[i] == m && there(i)) at = min(at, index_of(i));
+        t = fmaf(d, w, t);
+        if (v[i] == m) which = i;
     }
+    {
+        const float d = floored(v[kHeld * 4] - base), w = ex2(d * kLog2E);
+        s += w;
+        t = fmaf(d, w, t);
+    }
+    uint32_t at = which < kHeld * 4 && there(which) ? index_of(which) : 0xffffffffu;
+    if (v[kHeld * 4] == m) at = min(at, single);  // (the single entry may lie in front of or behind the others; none: no index)
     // the threads' best entries, sorted: the n_top-th of them is no better than the slice's n_top-th entry
     uint64_t list = sorted(at != 0xffffffffu ? rank_key(m, at) : 0ull, lane);
     best_of[warp][lane] = list;
@@ -250,12 +263,22 @@ log_probs_top_kernel(LogProbArgs a) {
     const uint32_t bound_index = bound ? key_index(bound) : 0xffffffffu;
     auto enters = [&](uint32_t i) { return v[i] >= bound_value && there(i) && (v[i] > bound_value || index_of(i) <= bound_index); };
     if (m >= bound_value) {
+        uint32_t as_good = 0;  // (most threads have one such entry at most, the one they know)
 #pragma unroll
-        for (uint32_t i = 0; i <= kHeld * 4; ++i)
-            if (enters(i)) {
-                const uint32_t at = atomicAdd(&n_candidates, 1u);
-                if (at < kCandidates) candidates[at] = rank_key(v[i], index_of(i));
+        for (uint32_t i = 0; i <= kHeld * 4; ++i) as_good += v[i] >= bound_value;
+        if (as_good == 1 && at != 0xffffffffu) {
+            if (m > bound_value || at <= bound_index) {
+                const uint32_t place = atomicAdd(&n_candidates, 1u);
+                if (place < kCandidates) candidates[place] = rank_key(m, at);
             }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i <= kHeld * 4; ++i)
+                if (enters(i)) {
+                    const uint32_t place = atomicAdd(&n_candidates, 1u);
+                    if (place < kCandidates) candidates[place] = rank_key(v[i], index_of(i));
+                }
+        }
     }
     __syncthreads();
     const uint32_t n = n_candidates;

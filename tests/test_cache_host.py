@@ -96,9 +96,14 @@ PREFIXES = [
 @pytest.mark.parametrize("change,text", PREFIXES + [
     (dict(batch=3), "the cache has 2 slots"), (dict(heads=5), "n_kv_heads must divide n_heads"), (dict(q=None), "q is null"),
     (dict(out=None), "out is null"), (dict(q_stride=32), "q: rows of 64"), (dict(out_stride=63), "out: rows of 64"),
-    (dict(kv_len=None), "kv_len is null"), (dict(heads=1 << 17), "more than one call takes")])
+    (dict(kv_len=None), "kv_len is null"), (dict(wide=True, scratch=None), "scratch is null"),
+    (dict(wide=True, scratch=P + 8), "no 16-byte boundary"), (dict(heads=1 << 17), "more than one call takes")])
 def test_attend(change, text):
-    refused(attend(cache(), **change), text)
+    change = dict(change)
+    if change.pop("wide", False):   # a shape whose keys are split over blocks
+        refused(attend(cache(rows=5000, d=128), q_stride=512, out_stride=512, **change), text)
+    else:
+        refused(attend(cache(), **change), text)
 
 
 @pytest.mark.parametrize("change,text", PREFIXES + [
