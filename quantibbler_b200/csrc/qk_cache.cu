@@ -477,6 +477,18 @@ bool aligned_rows(const CacheView &v) { return aligned(v.k) && aligned(v.v); }
 
 constexpr size_t kWantBlocks = 148 * 8, kMinChunk = 128;
 
+// The tile kernel takes 128 query rows to an SM: how often the keys (64 to a block, two blocks at a time) are split so
+// that the SMs have work.
+uint32_t tile_splits(size_t tiles, size_t keys) {
+    const size_t pairs = qk::ceil_div(keys, 128);
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>({64, pairs, 148 / tiles}));
+}
+size_t tiles_of(const qk_kv_cache *c, size_t queries, size_t n_heads) {
+    return qk::ceil_div(queries * (n_heads / c->n_kv_heads), 128) * c->n_kv_heads;
+}
+// More query rows than this on a prefix go through the tile kernel.  (A block of the other kernel takes eight rows.)
+constexpr size_t kTileRows = 16;
+
 Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_heads) {
     Plan pl{};
     const size_t group = n_heads / c->n_kv_heads;
@@ -484,7 +496,9 @@ Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_h
         const size_t most = std::min<size_t>(128, qk::ceil_div(rows, kMinChunk));
         return (uint32_t)std::max<size_t>(1, std::min(most, qk::ceil_div(kWantBlocks, blocks)));
     };
-    if (prefix_len) {
+    if (prefix_len && batch * group > kTileRows) {
+        pl.prefix_splits = tile_splits(tiles_of(c, batch, n_heads), prefix_len);
+    } else if (prefix_len) {
         pl.prefix_subs = (uint32_t)qk::ceil_div(batch * group, 8);
         pl.prefix_splits = splits(pl.prefix_subs * c->n_kv_heads, prefix_len);
         pl.prefix_chunk = (uint32_t)(qk::ceil_div(qk::ceil_div(prefix_len, pl.prefix_splits), 64) * 64);
@@ -497,8 +511,39 @@ Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_h
     return pl;
 }
 
+struct PortionPlan {
+    uint32_t prefix_splits, own_splits;
+};
+PortionPlan plan_portion(const qk_kv_cache *c, size_t first_row, size_t prefix_len, size_t tokens, size_t n_heads) {
+    const size_t tiles = tiles_of(c, tokens, n_heads);
+    return {prefix_len ? tile_splits(tiles, prefix_len) : 0, tile_splits(tiles, first_row + tokens)};
+}
+
 size_t partial_bytes(size_t queries, size_t n_heads, size_t slots, size_t d) {
     return slots > 1 ? queries * n_heads * slots * (d + 2) * sizeof(float) : 0;
+}
+
+qk_status join(qk_ctx *c, const qk::AttendArgs &a, uint32_t n_slots, uint32_t d) {
+    if (n_slots == 1) return QK_OK;
+    const dim3 grid(a.n_queries * a.n_heads);
+    if (d == 128) QK_PDL(c, join_kernel<128>, grid, dim3(128), 0, a, n_slots);
+    else QK_PDL(c, join_kernel<64>, grid, dim3(128), 0, a, n_slots);
+    QK_CUDA(cudaGetLastError());
+    c->launches++;
+    return QK_OK;
+}
+
+qk::TileArgs tile_args(const qk::AttendArgs &a, uint32_t n_splits, uint32_t slot0, uint32_t n_slots) {
+    qk::TileArgs t{};
+    t.q = a.q, t.q_stride = a.q_stride, t.out = a.out, t.out_stride = a.out_stride, t.scratch = a.scratch;
+    t.n_queries = a.n_queries, t.n_heads = a.n_heads;
+    t.n_splits = n_splits, t.slot0 = slot0, t.n_slots = n_slots;
+    return t;
+}
+qk_status prefix_tiles(qk_ctx *c, const CacheView &pre, const qk::AttendArgs &a, uint32_t n_splits, uint32_t n_slots) {
+    qk::TileArgs t = tile_args(a, n_splits, 0, n_slots);
+    t.seq = a.prefix_seq, t.n_keys = a.prefix_len;
+    return qk::attend_tiles(c, pre, t);
 }
 
 template <bool kI8, int D, int kMost>
@@ -510,16 +555,15 @@ qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, con
     QK_PDL(c, (attend_rows_kernel<kI8, D, kMost>), dim3(blocks), dim3(128), smem, own, pre, a, pl);
     QK_CUDA(cudaGetLastError());
     c->launches++;
-    if (pl.n_slots > 1) {
-        QK_PDL(c, join_kernel<D>, dim3(a.n_queries * a.n_heads), dim3(128), 0, a, pl.n_slots);
-        QK_CUDA(cudaGetLastError());
-        c->launches++;
-    }
-    return QK_OK;
+    return join(c, a, pl.n_slots, D);
 }
 template <bool kI8, int D>
 qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, const qk::AttendArgs &a, const Plan &pl) {
-    const uint32_t rows = a.prefix_len ? std::max(pl.own_rows, std::min(8u, a.n_queries * (a.n_heads / own.n_kv))) : pl.own_rows;
+    if (a.prefix_len && !pl.prefix_blocks) {
+        qk_status st = prefix_tiles(c, pre, a, pl.prefix_splits, pl.n_slots);
+        if (st != QK_OK) return st;
+    }
+    const uint32_t rows = pl.prefix_blocks ? std::max(pl.own_rows, std::min(8u, a.n_queries * (a.n_heads / own.n_kv))) : pl.own_rows;
     return rows > 4 ? launch_rows<kI8, D, 2>(c, own, pre, a, pl) : launch_rows<kI8, D, 1>(c, own, pre, a, pl);
 }
 
@@ -530,7 +574,17 @@ qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefi
     if (st != QK_OK) return st;
     std::lock_guard<std::mutex> lock(c->mu);
     const CacheView own = view(cache), pre = view(a.prefix_len ? prefix : nullptr);
-    if (a.kv_len && takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0) {
+    if (takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0) {
+        if ((st = ready_error_word(c)) != QK_OK) return st;
+        if (!a.kv_len) {
+            const PortionPlan pp = plan_portion(cache, a.first_row, a.prefix_len, a.n_queries, a.n_heads);
+            const uint32_t slots = pp.prefix_splits + pp.own_splits;
+            if (a.prefix_len && (st = prefix_tiles(c, pre, a, pp.prefix_splits, slots)) != QK_OK) return st;
+            qk::TileArgs t = tile_args(a, pp.own_splits, pp.prefix_splits, slots);
+            t.seq = a.seq, t.first_row = a.first_row, t.causal = 1;
+            if ((st = qk::attend_tiles(c, own, t)) != QK_OK) return st;
+            return join(c, a, slots, own.d);
+        }
         const Plan pl = plan_rows(cache, a.prefix_len, a.n_queries, a.n_heads);
         if (own.dtype == QK_I8)
             return own.d == 128 ? launch_rows<true, 128>(c, own, pre, a, pl) : launch_rows<true, 64>(c, own, pre, a, pl);
@@ -686,8 +740,9 @@ qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cac
 
 size_t qk_cache_portion_scratch(const qk_kv_cache *cache, size_t first_row, size_t prefix_len, size_t n_tokens,
                                 size_t n_heads) {
-    (void)cache, (void)first_row, (void)prefix_len, (void)n_tokens, (void)n_heads;
-    return 0;
+    if (!cache || cache->n_kv_heads == 0 || n_heads < cache->n_kv_heads || !n_tokens || !takes_rows(cache)) return 0;
+    const PortionPlan pp = plan_portion(cache, first_row, prefix_len, n_tokens, n_heads);
+    return partial_bytes(n_tokens, n_heads, pp.prefix_splits + pp.own_splits, cache->head_dim);
 }
 
 qk_status qk_cache_portion(qk_ctx *ctx, const qk_kv_cache *cache, size_t seq, size_t first_row, const qk_kv_cache *prefix,

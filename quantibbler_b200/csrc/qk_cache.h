@@ -26,4 +26,22 @@ struct AttendArgs {
     float *scratch;
 };
 
+// One launch of the tile kernel (qk_cache_tile.cu): all queries against rows of one slot.
+struct TileArgs {
+    const float *q;
+    size_t q_stride;
+    float *out;
+    size_t out_stride;
+    float *scratch;            // partial results where n_slots > 1: outputs [query][head][slot][d], then {maximum, sum}
+    uint32_t n_queries, n_heads;
+    size_t seq;
+    int32_t causal;            // query t sees rows 0 .. first_row + t; else all see rows 0 .. n_keys - 1
+    uint32_t first_row, n_keys;
+    uint32_t n_splits, slot0, n_slots;  // the keys' splits go to slots slot0 .. of the n_slots of a (query, head)
+    int *error;
+    uint32_t wait_limit;
+};
+// INT8 or bfloat16, head_dim 64 or 128, everything on 16-byte boundaries; the context's error word exists.
+qk_status attend_tiles(qk_ctx *c, const CacheView &cache, TileArgs a);
+
 }  // namespace qk
