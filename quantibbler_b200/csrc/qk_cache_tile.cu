@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "qk_cache.h"
 #include "qk_decoder_dev.cuh"
@@ -128,7 +129,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     constexpr uint32_t kTerms = S::kTerms, kChunks = S::kChunks, kStages = S::kStages;
     qk::pdl_launch();
     extern __shared__ __align__(1024) uint8_t raw_smem[];
-    uint8_t *qs = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
+    uint8_t *qs = raw_smem + (-smem_u32(raw_smem) & 1023u);  // (an offset: the compiler still sees shared memory)
     uint8_t *ring = qs + kTerms * S::kQTermBytes;
     float *scales = reinterpret_cast<float *>(ring + kStages * S::kStageBytes);  // [stage][kScaleFloats]
     float *row_peak = scales + kStages * S::kScaleFloats;                       // [2][128]
@@ -400,71 +401,78 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const bool edge = key0 + (int)kKeys > min(seen0, (int)keys);  // some row of the tile does not see the whole block
             const int limit = min(seen, (int)keys) - key0;                // keys of the block that this row sees
             const float *ks = scales + (g % kStages) * S::kScaleFloats, *vs = ks + kKeys;
-            float top = -INFINITY;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                uint32_t s[32];
-                tmem_ld32(unit + 32 * part, s);
-                tmem_ld_wait();
-                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    float4 x = make_float4(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]),
-                                           __uint_as_float(s[e + 3]));
-                    if constexpr (kI8) {
-                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * part + e);
-                        const float2 lo = __fmul2_rn(make_float2(x.x, x.y), make_float2(k4.x, k4.y));
-                        const float2 hi = __fmul2_rn(make_float2(x.z, x.w), make_float2(k4.z, k4.w));
-                        x = make_float4(lo.x, lo.y, hi.x, hi.y);
-                    }
-                    if (edge) {
-                        x.x = 32 * part + e < limit ? x.x : -INFINITY;
-                        x.y = 32 * part + e + 1 < limit ? x.y : -INFINITY;
-                        x.z = 32 * part + e + 2 < limit ? x.z : -INFINITY;
-                        x.w = 32 * part + e + 3 < limit ? x.w : -INFINITY;
-                    }
-                    t4[0] = fmaxf(t4[0], x.x), t4[1] = fmaxf(t4[1], x.y), t4[2] = fmaxf(t4[2], x.z), t4[3] = fmaxf(t4[3], x.w);
-                }
-                top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
-            }
-            const float m_new = fmaxf(m, top * f);
-            const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
-            float alpha = ex2(m - base);
-            m = m_new;
-            const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
+            float alpha;
             float2 sum = make_float2(0.f, 0.f);
+            // (kEdge in the type: a select per score would be paid in every block)
+            auto weights = [&](auto edge_tag) {
+                constexpr bool kEdge = decltype(edge_tag)::value;
+                float top = -INFINITY;
 #pragma unroll
-            for (int part = 0; part < 4; ++part) {
-                uint32_t s[16], t[kTerms][8];
-                tmem_ld16(unit + 16 * part, s);
-                tmem_ld_wait();
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t s[32];
+                    tmem_ld32(unit + 32 * part, s);
+                    tmem_ld_wait();
+                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-                    const int at = 16 * part + 2 * e;
-                    if constexpr (kI8) x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(ks + at));
-                    x = __ffma2_rn(x, f2, base2);
-                    if (edge) {
-                        x.x = at < limit ? x.x : -INFINITY;
-                        x.y = at + 1 < limit ? x.y : -INFINITY;
-                    }
-                    x = make_float2(ex2(x.x), ex2(x.y));
-                    sum = __fadd2_rn(sum, x);
-                    if constexpr (kI8) {
-                        x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(vs + at));
-                        if (edge) {  // (a key that this row does not see may have the scale NaN)
-                            x.x = at < limit ? x.x : 0.f;
-                            x.y = at + 1 < limit ? x.y : 0.f;
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 x = make_float4(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]),
+                                               __uint_as_float(s[e + 3]));
+                        if constexpr (kI8) {
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * part + e);
+                            const float2 lo = __fmul2_rn(make_float2(x.x, x.y), make_float2(k4.x, k4.y));
+                            const float2 hi = __fmul2_rn(make_float2(x.z, x.w), make_float2(k4.z, k4.w));
+                            x = make_float4(lo.x, lo.y, hi.x, hi.y);
                         }
+                        if constexpr (kEdge) {
+                            x.x = 32 * part + e < limit ? x.x : -INFINITY;
+                            x.y = 32 * part + e + 1 < limit ? x.y : -INFINITY;
+                            x.z = 32 * part + e + 2 < limit ? x.z : -INFINITY;
+                            x.w = 32 * part + e + 3 < limit ? x.w : -INFINITY;
+                        }
+                        t4[0] = fmaxf(t4[0], x.x), t4[1] = fmaxf(t4[1], x.y), t4[2] = fmaxf(t4[2], x.z), t4[3] = fmaxf(t4[3], x.w);
                     }
-                    uint32_t w[3];
-                    terms_of<kI8>(x.x, x.y, w);
-#pragma unroll
-                    for (uint32_t n = 0; n < kTerms; ++n) t[n][e] = w[n];
+                    top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
                 }
+                const float m_new = fmaxf(m, top * f);
+                const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
+                alpha = ex2(m - base);
+                m = m_new;
+                const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
 #pragma unroll
-                for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(unit + S::weight_col(n) + 8 * part, t[n]);
-            }
+                for (int part = 0; part < 4; ++part) {
+                    uint32_t s[16], t[kTerms][8];
+                    tmem_ld16(unit + 16 * part, s);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+                        const int at = 16 * part + 2 * e;
+                        if constexpr (kI8) x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(ks + at));
+                        x = __ffma2_rn(x, f2, base2);
+                        if constexpr (kEdge) {
+                            x.x = at < limit ? x.x : -INFINITY;
+                            x.y = at + 1 < limit ? x.y : -INFINITY;
+                        }
+                        x = make_float2(ex2(x.x), ex2(x.y));
+                        sum = __fadd2_rn(sum, x);
+                        if constexpr (kI8) {
+                            x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(vs + at));
+                            if constexpr (kEdge) {  // (a key that this row does not see may have the scale NaN)
+                                x.x = at < limit ? x.x : 0.f;
+                                x.y = at + 1 < limit ? x.y : 0.f;
+                            }
+                        }
+                        uint32_t w[3];
+                        terms_of<kI8>(x.x, x.y, w);
+#pragma unroll
+                        for (uint32_t n = 0; n < kTerms; ++n) t[n][e] = w[n];
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(unit + S::weight_col(n) + 8 * part, t[n]);
+                }
+            };
+            if (edge) weights(std::true_type{});
+            else weights(std::false_type{});
             l = fmaf(l, alpha, sum.x + sum.y);
             if constexpr (kI8) {
                 const int e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
