@@ -4,8 +4,10 @@
 // The queries that read one kv head are the rows of one product: row r is query r / group, head r % group of the kv
 // head, 128 rows to a CTA, which takes a range of keys 64 at a time.  Two units of four warps take the key blocks in
 // turn, a thread owns a row (no shuffles): running maximum, sum and output in registers, the two units joined at the
-// end.  While one unit is at its exponentials the tensor core works for the other.  The weights go back to tensor
-// memory as the A operand; v is read as it lies (MN-major B).  Three warps bring the key blocks in.
+// end.  While one unit is at its exponentials the tensor core works for the other; a block's output is read out when
+// the maximum of the unit's next block is known.  The weights go back to tensor
+// memory as the A operand; v is read as it lies (MN-major B).  Three warps bring the
+// key blocks in, three the value blocks.
 //
 // Exactness.  INT8 rows: codes as float16 are exact (three warps convert them on their way into shared memory); q is
 // two float16 terms after scaling by a power of two per row (22 bits), and so are the weights times the value scales,
@@ -30,10 +32,11 @@ using qk::CacheView;
 using qk::TileArgs;
 
 constexpr uint32_t kRows = 128, kKeys = 64;  // query rows of a CTA, keys of a block
-constexpr uint32_t kThreads = 384, kLoaders = 96, kFirstLoader = 8, kMmaWarp = 11;
-constexpr int kUnitRegs = 208, kOtherRegs = 88, kLaunchRegs = 168;
-static_assert(2 * 128 * kUnitRegs + 128 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
-constexpr uint32_t kTmemCols = 512, kUnitCols = 256, kOutCol = 128;  // a unit's columns: scores, weights, outputs
+constexpr uint32_t kThreads = 512, kLoaders = 96, kKeyWarp = 8, kValueWarp = 11, kScaleWarp = 14, kMmaWarp = 15;  // three warps a loader
+constexpr int kUnitRegs = 184, kOtherRegs = 72, kLaunchRegs = 128;
+static_assert(256 * kUnitRegs + 256 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kAhead = 2;  // a block's scores are formed when the product of the unit's block before is under way
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;
 constexpr uint32_t kWaitLimit = 1u << 22;
@@ -44,13 +47,23 @@ struct TileShape {
     static constexpr uint32_t kChunks = D / 64;                        // of 64 channels, rows of 128 bytes
     static constexpr uint32_t kChunkBytes = kKeys * 128, kTileBytes = kChunks * kChunkBytes;
     static constexpr uint32_t kQChunkBytes = kRows * 128, kQTermBytes = kChunks * kQChunkBytes;
-    static constexpr uint32_t kStages = kI8 || D == 64 ? 4 : 3, kStageBytes = 2 * kTileBytes;
-    static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a stage's key and value scales, and E
-    static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kStages * kStageBytes + kStages * kScaleFloats * 4 + 1024 + 256;
+    static constexpr uint32_t kStages = kI8 || D == 64 ? 4 : 3;        // of the keys' ring, and of the values'
+    static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a block's key and value scales, and E
+    static constexpr uint32_t kRingBytes = 2 * kStages * kTileBytes;
+    static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 384;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
-    static_assert(kStages * kStageBytes >= (D * kRows + 4 * kRows) * 4, "the units' exchange lies in the ring");
-    // Column of the weights' term n; the third lies over scores that have been read.
-    __device__ static constexpr uint32_t weight_col(uint32_t n) { return n == 2 ? 0 : 64 + 32 * n; }
+    // Tensor memory.  INT8: q's terms (the A operand of the scores, so that shared memory is not read for them in every
+    // block), a unit's scores, over which its weights lie (16 columns of scores become eight of either term), its
+    // outputs.  bfloat16, whose terms are three, has q in shared memory and the first two terms of the weights behind
+    // the scores, the third over scores that have been read.
+    static constexpr bool kQInTmem = kI8;
+    __device__ static constexpr uint32_t q_col(uint32_t term) { return 64 * term; }
+    __device__ static constexpr uint32_t score_col(uint32_t u) { return kI8 ? 128 + 64 * u : 256 * u; }
+    __device__ static constexpr uint32_t out_col(uint32_t u) { return kI8 ? 256 + 128 * u : 256 * u + 128; }
+    __device__ static constexpr uint32_t weight_col(uint32_t term, uint32_t step) {  // of a step of 16 keys, from score_col
+        return kI8 ? 16 * step + 8 * term : (term == 2 ? 0 : 64 + 32 * term) + 8 * step;
+    }
+    static_assert(kRingBytes >= (D * kRows + 5 * kRows) * 4, "the units' exchange lies in the ring");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -131,10 +144,12 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *qs = raw_smem + (-smem_u32(raw_smem) & 1023u);  // (an offset: the compiler still sees shared memory)
     uint8_t *ring = qs + kTerms * S::kQTermBytes;
-    float *scales = reinterpret_cast<float *>(ring + kStages * S::kStageBytes);  // [stage][kScaleFloats]
-    float *row_peak = scales + kStages * S::kScaleFloats;                       // [2][128]
-    uint64_t *q_full = reinterpret_cast<uint64_t *>(row_peak + 256);
-    uint64_t *full = q_full + 1, *empty = full + kStages, *s_full = empty + kStages, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint8_t *v_ring = ring + kStages * S::kTileBytes;
+    float *scales = reinterpret_cast<float *>(ring + S::kRingBytes);             // [stage of the values][kScaleFloats]
+    float *row_factor = scales + kStages * S::kScaleFloats;                     // [128]
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(row_factor + 128);
+    uint64_t *k_full = q_full + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages, *v_empty = v_full + kStages;
+    uint64_t *s_full = v_empty + kStages, *p_full = s_full + 2, *o_full = p_full + 2;
     uint64_t *drain = o_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -151,8 +166,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     if (threadIdx.x == 0) {
         mbar_init(q_full, 8);
         for (uint32_t s = 0; s < kStages; ++s) {
-            mbar_init(full + s, kLoaders / 32);
-            mbar_init(empty + s, 1);
+            mbar_init(k_full + s, kLoaders / 32);
+            mbar_init(k_empty + s, 1);
+            mbar_init(v_full + s, kLoaders / 32 + (kI8 ? 1 : 0));
+            mbar_init(v_empty + s, 1);
         }
         for (int u = 0; u < 2; ++u) {
             mbar_init(s_full + u, 1);
@@ -178,20 +195,30 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     const size_t line0 = (a.seq * c.n_kv + kvh) * (size_t)c.rows + (size_t)block0 * kKeys;  // first key's row
     const uint32_t keys = n_blocks ? min(n_keys - block0 * kKeys, n_blocks * kKeys) : 0;    // of this CTA
 
-    if (warp >= kFirstLoader) {
+    if (warp >= kKeyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp != kMmaWarp) {
-            // ---- key blocks into the ring; rows past the end are zeros
-            const uint32_t tid = threadIdx.x - kFirstLoader * 32;
+        if (warp < kScaleWarp) {
+            // ---- key blocks into their ring, value blocks into theirs; rows past the end are zeros
+            const bool is_v = warp >= kValueWarp;
+            const uint32_t tid = threadIdx.x - (is_v ? kValueWarp : kKeyWarp) * 32;
             constexpr uint32_t kRowBytes = kI8 ? D : 2 * D, kPieces = kRowBytes / 16, kStep = kLoaders / kPieces;
             constexpr uint32_t kPasses = (kKeys + kStep - 1) / kStep;
-            const uint32_t piece = tid % kPieces, first = tid / kPieces;  // a thread's rows: first, first + kStep, ..
-            const uint8_t *kb = static_cast<const uint8_t *>(c.k) + line0 * kRowBytes + piece * 16;
-            const uint8_t *vb = static_cast<const uint8_t *>(c.v) + line0 * kRowBytes + piece * 16;
+            // A thread's piece, and its rows: first, first + kStep, ..  (INT8, head size 128: eight threads store two rows of
+            // one chunk of 64 channels and meet no bank twice.)
+            const uint32_t piece = kI8 && D == 128 ? tid / 8 % 2 * 4 + tid % 4 : tid % kPieces;
+            const uint32_t first = kI8 && D == 128 ? tid / 16 * 2 + tid / 4 % 2 : tid / kPieces;
+            const uint8_t *base = static_cast<const uint8_t *>(is_v ? c.v : c.k) + line0 * kRowBytes + piece * 16;
+            uint8_t *tiles = is_v ? v_ring : ring;
+            uint64_t *fulls = is_v ? v_full : k_full, *empties = is_v ? v_empty : k_empty;
             bool ok = true;
+            auto hand_over = [&](uint64_t *bar) {
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
             if constexpr (kI8) {
-                uint4 held[kPasses];
-                auto load = [&](const uint8_t *base, uint32_t g) {
+                uint4 held[kPasses];  // the next block's, on their way while this one is converted
+                auto load = [&](uint32_t g) {
 #pragma unroll
                     for (uint32_t i = 0; i < kPasses; ++i) {
                         const uint32_t row = first + i * kStep, key = g * kKeys + row;
@@ -199,9 +226,14 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                                                             : make_uint4(0u, 0u, 0u, 0u);
                     }
                 };
-                auto store = [&](uint8_t *to) {  // sixteen codes: two pieces of eight float16
+                load(0);
+                for (uint32_t g = 0; g < n_blocks; ++g) {
+                    const uint32_t s = g % kStages;
+                    ok = mbar_wait(empties + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
+                    if (!ok) break;
+                    uint8_t *tile_at = tiles + s * S::kTileBytes + piece / 4 * S::kChunkBytes;
 #pragma unroll
-                    for (uint32_t i = 0; i < kPasses; ++i) {
+                    for (uint32_t i = 0; i < kPasses; ++i) {  // sixteen codes: two pieces of eight float16
                         const uint32_t row = first + i * kStep;
                         if (row >= kKeys) break;
                         uint32_t w[8];
@@ -209,177 +241,188 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         codes_to_f16(held[i].y, w[2], w[3]);
                         codes_to_f16(held[i].z, w[4], w[5]);
                         codes_to_f16(held[i].w, w[6], w[7]);
-                        uint8_t *line = to + piece / 4 * S::kChunkBytes + row * 128;
-                        const uint32_t at = 2 * (piece % 4), flip = piece / 4;  // (the two chunks in turn: no bank twice)
-#pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            const bool second = (h ^ flip) != 0;
-                            *reinterpret_cast<uint4 *>(line + (((at + (second ? 1 : 0)) ^ (row & 7)) << 4)) =
-                                second ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        const uint32_t at = 2 * (piece % 4);
+                        *reinterpret_cast<uint4 *>(tile_at + row * 128 + ((at ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4 *>(tile_at + row * 128 + (((at + 1) ^ (row & 7)) << 4)) =
+                            make_uint4(w[4], w[5], w[6], w[7]);
                     }
-                };
-                int e_max = -100;
-                load(kb, 0);
-                for (uint32_t g = 0; g < n_blocks; ++g) {
-                    const uint32_t s = g % kStages;
-                    float sc[4] = {0.f, 0.f, 0.f, 0.f};  // (first warp) key and value scales of keys lane, lane + 32
-                    if (warp == kFirstLoader) {
-#pragma unroll
-                        for (uint32_t i = 0; i < 2; ++i) {
-                            const uint32_t key = g * kKeys + lane + 32 * i;
-                            if (key < keys) sc[i] = c.k_scale[line0 + key], sc[2 + i] = c.v_scale[line0 + key];
-                        }
-                    }
-                    ok = mbar_wait(empty + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
-                    if (!ok) break;
-                    uint8_t *stage = ring + s * S::kStageBytes;
-                    store(stage);
-                    load(vb, g);
-                    if (warp == kFirstLoader) {
-                        const uint32_t top = __reduce_max_sync(
-                            0xffffffffu, max(__float_as_uint(fabsf(sc[2])), __float_as_uint(fabsf(sc[3]))));
-                        e_max = max(e_max, exponent_of(top));
-                        const float mul = pow2(-1 - e_max);
-                        float *dst = scales + s * S::kScaleFloats;
-                        dst[lane] = sc[0], dst[32 + lane] = sc[1];
-                        dst[kKeys + lane] = sc[2] * mul * kWeightScale, dst[kKeys + 32 + lane] = sc[3] * mul * kWeightScale;
-                        if (lane == 0) reinterpret_cast<int *>(dst)[2 * kKeys] = e_max;
-                    }
-                    store(stage + S::kTileBytes);
-                    if (g + 1 < n_blocks) load(kb, g + 1);
-                    fence_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + s);
+                    load(g + 1);
+                    hand_over(fulls + s);
                 }
             } else {
-                auto copy = [&](const uint8_t *base, uint8_t *to, uint32_t g) {
+                for (uint32_t g = 0; g < n_blocks; ++g) {
+                    const uint32_t s = g % kStages;
+                    ok = mbar_wait(empties + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
+                    if (!ok) break;
+                    uint8_t *tile_at = tiles + s * S::kTileBytes + piece / 8 * S::kChunkBytes;
 #pragma unroll
                     for (uint32_t i = 0; i < kPasses; ++i) {
                         const uint32_t row = first + i * kStep, key = g * kKeys + row;
                         if (row >= kKeys) break;
                         const bool live = key < keys;
-                        const uint32_t at = smem_u32(to + piece / 8 * S::kChunkBytes + row * 128 + (((piece % 8) ^ (row & 7)) << 4));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at),
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_u32(tile_at + row * 128 + (((piece % 8) ^ (row & 7)) << 4))),
                                      "l"(base + (live ? (size_t)key * kRowBytes : 0)), "r"(live ? 16u : 0u)
                                      : "memory");
                     }
-                };
-                for (uint32_t g = 0; g < n_blocks + 1; ++g) {  // (a block is handed over when the next one is under way)
-                    if (g < n_blocks) {
-                        ok = mbar_wait(empty + g % kStages, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
-                        if (!ok) break;
-                        uint8_t *stage = ring + g % kStages * S::kStageBytes;
-                        copy(kb, stage, g);
-                        copy(vb, stage + S::kTileBytes, g);
-                    }
                     asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (g == 0) continue;
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    fence_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + (g - 1) % kStages);
+                    if (g) {  // (a block is handed over when the next one is under way)
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        hand_over(fulls + (g - 1) % kStages);
+                    }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
+                if (ok && n_blocks) hand_over(fulls + (n_blocks - 1) % kStages);
             }
             if (!ok) *abort_flag = 1;
+        } else if (warp == kScaleWarp) {
+            // ---- INT8: the scales, those of the values relative to the running maximum's power of two
+            if constexpr (kI8) {
+                float sc[4];  // key and value scales of keys lane, lane + 32 of the next block
+                auto load = [&](uint32_t g) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const uint32_t key = g * kKeys + lane + 32 * i;
+                        sc[i] = key < keys ? c.k_scale[line0 + key] : 0.f, sc[2 + i] = key < keys ? c.v_scale[line0 + key] : 0.f;
+                    }
+                };
+                int e_max = -100;
+                bool ok = true;
+                load(0);
+                for (uint32_t g = 0; g < n_blocks; ++g) {
+                    const uint32_t s = g % kStages;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu,
+                                                           max(__float_as_uint(fabsf(sc[2])), __float_as_uint(fabsf(sc[3]))));
+                    e_max = max(e_max, exponent_of(top));
+                    const float mul = pow2(-1 - e_max);
+                    ok = mbar_wait(v_empty + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
+                    if (!ok) break;
+                    float *dst = scales + s * S::kScaleFloats;
+                    dst[lane] = sc[0], dst[32 + lane] = sc[1];
+                    dst[kKeys + lane] = sc[2] * mul * kWeightScale, dst[kKeys + 32 + lane] = sc[3] * mul * kWeightScale;
+                    if (lane == 0) reinterpret_cast<int *>(dst)[2 * kKeys] = e_max;
+                    load(g + 1);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(v_full + s);
+                }
+                if (!ok) *abort_flag = 1;
+            }
         } else {
             // ---- products
             constexpr uint32_t kind = kI8 ? 0 : 1;
             const uint32_t idesc_s = instruction(kKeys, 0, kind), idesc_o = instruction(D, 1, kind);
             const uint64_t q_desc = umma_desc(smem_u32(qs)), k_desc = umma_desc(smem_u32(ring));
             // (MN-major: chunks of 64 channels kChunkBytes apart)
-            const uint64_t v_desc = umma_desc(smem_u32(ring) + S::kTileBytes) | ((uint64_t)(S::kChunkBytes >> 4) << 16);
+            const uint64_t v_desc = umma_desc(smem_u32(v_ring)) | ((uint64_t)(S::kChunkBytes >> 4) << 16);
             auto scores = [&](uint32_t g) {  // (one lane) small terms first
-                const uint64_t kd = k_desc + (uint64_t)((g % kStages) * (S::kStageBytes >> 4));
-                const uint32_t dst = tmem + kUnitCols * (g & 1);
+                const uint64_t kd = k_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
+                const uint32_t dst = tmem + S::score_col(g & 1);
 #pragma unroll
                 for (uint32_t i = 0; i < kTerms; ++i)
 #pragma unroll
-                    for (uint32_t k = 0; k < 4 * kChunks; ++k)
-                        mma_ss(dst, q_desc + (((kTerms - 1 - i) * S::kQTermBytes + k / 4 * S::kQChunkBytes + k % 4 * 32) >> 4),
-                               kd + ((k / 4 * S::kChunkBytes + k % 4 * 32) >> 4), idesc_s, i + k != 0);
+                    for (uint32_t k = 0; k < 4 * kChunks; ++k) {
+                        const uint64_t kk = kd + ((k / 4 * S::kChunkBytes + k % 4 * 32) >> 4);
+                        if constexpr (S::kQInTmem)
+                            mma_ts(dst, tmem + S::q_col(kTerms - 1 - i) + 8 * k, kk, idesc_s, i + k != 0);
+                        else
+                            mma_ss(dst, q_desc + (((kTerms - 1 - i) * S::kQTermBytes + k / 4 * S::kQChunkBytes + k % 4 * 32) >> 4),
+                                   kk, idesc_s, i + k != 0);
+                    }
+                umma_commit(k_empty + g % kStages);
                 umma_commit(s_full + (g & 1));
             };
             auto values = [&](uint32_t g) {  // (one lane)
-                const uint64_t vd = v_desc + (uint64_t)((g % kStages) * (S::kStageBytes >> 4));
-                const uint32_t unit = tmem + kUnitCols * (g & 1);
+                const uint64_t vd = v_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
+                const uint32_t weights = tmem + S::score_col(g & 1), dst = tmem + S::out_col(g & 1);
 #pragma unroll
                 for (uint32_t i = 0; i < kTerms; ++i)
 #pragma unroll
                     for (uint32_t k = 0; k < kKeys / 16; ++k)
-                        mma_ts(unit + kOutCol, unit + S::weight_col(kTerms - 1 - i) + k * 8, vd + ((k * 2048) >> 4), idesc_o,
+                        mma_ts(dst, weights + S::weight_col(kTerms - 1 - i, k), vd + ((k * 2048) >> 4), idesc_o,
                                i + k != 0);
-                umma_commit(empty + g % kStages);
+                umma_commit(v_empty + g % kStages);
                 umma_commit(o_full + (g & 1));
             };
-            bool ok = mbar_wait(q_full, 0, abort_flag, a.wait_limit);
-            for (uint32_t g = 0; g < 2 && g < n_blocks && ok; ++g) {
-                ok = mbar_wait(full + g % kStages, 0, abort_flag, a.wait_limit);
-                if (!ok) break;
+            auto form = [&](uint32_t g) {  // (over columns whose weights an earlier product has read)
+                if (!mbar_wait(k_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) scores(g);
                 __syncwarp();
-            }
+                return true;
+            };
+            bool ok = mbar_wait(q_full, 0, abort_flag, a.wait_limit);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (uint32_t g = 0; g < kAhead && g < n_blocks && ok; ++g) ok = form(g);
             for (uint32_t g = 0; g < n_blocks && ok; ++g) {
-                ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
+                ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                if (ok) ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) values(g);
                 __syncwarp();
-                if (g + 2 >= n_blocks) continue;
-                ok = mbar_wait(full + (g + 2) % kStages, ((g + 2) / kStages) & 1, abort_flag, a.wait_limit);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) scores(g + 2);  // (over scores that the unit has read: it has handed in their weights)
-                __syncwarp();
+                if (g + kAhead < n_blocks) ok = form(g + kAhead);
             }
             if (!ok) *abort_flag = 1;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUnitRegs));
         const uint32_t u = warp / 4, r = threadIdx.x % 128;
-        const uint32_t row = min(row0 + r, n_rows - 1), query = row / group, head = kvh * group + row % group;
-        // q: a unit takes one chunk of 64 channels, a thread its row
-        float f = kLog2E / sqrtf((float)D);  // what turns a raw score into log2 units
+        const uint32_t query = min(row0 + r, n_rows - 1) / group;
+        // q: a warp takes sixteen rows, D / 4 lanes a row
         {
-            const bool live = r < rows && u < kChunks;
-            const float *src = a.q + query * a.q_stride + (size_t)head * D + u * 64;
-            float x[64];
+            constexpr uint32_t kLanes = D / 4, kSide = 32 / kLanes;
+            const uint32_t ch = 4 * (lane % kLanes);
+            const float unit_scale = kLog2E / sqrtf((float)D);
+#pragma unroll 4
+            for (uint32_t i = 0; i < 16; i += kSide) {
+                const uint32_t at = warp * 16 + i + lane / kLanes, which = row0 + min(at, rows - 1);
+                float4 x = *reinterpret_cast<const float4 *>(a.q + (which / group) * a.q_stride +
+                                                             (size_t)(kvh * group + which % group) * D + ch);
+                float factor = unit_scale, mul = 1.f;  // factor: what turns a raw score into log2 units
+                if constexpr (kI8) {
+                    uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
+                                       max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) {
-                const float4 t = live ? *reinterpret_cast<const float4 *>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[i] = t.x, x[i + 1] = t.y, x[i + 2] = t.z, x[i + 3] = t.w;
-            }
-            float mul = 1.f;
-            if constexpr (kI8) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < 64; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-                row_peak[u * 128 + r] = __uint_as_float(top);
-                asm volatile("bar.sync 3, 256;" ::: "memory");
-                top = max(top, __float_as_uint(row_peak[(u ^ 1) * 128 + r]));
-                const int e = exponent_of(top);
-                mul = pow2(14 - e);
-                f = top < 0x7f800000u ? f * pow2(e - 14) : __int_as_float(0x7fffffff);  // (an infinity or NaN: the row is NaN)
-            }
-            if (u < kChunks) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t t[4][3];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) terms_of<kI8>(x[8 * i + 2 * e] * mul, x[8 * i + 2 * e + 1] * mul, t[e]);
-#pragma unroll
-                    for (uint32_t n = 0; n < kTerms; ++n)
-                        *reinterpret_cast<uint4 *>(qs + n * S::kQTermBytes + u * S::kQChunkBytes + r * 128 + ((i ^ (r & 7)) << 4)) =
-                            make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]);
+                    for (uint32_t off = kLanes / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+                    const int e = exponent_of(top);
+                    mul = pow2(14 - e);
+                    // (an infinity or NaN: the row is NaN)
+                    factor = top < 0x7f800000u ? factor * pow2(e - 14) : __int_as_float(0x7fffffff);
                 }
+                uint32_t t0[3], t1[3];
+                terms_of<kI8>(x.x * mul, x.y * mul, t0);
+                terms_of<kI8>(x.z * mul, x.w * mul, t1);
+                uint8_t *to = qs + ch / 64 * S::kQChunkBytes + at * 128 + (((ch % 64 / 8) ^ (at & 7)) << 4) + ch % 8 * 2;
+#pragma unroll
+                for (uint32_t n = 0; n < kTerms; ++n) *reinterpret_cast<uint2 *>(to + n * S::kQTermBytes) = make_uint2(t0[n], t1[n]);
+                if (lane % kLanes == 0) row_factor[at] = factor;
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
+            if constexpr (!S::kQInTmem) {
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if constexpr (S::kQInTmem) {  // a unit takes one term, a thread its row
+                static_assert(kTerms == 2, "a term for each unit");
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * kChunks; ++i) {  // sixteen channels: eight columns
+                    uint32_t w[8];
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+                        *reinterpret_cast<uint4 *>(w + 4 * h) = *reinterpret_cast<const uint4 *>(
+                            qs + u * S::kQTermBytes + i / 4 * S::kQChunkBytes + r * 128 + (((2 * (i % 4) + h) ^ (r & 7)) << 4));
+                    tmem_st8(tmem + S::q_col(u) + 8 * i + (((warp % 4) * 32) << 16), w);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
         }
-        const uint32_t unit = tmem + kUnitCols * u + (((warp % 4) * 32) << 16);
+        const float f = row_factor[r];
+        const uint32_t cols = tmem + S::score_col(u) + (((warp % 4) * 32) << 16);  // scores and weights
+        const uint32_t outs = tmem + S::out_col(u) + (((warp % 4) * 32) << 16);
         // keys of this CTA that this row sees, and its tile's first row
         const int base_key = (int)(block0 * kKeys);
         const int seen = a.causal ? (int)(a.first_row + query) + 1 - base_key : (int)keys;
@@ -390,18 +433,40 @@ attend_tile_kernel(CacheView c, TileArgs a) {
 #pragma unroll
         for (int i = 0; i < D; ++i) o[i] = 0.f;
         bool ok = true;
-        for (uint32_t g = u, it = 0; g < n_blocks; g += 2, ++it) {
+        float alpha = 1.f;  // of the block whose product has not joined the output yet
+        // The product of the unit's block before joins the output (in registers: the sum is rounded, not truncated).
+        auto take_output = [&](uint32_t done) {
+            ok = mbar_wait(o_full + u, done & 1, abort_flag, a.wait_limit);
+            ok = u ? vote<2, 128>(ok) : vote<1, 128>(ok);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int part = 0; part < D / 32; ++part) {
+                uint32_t w[32];
+                tmem_ld32(outs + 32 * part, w);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = __ffma2_rn(make_float2(o[32 * part + i], o[32 * part + i + 1]), make_float2(alpha, alpha),
+                                                make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])));
+                    o[32 * part + i] = x.x, o[32 * part + i + 1] = x.y;
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        };
+        uint32_t it = 0;
+        for (uint32_t g = u; g < n_blocks; g += 2, ++it) {
             const int key0 = (int)(g * kKeys);
             ok = mbar_wait(s_full + u, it & 1, abort_flag, a.wait_limit);
-            // (the scales in the block's stage)
-            if (kI8) ok = ok && mbar_wait(full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+            // (the scales come with the values)
+            if (kI8) ok = ok && mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
             ok = u ? vote<2, 128>(ok) : vote<1, 128>(ok);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool edge = key0 + (int)kKeys > min(seen0, (int)keys);  // some row of the tile does not see the whole block
             const int limit = min(seen, (int)keys) - key0;                // keys of the block that this row sees
             const float *ks = scales + (g % kStages) * S::kScaleFloats, *vs = ks + kKeys;
-            float alpha;
+            float alpha_new;
             float2 sum = make_float2(0.f, 0.f);
             // (kEdge in the type: a select per score would be paid in every block)
             auto weights = [&](auto edge_tag) {
@@ -410,7 +475,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     uint32_t s[32];
-                    tmem_ld32(unit + 32 * part, s);
+                    tmem_ld32(cols + 32 * part, s);
                     tmem_ld_wait();
                     float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -435,13 +500,15 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 }
                 const float m_new = fmaxf(m, top * f);
                 const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
-                alpha = ex2(m - base);
+                alpha_new = ex2(m - base);
                 m = m_new;
+                if (it) take_output(it - 1);
+                if (!ok) return;
                 const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
 #pragma unroll
                 for (int part = 0; part < 4; ++part) {
                     uint32_t s[16], t[kTerms][8];
-                    tmem_ld16(unit + 16 * part, s);
+                    tmem_ld16(cols + 16 * part, s);
                     tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -468,12 +535,14 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         for (uint32_t n = 0; n < kTerms; ++n) t[n][e] = w[n];
                     }
 #pragma unroll
-                    for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(unit + S::weight_col(n) + 8 * part, t[n]);
+                    for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(cols + S::weight_col(n, part), t[n]);
                 }
             };
             if (edge) weights(std::true_type{});
             else weights(std::false_type{});
-            l = fmaf(l, alpha, sum.x + sum.y);
+            if (!ok) break;
+            l = fmaf(l, alpha_new, sum.x + sum.y);
+            alpha = alpha_new;
             if constexpr (kI8) {
                 const int e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
                 alpha *= pow2(max(-126, e_here - e_new));
@@ -483,25 +552,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + u);
-            // the block's product joins the output (in registers: the sum is rounded, not truncated)
-            ok = mbar_wait(o_full + u, it & 1, abort_flag, a.wait_limit);
-            ok = u ? vote<2, 128>(ok) : vote<1, 128>(ok);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int part = 0; part < D / 32; ++part) {
-                uint32_t w[32];
-                tmem_ld32(unit + kOutCol + 32 * part, w);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = __ffma2_rn(make_float2(o[32 * part + i], o[32 * part + i + 1]), make_float2(alpha, alpha),
-                                                make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])));
-                    o[32 * part + i] = x.x, o[32 * part + i + 1] = x.y;
-                }
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
+        if (ok && it) take_output(it - 1);
         if (!ok) *abort_flag = 1;
         // ---- the units join: each finishes half of the channels and hands the others over, through the ring (every
         // product has been read out, every block consumed once both units are here)
@@ -526,26 +578,30 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const float inv = !direct ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             const float a1 = w1 * inv * undo, a2 = w2 * inv;
             const float *other = swap + (u ^ 1) * kHalf * kRows;
-            const size_t at_slot = ((size_t)query * a.n_heads + head) * a.n_slots + a.slot0 + split;
-            float *dst = (direct ? a.out + query * a.out_stride + (size_t)head * D : a.scratch + at_slot * D) + u * kHalf;
-            if (r < rows) {
-                if (!direct && u == 0)
-                    *reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * a.n_slots * D + 2 * at_slot) =
-                        make_float2(top, sum);
-                const bool wide = ((uintptr_t)dst & 15) == 0;
+            // (through shared memory, where q has been, so that rows are written whole: pieces of 16 bytes, swizzled)
+            if (u == 0) row_factor[r] = top, stat[512 + r] = sum;
+            uint8_t *line = qs + r * (D * 4);
 #pragma unroll
-                for (int i = 0; i < kHalf; i += 4) {
-                    float x[4];
+            for (int i = 0; i < kHalf; i += 4) {
+                float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[e] = fmaf(u ? o[kHalf + i + e] : o[i + e], a1, other[(i + e) * kRows + r] * a2);
-                    if (wide) {
-                        *reinterpret_cast<float4 *>(dst + i) = make_float4(x[0], x[1], x[2], x[3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) dst[i + e] = x[e];
-                    }
-                }
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(u ? o[kHalf + i + e] : o[i + e], a1, other[(i + e) * kRows + r] * a2);
+                *reinterpret_cast<float4 *>(line + (((u * kHalf + i) / 4 ^ (r & 7)) << 4)) = make_float4(x[0], x[1], x[2], x[3]);
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            constexpr uint32_t kLanes = D / 4, kSide = 32 / kLanes;
+            float2 *stats = reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * a.n_slots * D);
+#pragma unroll 4
+            for (uint32_t i = 0; i < 16; i += kSide) {
+                const uint32_t at = warp * 16 + i + lane / kLanes, which = row0 + at, ch = lane % kLanes;
+                if (at >= rows) break;
+                const float4 x = *reinterpret_cast<const float4 *>(qs + at * (D * 4) + ((ch ^ (at & 7)) << 4));
+                const uint32_t whose = which / group, of = kvh * group + which % group;
+                const size_t at_slot = ((size_t)whose * a.n_heads + of) * a.n_slots + a.slot0 + split;
+                float *dst = (direct ? a.out + whose * a.out_stride + (size_t)of * D : a.scratch + at_slot * D) + 4 * ch;
+                if (((uintptr_t)dst & 15) == 0) *reinterpret_cast<float4 *>(dst) = x;
+                else dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
+                if (!direct && ch == 0) stats[at_slot] = make_float2(row_factor[at], stat[512 + at]);
             }
         }
     }
