@@ -40,6 +40,7 @@ constexpr uint32_t kAhead = 2;  // a block's scores are formed when the product 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;
 constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr uint32_t kSms = 148;
 
 template <bool kI8, int D>
 struct TileShape {
@@ -276,6 +277,16 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             }
             if (!ok) *abort_flag = 1;
         } else if (warp == kScaleWarp) {
+            // ---- q of the tile that comes to an SM after this one (one CTA each is resident) on its way to L2
+            if (blockIdx.x + kSms < gridDim.x) {
+                const uint32_t next = blockIdx.x + kSms, kvh2 = next % c.n_kv, tile2 = gridDim.x / c.n_kv - 1 - next / c.n_kv;
+                const uint32_t end = min(kRows, n_rows - tile2 * kRows) * (D / 32);  // lines of 128 bytes
+                for (uint32_t i = lane; i < end; i += 32) {
+                    const uint32_t which = tile2 * kRows + i / (D / 32);
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + which / group * a.q_stride +
+                                                                  (size_t)(kvh2 * group + which % group) * D + i % (D / 32) * 32));
+                }
+            }
             // ---- INT8: the scales, those of the values relative to the running maximum's power of two
             if constexpr (kI8) {
                 float sc[4];  // key and value scales of keys lane, lane + 32 of the next block
@@ -343,24 +354,27 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 umma_commit(v_empty + g % kStages);
                 umma_commit(o_full + (g & 1));
             };
-            auto form = [&](uint32_t g) {  // (over columns whose weights an earlier product has read)
-                if (!mbar_wait(k_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit)) return false;
+            bool ok = mbar_wait(q_full, 0, abort_flag, a.wait_limit);
+            for (uint32_t g = 0; g < kAhead && g < n_blocks && ok; ++g) {
+                ok = mbar_wait(k_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) scores(g);
                 __syncwarp();
-                return true;
-            };
-            bool ok = mbar_wait(q_full, 0, abort_flag, a.wait_limit);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (uint32_t g = 0; g < kAhead && g < n_blocks && ok; ++g) ok = form(g);
+            }
             for (uint32_t g = 0; g < n_blocks && ok; ++g) {
+                const bool more = g + kAhead < n_blocks;
+                // (what the loaders bring is there, most often, before the weights are)
                 ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                if (ok && more) ok = mbar_wait(k_full + (g + kAhead) % kStages, ((g + kAhead) / kStages) & 1, abort_flag, a.wait_limit);
                 if (ok) ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) values(g);
+                if (elect_one()) {
+                    values(g);
+                    if (more) scores(g + kAhead);  // (over columns whose weights the product before reads first)
+                }
                 __syncwarp();
-                if (g + kAhead < n_blocks) ok = form(g + kAhead);
             }
             if (!ok) *abort_flag = 1;
         }
@@ -373,17 +387,28 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             constexpr uint32_t kLanes = D / 4, kSide = 32 / kLanes;
             const uint32_t ch = 4 * (lane % kLanes);
             const float unit_scale = kLog2E / sqrtf((float)D);
-#pragma unroll 4
-            for (uint32_t i = 0; i < 16; i += kSide) {
-                const uint32_t at = warp * 16 + i + lane / kLanes, which = row0 + min(at, rows - 1);
-                float4 x = *reinterpret_cast<const float4 *>(a.q + (which / group) * a.q_stride +
-                                                             (size_t)(kvh * group + which % group) * D + ch);
+            constexpr uint32_t kTurns = 16 / kSide;
+            float4 held[kTurns];
+            // (rows past the last repeat it)
+            const uint32_t which = row0 + min(warp * 16 + lane % 16, rows - 1);
+            const size_t where = which / group * a.q_stride + (size_t)(kvh * group + which % group) * D;  // of the row lane % 16
+#pragma unroll
+            for (uint32_t i = 0; i < kTurns; ++i)
+                held[i] = __ldg(reinterpret_cast<const float4 *>(a.q + __shfl_sync(0xffffffffu, where, i * kSide + lane / kLanes) + ch));
+#pragma unroll
+            for (uint32_t i = 0; i < kTurns; ++i) {
+                const uint32_t at = warp * 16 + i * kSide + lane / kLanes;
+                const float4 x = held[i];
                 float factor = unit_scale, mul = 1.f;  // factor: what turns a raw score into log2 units
                 if constexpr (kI8) {
                     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
                                        max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
+                    if constexpr (kLanes == 32) {
+                        top = __reduce_max_sync(0xffffffffu, top);
+                    } else {
 #pragma unroll
-                    for (uint32_t off = kLanes / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+                        for (uint32_t off = kLanes / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+                    }
                     const int e = exponent_of(top);
                     mul = pow2(14 - e);
                     // (an infinity or NaN: the row is NaN)
@@ -437,7 +462,6 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         // The product of the unit's block before joins the output (in registers: the sum is rounded, not truncated).
         auto take_output = [&](uint32_t done) {
             ok = mbar_wait(o_full + u, done & 1, abort_flag, a.wait_limit);
-            ok = u ? vote<2, 128>(ok) : vote<1, 128>(ok);
             if (!ok) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -457,11 +481,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         uint32_t it = 0;
         for (uint32_t g = u; g < n_blocks; g += 2, ++it) {
             const int key0 = (int)(g * kKeys);
-            ok = mbar_wait(s_full + u, it & 1, abort_flag, a.wait_limit);
-            // (the scales come with the values)
-            if (kI8) ok = ok && mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
-            ok = u ? vote<2, 128>(ok) : vote<1, 128>(ok);
-            if (!ok) break;
+            // (the scales come with the values, most often before the scores)
+            if (kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+            ok = ok && mbar_wait(s_full + u, it & 1, abort_flag, a.wait_limit);
+            if (!ok) break;  // (a warp at a time: the others' waits end with the flag below)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool edge = key0 + (int)kKeys > min(seen0, (int)keys);  // some row of the tile does not see the whole block
             const int limit = min(seen, (int)keys) - key0;                // keys of the block that this row sees
@@ -562,9 +585,11 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             constexpr int kHalf = D / 2;
             const float undo = kI8 ? pow2(e_here + 1) * (1.f / kWeightScale) : 1.f;
             float *swap = reinterpret_cast<float *>(ring), *stat = swap + 2 * kHalf * kRows;  // [unit][channel][128], [unit][m, l][128]
-            float *mine = swap + u * kHalf * kRows;
+            float4 *mine = reinterpret_cast<float4 *>(swap + u * kHalf * kRows);  // [four channels][row]
 #pragma unroll
-            for (int i = 0; i < kHalf; ++i) mine[i * kRows + r] = (u ? o[i] : o[kHalf + i]) * undo;
+            for (int i = 0; i < kHalf; i += 4)
+                mine[i / 4 * kRows + r] = make_float4((u ? o[i] : o[kHalf + i]) * undo, (u ? o[i + 1] : o[kHalf + i + 1]) * undo,
+                                                      (u ? o[i + 2] : o[kHalf + i + 2]) * undo, (u ? o[i + 3] : o[kHalf + i + 3]) * undo);
             stat[u * 256 + r] = m;
             stat[u * 256 + 128 + r] = l;
             asm volatile("bar.sync 3, 256;" ::: "memory");
@@ -577,31 +602,38 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const bool direct = a.n_slots == 1;
             const float inv = !direct ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             const float a1 = w1 * inv * undo, a2 = w2 * inv;
-            const float *other = swap + (u ^ 1) * kHalf * kRows;
+            const float4 *other = reinterpret_cast<const float4 *>(swap + (u ^ 1) * kHalf * kRows);
             // (through shared memory, where q has been, so that rows are written whole: pieces of 16 bytes, swizzled)
             if (u == 0) row_factor[r] = top, stat[512 + r] = sum;
             uint8_t *line = qs + r * (D * 4);
 #pragma unroll
             for (int i = 0; i < kHalf; i += 4) {
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf(u ? o[kHalf + i + e] : o[i + e], a1, other[(i + e) * kRows + r] * a2);
+                const float4 y = other[i / 4 * kRows + r];
+                const float x[4] = {fmaf(u ? o[kHalf + i] : o[i], a1, y.x * a2), fmaf(u ? o[kHalf + i + 1] : o[i + 1], a1, y.y * a2),
+                                    fmaf(u ? o[kHalf + i + 2] : o[i + 2], a1, y.z * a2),
+                                    fmaf(u ? o[kHalf + i + 3] : o[i + 3], a1, y.w * a2)};
                 *reinterpret_cast<float4 *>(line + (((u * kHalf + i) / 4 ^ (r & 7)) << 4)) = make_float4(x[0], x[1], x[2], x[3]);
             }
             asm volatile("bar.sync 3, 256;" ::: "memory");
             constexpr uint32_t kLanes = D / 4, kSide = 32 / kLanes;
             float2 *stats = reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * a.n_slots * D);
+            const uint32_t ch = lane % kLanes, which = row0 + min(warp * 16 + lane % 16, rows - 1);
+            // where the row lane % 16 goes, and (lanes below 16) its sums
+            const size_t head = (size_t)(which / group) * a.n_heads + kvh * group + which % group;
+            const size_t at_slot = head * a.n_slots + a.slot0 + split;
+            const size_t where = direct ? which / group * a.out_stride + (size_t)(kvh * group + which % group) * D : at_slot * D;
+            if (!direct && lane < 16 && warp * 16 + lane < rows)
+                stats[at_slot] = make_float2(row_factor[warp * 16 + lane], stat[512 + warp * 16 + lane]);
+            float *base_out = direct ? a.out : a.scratch;
+            const bool wide = ((uintptr_t)base_out & 15) == 0 && (!direct || a.out_stride % 4 == 0);
 #pragma unroll 4
             for (uint32_t i = 0; i < 16; i += kSide) {
-                const uint32_t at = warp * 16 + i + lane / kLanes, which = row0 + at, ch = lane % kLanes;
-                if (at >= rows) break;
+                const uint32_t at = warp * 16 + i + lane / kLanes;
+                float *dst = base_out + __shfl_sync(0xffffffffu, where, i + lane / kLanes) + 4 * ch;
+                if (at >= rows) continue;
                 const float4 x = *reinterpret_cast<const float4 *>(qs + at * (D * 4) + ((ch ^ (at & 7)) << 4));
-                const uint32_t whose = which / group, of = kvh * group + which % group;
-                const size_t at_slot = ((size_t)whose * a.n_heads + of) * a.n_slots + a.slot0 + split;
-                float *dst = (direct ? a.out + whose * a.out_stride + (size_t)of * D : a.scratch + at_slot * D) + 4 * ch;
-                if (((uintptr_t)dst & 15) == 0) *reinterpret_cast<float4 *>(dst) = x;
+                if (wide) *reinterpret_cast<float4 *>(dst) = x;
                 else dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
-                if (!direct && ch == 0) stats[at_slot] = make_float2(row_factor[at], stat[512 + at]);
             }
         }
     }
