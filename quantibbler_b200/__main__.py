@@ -1,6 +1,8 @@
-"""Command line: greedy generation from token ids with any model the registry knows.
+"""Command line: greedy generation from token ids with any model the registry knows, log probabilities of given
+continuations with the factorized decoder.
 
     python -m quantibbler_b200 generate --model DIR --prompt 5,17,3 --max-tokens 32
+    python -m quantibbler_b200 score --model DIR --prompt 5,17,3 --continuation 9,2 --continuation 4 --top 5
     python -m quantibbler_b200 trace --model DIR --out OUT < steps.jsonl
 
 Prints one JSON object (token ids in and out: text needs the model's tokenizer, which is not part
@@ -26,12 +28,30 @@ def main(argv=None) -> int:
     g.add_argument("--max-tokens", type=int, default=32)
     g.add_argument("--eos", type=int, default=None, help="token id that ends the generation")
     g.add_argument("--dtype", choices=("bfloat16", "float32"), default=None, help="default: the model's own")
+    g.add_argument("--kv-dtype", choices=("bfloat16", "float32", "int8"), default=None,
+                   help="storage of the key/value cache (factorized decoder; default: the model's own)")
+    sc = sub.add_parser("score", help="log probabilities of continuations of a prompt")
+    sc.add_argument("--model", required=True, help="a model directory or a blob")
+    sc.add_argument("--prompt", required=True, help="token ids, with commas between them")
+    sc.add_argument("--continuation", required=True, action="append", help="token ids; may be given several times")
+    sc.add_argument("--top", type=int, default=0, help="most probable alternatives to print at each place")
+    sc.add_argument("--dtype", choices=("bfloat16", "float32"), default=None, help="default: the model's own")
+    sc.add_argument("--kv-dtype", choices=("bfloat16", "float32", "int8"), default=None,
+                    help="storage of the key/value cache")
     sub.add_parser("trace", help="replay a trace of token ids (see bin/trace_run)")
     a = ap.parse_args(argv)
     from .gpu import GpuContext
     from .registry import load_decoder
     prompt = [int(t) for t in a.prompt.split(",")]
     settings = {} if a.dtype is None else {"serving": a.dtype}
+    if a.kv_dtype is not None:
+        settings["kv_dtype"] = a.kv_dtype
+    if a.command == "score":
+        conts = [[int(t) for t in c.split(",")] for c in a.continuation]
+        decoder = load_decoder(GpuContext.init(), a.model, max_batch=len(conts), max_prefix=len(prompt),
+                               max_seq=max(len(c) for c in conts), **settings)
+        print(json.dumps(decoder.score(prompt, conts, a.top)))
+        return 0
     decoder = load_decoder(GpuContext.init(), a.model, max_seq=len(prompt) + max(a.max_tokens, 1), **settings)
     print(json.dumps(decoder.generate(prompt, a.max_tokens, a.eos)))
     return 0

@@ -20,7 +20,9 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib, tp
-from ._lib import QK_BF16, QK_F32, KernelError, check
+from ._lib import QK_BF16, QK_F32, QK_I8, KernelError, check
+from .cache import DTYPES as KV_DTYPES
+from .cache import KvCache
 from .gpu import (PREFILL_NORM_MAX, DecodeStep, GpuContext, LayerPlan, PackedLayer, apply_prefill_many,
                   apply_prefill_many_gated, apply_prefill_many_normed, make_feed)
 
@@ -39,8 +41,13 @@ class DecoderConfig:
     rms_eps: float = 1e-5
     rope_theta: float = 10000.0
     serving: str = "float32"       # ServingDtype of the linears and norms
-    kv_dtype: str = "bfloat16"     # storage of the KV cache
+    # Storage of the KV cache: "bfloat16", "float32", or "int8" (codes with a float32 scale per token and kv head,
+    # head_dim + 4 bytes a row instead of 2 head_dim; cache.KvCache)
+    kv_dtype: str = "bfloat16"
     max_seq: int = 4096
+    # > 0: room for a prefix of so many tokens that all sequences share (set_prefix): it is stored once and read once
+    # a step for the whole batch; max_seq is then what every sequence may have behind it
+    max_prefix: int = 0
     max_batch: int = 1
     n_splits: int = 0              # key splits of the decode attention (0 = choose)
     # bfloat16 serving: batches this large take the tensor-core GEMM (measured per step on the
@@ -91,7 +98,7 @@ def rope_table(cfg: DecoderConfig) -> np.ndarray:
     results cast to float32 (engine/mod.rs:1169-1184)."""
     half = cfg.head_dim // 2
     inv_freq = cfg.rope_theta ** (-(2.0 * np.arange(half, dtype=np.float64)) / cfg.head_dim)
-    ang = np.arange(cfg.max_seq, dtype=np.float64)[:, None] * inv_freq[None, :]
+    ang = np.arange(cfg.max_seq + cfg.max_prefix, dtype=np.float64)[:, None] * inv_freq[None, :]
     return np.stack([np.cos(ang), np.sin(ang)], axis=-1).astype(np.float32)
 
 
@@ -179,7 +186,13 @@ class SlotDecoder:
 
     tp_size, group = 1, None
     logit_softcap = None  # logits <- cap tanh(logits / cap)
+    prefix_len = 0        # tokens of a prefix that all sequences share (Decoder.set_prefix)
     keeps_state = False   # True: a step changes more than the cache row of its own position
+
+    @property
+    def positions_end(self) -> int:
+        """Positions from here on do not fit the caches."""
+        return self.cfg.max_seq
 
     def _setup_driver(self) -> None:
         self.graph = None
@@ -200,8 +213,8 @@ class SlotDecoder:
         if self.tp_size > 1:
             self._gather_argmax(best_val, best_idx)
 
-    def prefill(self, tokens, seq: int = 0, first_position: int = 0, want=None):
-        """All of ``tokens`` (consecutive positions ``first_position ...`` of sequence slot ``seq``)
+    def prefill(self, tokens, seq: int = 0, first_position: int | None = None, want=None):
+        """All of ``tokens`` (consecutive positions ``first_position ...`` of sequence slot ``seq``; default: its first)
         through the trunk in one pass per ``prefill_chunk`` positions: the batched form of the
         reference's prompt loop (engine/mod.rs:1393-1413, one ``transformer`` call per prompt
         token).  Appends what every position leaves in the cache or state and puts the greedy token
@@ -215,13 +228,14 @@ class SlotDecoder:
             raise ValueError("prefill needs at least one token")
         if not 0 <= seq < cfg.max_batch:
             raise ValueError(f"sequence slot {seq} outside the batch of {cfg.max_batch}")
-        check_cache_capacity([first_position], len(toks), cfg.max_seq)
+        first_position = self.prefix_len if first_position is None else first_position
+        if first_position < self.prefix_len:
+            raise ValueError(f"position {first_position} lies in the shared prefix of {self.prefix_len}")
+        check_cache_capacity([first_position], len(toks), self.positions_end)
         want = None if want is None else [int(w) for w in want]
         if want and not 0 <= min(want) <= max(want) < len(toks):
             raise ValueError(f"wanted places {min(want)}..{max(want)} outside the {len(toks)} tokens")
-        handle = self.ctx.stream
-        # (handles 0 and 1 are the legacy default stream, which torch wraps itself)
-        stream = torch.cuda.ExternalStream(handle) if handle > 2 else torch.cuda.default_stream()
+        stream = self._stream()
         stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(stream):
             logits = None if want is None else torch.empty(len(want), self.v_loc, dtype=torch.float32,
@@ -249,6 +263,12 @@ class SlotDecoder:
         self._host_positions[seq] = last
         self.ctx.synchronize()
         return logits
+
+    def _stream(self):
+        """The context's stream as torch knows it."""
+        handle = self.ctx.stream
+        # (handles 0 and 1 are the legacy default stream, which torch wraps itself)
+        return self.torch.cuda.ExternalStream(handle) if handle > 2 else self.torch.cuda.default_stream()
 
     def _reset_slot(self, seq: int, token: int, position: int) -> None:
         self.token_ids[seq:seq + 1].fill_(token)
@@ -303,14 +323,14 @@ class SlotDecoder:
 
     def start(self, token_ids, positions) -> None:
         torch = self.torch
-        check_cache_capacity(positions, 1, self.cfg.max_seq)
+        check_cache_capacity(positions, 1, self.positions_end)
         self._host_positions = [int(p) for p in positions]
         self.token_ids.copy_(torch.as_tensor(token_ids, dtype=torch.int32))
         self.positions.copy_(torch.as_tensor(positions, dtype=torch.int32))
 
     def decode(self, n_steps: int) -> np.ndarray:
         """Greedy decode; returns the [n_steps, batch] generated ids."""
-        check_cache_capacity([p for p in self._host_positions if p is not None], n_steps, self.cfg.max_seq)
+        check_cache_capacity([p for p in self._host_positions if p is not None], n_steps, self.positions_end)
         self._host_positions = [None if p is None else p + n_steps for p in self._host_positions]
         out = []
         for _ in range(n_steps):
@@ -333,7 +353,7 @@ class SlotDecoder:
         the completion ends at ``max_tokens`` tokens (finish ``"length"``; as in the
         reference the first token is kept even when ``max_tokens`` is 0).  ``prompt_ms`` is the
         prefill span rounded up to a whole millisecond, at least 1.  Stop strings are text-side
-        (they need the tokenizer) and stay with the caller.
+        (they need the tokenizer) and stay with the caller.  With a shared prefix set, the prompt follows it.
         """
         import math
         import time
@@ -350,10 +370,10 @@ class SlotDecoder:
                 raise ValueError(f"token id {tok} out of range (vocab_size {self.cfg.vocab})")
         started = time.perf_counter()
         if len(prompt) >= self.cfg.prefill_min_tokens:
-            self.prefill(prompt, seq=0, first_position=0)   # the whole prompt in one pass
+            self.prefill(prompt, seq=0)   # the whole prompt in one pass
         else:
             for pos, tok in enumerate(prompt):
-                self.start([tok], [pos])
+                self.start([tok], [self.prefix_len + pos])
                 self.step()
         self.ctx.synchronize()
         prompt_ms = max(1, math.ceil((time.perf_counter() - started) * 1000.0))
@@ -397,7 +417,9 @@ class Decoder(SlotDecoder):
         self.h_loc, self.kv_loc = cfg.n_heads // tp_size, cfg.n_kv_heads // tp_size
         self.ff_loc, self.v_loc = cfg.d_ff // tp_size, cfg.vocab // tp_size
         self.serving_tag = QK_F32 if cfg.serving == "float32" else QK_BF16
-        self.kv_tag = QK_F32 if cfg.kv_dtype == "float32" else QK_BF16
+        if cfg.kv_dtype not in KV_DTYPES:
+            raise KernelError(f"kv_dtype must be one of {', '.join(KV_DTYPES)}, got {cfg.kv_dtype!r}")
+        self.kv_tag = {"float32": QK_F32, "bfloat16": QK_BF16, "int8": QK_I8}[cfg.kv_dtype]
         f32 = dict(dtype=torch.float32, device=dev)
         i32 = dict(dtype=torch.int32, device=dev)
 
@@ -448,11 +470,20 @@ class Decoder(SlotDecoder):
         self.positions = torch.zeros(B, **i32)
         self.kv_len = torch.ones(B, **i32)
         self.seq_index = torch.arange(B, **i32)
-        kv_t = torch.float32 if cfg.kv_dtype == "float32" else torch.bfloat16
-        self.cache_k = [torch.zeros(B, self.kv_loc, cfg.max_seq, hd, dtype=kv_t, device=dev)
-                        for _ in range(cfg.n_layers)]
-        self.cache_v = [torch.zeros(B, self.kv_loc, cfg.max_seq, hd, dtype=kv_t, device=dev)
-                        for _ in range(cfg.n_layers)]
+        # INT8 caches, and caches behind a shared prefix, go through KvCache
+        self.kv, self.prefix, self.prefix_len = None, None, 0
+        if cfg.kv_dtype == "int8" or cfg.max_prefix > 0:
+            make = lambda n, rows: [KvCache.empty(ctx, n, self.kv_loc, rows, hd, cfg.kv_dtype)  # noqa: E731
+                                    for _ in range(cfg.n_layers)]
+            self.kv = make(B, cfg.max_seq)
+            self.prefix = make(1, cfg.max_prefix) if cfg.max_prefix > 0 else None
+            self.cache_k, self.cache_v = [c.k for c in self.kv], [c.v for c in self.kv]
+        else:
+            kv_t = torch.float32 if cfg.kv_dtype == "float32" else torch.bfloat16
+            self.cache_k = [torch.zeros(B, self.kv_loc, cfg.max_seq, hd, dtype=kv_t, device=dev)
+                            for _ in range(cfg.n_layers)]
+            self.cache_v = [torch.zeros(B, self.kv_loc, cfg.max_seq, hd, dtype=kv_t, device=dev)
+                            for _ in range(cfg.n_layers)]
         # Key splits: about 256 blocks of 128 threads per launch (two per SM is what stays
         # resident) in chunks of at least ~64 keys.  Measured per step on the Llama-3-8B
         # shape at 2048 keys, by batch (best split count: ms against the former "eight blocks
@@ -473,13 +504,14 @@ class Decoder(SlotDecoder):
         self.n_splits = cfg.n_splits or max(1, min(most, want, max(1, cfg.max_seq // 64)))
         # (the one-launch form is the tensor-core attention; a context switched to the scalar
         # kernel keeps the separate launches)
-        self.fused_attention = (cfg.fused_attention and B <= cfg.fused_attention_max_batch
+        self.fused_attention = (cfg.fused_attention and self.kv is None and B <= cfg.fused_attention_max_batch
                                 and cfg.kv_dtype == "bfloat16" and hd == 128
                                 and ctx.set_decode_attention_kernel(-1) != 0)
         scratch = max(_lib.lib().qk_decode_attention_scratch(B, self.h_loc, hd, self.n_splits),
                       _lib.lib().qk_decode_attention_rope_scratch(B, self.h_loc, self.kv_loc, hd, self.n_splits))
         self.att_scratch = torch.zeros(scratch // 4 + 4, **f32)
         self.cos_sin = dev_f32(rope_table(cfg))
+        self.angles = self.cos_sin.view(-1, hd // 2, 2)
         self.emb_tag = QK_BF16 if cfg.serving == "bfloat16" else QK_F32
         if share_from is not None:
             o = share_from
@@ -519,7 +551,7 @@ class Decoder(SlotDecoder):
                 return [(L[n], rows(src, b), rows(dst, b)) for b in range(B)
                         for n, dst in zip(names, dsts)]
 
-            fed = cfg.serving in ("float32", "bfloat16") and B <= cfg.feed_max_batch
+            fed = cfg.serving in ("float32", "bfloat16") and B <= cfg.feed_max_batch and self.kv is None
             gemm = cfg.serving == "bfloat16" and B >= cfg.gemm_min_batch
             self.gated_down = fed or (cfg.serving in ("float32", "bfloat16") and not gemm
                                       and B <= cfg.gated_down_max_batch)
@@ -593,7 +625,7 @@ class Decoder(SlotDecoder):
             self.plans.append(plan)
         self.step_kernel = None
         if (B <= cfg.fused_step_max_batch and tp_size == 1 and not self.has_qk_norm and hd == 128
-                and cfg.kv_dtype == "bfloat16"):
+                and cfg.kv_dtype == "bfloat16" and self.kv is None):
             blocks = [dict(L, input_norm=self.norms[li][0].data_ptr(), post_norm=self.norms[li][1].data_ptr(),
                            cache_k=self.cache_k[li].data_ptr(), cache_v=self.cache_v[li].data_ptr())
                       for li, L in enumerate(self.layers)]
@@ -615,7 +647,7 @@ class Decoder(SlotDecoder):
         # input, build its digit table).  Fed plans move that to the kernel that produces the
         # vector, once per vector: the norm feeds q,k,v and gate,up, the attention combine feeds
         # o, the SwiGLU feeds down.
-        self.fed = (not self.use_gemm) and B <= cfg.feed_max_batch
+        self.fed = (not self.use_gemm) and B <= cfg.feed_max_batch and self.kv is None
         self.feeds = []
         if self.fed:
             for plan in self.plans:
@@ -760,7 +792,9 @@ class Decoder(SlotDecoder):
                                              (self.k, self.kn, self.qk_norms[li][1], self.kv_loc)):
                     check(lib.qk_rmsnorm(c, _p(src), None, _p(wgt), B * heads, hd, cfg.rms_eps,
                                          self.serving_tag, _p(src), _p(dst)))
-            if self.fused_attention and not feeds:
+            if self.kv is not None:
+                self._cached_attention(li)
+            elif self.fused_attention and not feeds:
                 # RoPE, cache append, attention and combine in one launch
                 check(lib.qk_decode_attention_rope(
                     c, _p(self.qn), _p(self.kn), _p(self.v), _p(self.cos_sin), _p(self.positions),
@@ -800,6 +834,114 @@ class Decoder(SlotDecoder):
         self._norm(pending, self.final_norm, None, xa, xb)
         self._head(self.h, B, self.logits)
         self._greedy(self.logits, B, self.best_val, self.best_idx)
+
+    def _cached_attention(self, li: int) -> None:
+        """Rotation, append and attention of a step over ``KvCache`` rows and the shared prefix."""
+        B, hd, cache = self.cfg.max_batch, self.cfg.head_dim, self.kv[li]
+        q = self.qn.view(B, self.h_loc, hd)
+        cache.append(self.kn.view(B, self.kv_loc, hd), self.v.view(B, self.kv_loc, hd), self.angles, self.positions,
+                     self.seq_index, q=q, q_out=q)
+        cache.attend(q, self.kv_len, prefix=self.prefix[li] if self.prefix_len else None, prefix_len=self.prefix_len,
+                     out=self.attn.view(B, self.h_loc, hd))
+
+    # ------------------------------------------------------------------ a shared prefix
+    @property
+    def positions_end(self) -> int:
+        return self.cfg.max_seq + self.prefix_len
+
+    def set_prefix(self, tokens) -> None:
+        """All sequences now continue ``tokens``: they go through the trunk once, into a cache of their own that
+        every step and portion reads once for the whole batch.  Positions count from the prefix's first token, a
+        sequence's own rows begin behind it, and what its cache held is void.  Leaves every slot at the prefix's
+        last token, its logits in ``logits`` and the greedy continuation in ``best_idx``: ``advance()`` and
+        ``step()`` go on from there.  A captured step is dropped (it knows the prefix's length)."""
+        torch, cfg = self.torch, self.cfg
+        toks = [int(t) for t in tokens]
+        if not 1 <= len(toks) <= cfg.max_prefix:
+            raise ValueError(f"a prefix of {len(toks)} tokens does not fit the {cfg.max_prefix} of max_prefix")
+        for tok in toks:
+            if not 0 <= tok < cfg.vocab:
+                raise ValueError(f"token id {tok} out of range (vocab_size {cfg.vocab})")
+        self.graph, self.prefix_len = None, 0
+        for cache in self.kv:
+            cache.first_position = 0
+        stream = self._stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            reserve = min(len(toks), cfg.prefill_chunk)
+            for c0 in range(0, len(toks), cfg.prefill_chunk):
+                part = toks[c0:c0 + cfg.prefill_chunk]
+                self._prefill_portion(part, 0, c0, reserve, into_prefix=True)
+            self._portion_hidden([len(part) - 1], self.h[:1])
+            self._head(self.h[:1], 1, self.logits[:1])
+            self._greedy(self.logits[:1], 1, self.best_val[:1], self.best_idx[:1])
+            for t in (self.logits, self.best_val, self.best_idx):
+                t.copy_(t[:1].clone().expand_as(t))
+            self.prefix_len = len(toks)
+            for cache in self.kv:
+                cache.first_position = self.prefix_len
+            self.token_ids.fill_(toks[-1])
+            self.positions.fill_(self.prefix_len - 1)
+            self.kv_len.zero_()
+        stream.synchronize()
+        torch.cuda.current_stream().wait_stream(stream)
+        self._host_positions = [self.prefix_len - 1] * cfg.max_batch
+        self.ctx.synchronize()
+
+    def score(self, prompt, continuations, top: int = 0) -> list[dict]:
+        """How probable each of ``continuations`` (lists of token ids, at most ``max_batch``) is behind ``prompt``: per
+        continuation ``logprobs`` of its tokens (natural logarithm, each given all before it), their ``total``, the
+        ``entropy`` of each token's distribution, and with ``top`` > 0 the most probable ids and their log
+        probabilities at each place.  The prompt goes through the trunk once, the continuations in step behind it."""
+        from .scoring import log_probs
+        torch, cfg = self.torch, self.cfg
+        conts = [[int(t) for t in c] for c in continuations]
+        if self.tp_size > 1:
+            raise ValueError("score needs the whole vocabulary on one rank")
+        if not 1 <= len(conts) <= cfg.max_batch or not all(conts):
+            raise ValueError(f"score takes 1 to {cfg.max_batch} continuations (max_batch) of one token or more")
+        longest = max(len(c) for c in conts)
+        if longest > cfg.max_seq + 1:
+            raise ValueError(f"a continuation of {longest} tokens does not fit {cfg.max_seq} cache rows")
+        for tok in (t for c in conts for t in c):
+            if not 0 <= tok < cfg.vocab:
+                raise ValueError(f"token id {tok} out of range (vocab_size {cfg.vocab})")
+        self.set_prefix(prompt)
+        n, B, dev = len(conts), cfg.max_batch, self.logits.device
+        stream = self._stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            # token j of every continuation; a finished one repeats its last row, an unused slot writes its first
+            ids = torch.tensor([[c[min(j, len(c) - 1)] for c in conts] + [0] * (B - n) for j in range(longest)],
+                               dtype=torch.int32, device=dev)
+            rows = torch.tensor([[min(j, len(c) - 1) for c in conts] + [0] * (B - n) for j in range(longest)],
+                                dtype=torch.int32, device=dev)
+            targets = torch.tensor([[c[j] if j < len(c) else -1 for c in conts] for j in range(longest)],
+                                   dtype=torch.int32, device=dev)
+            found = []
+            for j in range(longest):
+                if j:
+                    self.token_ids.copy_(ids[j - 1])
+                    self.positions.copy_(rows[j - 1] + self.prefix_len)
+                    self.kv_len.copy_(rows[j - 1] + 1)
+                    self.step()
+                found.append(log_probs(self.ctx, self.logits[:n], targets[j], top))
+        stream.synchronize()
+        torch.cuda.current_stream().wait_stream(stream)
+        last = [min(longest - 1, len(c)) for c in conts]
+        self._host_positions = [self.prefix_len + max(p - 1, 0) for p in last] + [self.prefix_len] * (B - n)
+        self.ctx.synchronize()
+        out = []
+        logprob, entropy = (torch.stack([getattr(f, k) for f in found]).cpu().numpy() for k in ("logprob", "entropy"))
+        top_ids, top_lp = (torch.stack([getattr(f, k) for f in found]).cpu().numpy() for k in ("top_ids", "top_logprob"))
+        for i, c in enumerate(conts):
+            k = len(c)
+            item = {"logprobs": logprob[:k, i].tolist(), "total": float(logprob[:k, i].astype(np.float64).sum()),
+                    "entropy": entropy[:k, i].tolist()}
+            if top:
+                item["top_ids"], item["top_logprobs"] = top_ids[:k, i].tolist(), top_lp[:k, i].tolist()
+            out.append(item)
+        return out
 
     # ------------------------------------------------------------------ batched prefill
     def _prefill_buffers(self, n_tokens: int) -> dict:
@@ -852,7 +994,8 @@ class Decoder(SlotDecoder):
                                     n_tokens, d, cfg.rms_eps, self.serving_tag, _p(x), _p(pf["h"])))
         self._prefill_linears(li, names, pf["h"], dsts, n_tokens)
 
-    def _prefill_portion(self, part, seq: int, p0: int, reserve: int) -> None:
+    def _prefill_portion(self, part, seq: int, p0: int, reserve: int, into_prefix: bool = False) -> None:
+        """``into_prefix``: the portion belongs to the shared prefix, not to slot ``seq``."""
         torch, lib, c, cfg = self.torch, _lib.lib(), self.ctx.handle, self.cfg
         B, d, hd = cfg.max_batch, cfg.d_model, cfg.head_dim
         T = len(part)
@@ -871,14 +1014,23 @@ class Decoder(SlotDecoder):
                                              (pf["k"], pf["kn"], self.qk_norms[li][1], self.kv_loc)):
                     check(lib.qk_rmsnorm(c, _p(src), None, _p(wgt), T * heads, hd, cfg.rms_eps,
                                          self.serving_tag, _p(src), _p(dst)))
-            check(lib.qk_rope_cache(c, _p(pf["qn"]), _p(pf["kn"]), _p(pf["v"]), _p(self.cos_sin),
-                                    _p(pf["pos"]), _p(pf["seq"]), _p(self.cache_k[li]),
-                                    _p(self.cache_v[li]), self.kv_tag, T, self.h_loc,
-                                    self.kv_loc, hd, cfg.max_seq, B))
-            check(lib.qk_prefill_attention(c, _p(pf["qn"]), _p(self.cache_k[li]),
-                                           _p(self.cache_v[li]), self.kv_tag, seq, p0, T,
-                                           self.h_loc, self.kv_loc, hd, cfg.max_seq,
-                                           _p(pf["attn"])))
+            if self.kv is not None:
+                cache = self.prefix[li] if into_prefix else self.kv[li]
+                shared = 0 if into_prefix else self.prefix_len
+                q = pf["qn"][:T].view(T, self.h_loc, hd)
+                cache.append(pf["kn"][:T].view(T, self.kv_loc, hd), pf["v"][:T].view(T, self.kv_loc, hd), self.angles,
+                             pf["pos"][:T], pf["seq"][:T], q=q, q_out=q)
+                cache.portion(q, seq, p0, prefix=self.prefix[li] if shared else None, prefix_len=shared,
+                              out=pf["attn"][:T].view(T, self.h_loc, hd))
+            else:
+                check(lib.qk_rope_cache(c, _p(pf["qn"]), _p(pf["kn"]), _p(pf["v"]), _p(self.cos_sin),
+                                        _p(pf["pos"]), _p(pf["seq"]), _p(self.cache_k[li]),
+                                        _p(self.cache_v[li]), self.kv_tag, T, self.h_loc,
+                                        self.kv_loc, hd, cfg.max_seq, B))
+                check(lib.qk_prefill_attention(c, _p(pf["qn"]), _p(self.cache_k[li]),
+                                               _p(self.cache_v[li]), self.kv_tag, seq, p0, T,
+                                               self.h_loc, self.kv_loc, hd, cfg.max_seq,
+                                               _p(pf["attn"])))
             self._prefill_linears(li, ["o"], pf["attn"], [pf["delta"]], T)
             if self.tp_size > 1:
                 torch.distributed.all_reduce(pf["delta"][:T], group=self.group)
@@ -905,7 +1057,7 @@ class Decoder(SlotDecoder):
 
     def _reset_slot(self, seq: int, token: int, position: int) -> None:
         super()._reset_slot(seq, token, position)
-        self.kv_len[seq:seq + 1].fill_(position + 1)
+        self.kv_len[seq:seq + 1].fill_(position + 1 - self.prefix_len)
 
     def advance(self) -> None:
         super().advance()
@@ -914,6 +1066,19 @@ class Decoder(SlotDecoder):
     def _step_inputs(self) -> list:
         return [self.token_ids, self.positions, self.kv_len]
 
+    def capture(self) -> None:
+        # (its warm-up steps run where the sequences stand, which after set_prefix is in front of their own rows)
+        saved = [t.clone() for t in (self.positions, self.kv_len)]
+        if self.prefix_len:
+            self.positions.clamp_(min=self.prefix_len)
+            self.kv_len.clamp_(min=1)
+        super().capture()
+        self.positions.copy_(saved[0])
+        self.kv_len.copy_(saved[1])
+        self.torch.cuda.synchronize()
+
     def start(self, token_ids, positions) -> None:
+        if self.prefix_len and len(positions) and min(int(p) for p in positions) < self.prefix_len:
+            raise ValueError(f"position {min(int(p) for p in positions)} lies in the shared prefix of {self.prefix_len}")
         super().start(token_ids, positions)
-        self.kv_len.copy_(self.positions + 1)
+        self.kv_len.copy_(self.positions + 1 - self.prefix_len)

@@ -553,3 +553,171 @@ def test_python_refusals(gpu_ctx):
     assert c.portion(q[:0], 0, 8).shape == (0, 4, 64)
     assert c.append(q[:0, :2], q[:0, :2], cs, lens[:0], lens[:0]) is None
     gpu_ctx.synchronize()
+
+
+# ---------------------------------------------------------------------- the decoder over such caches
+RANKS = {n: 24 for n in ("q", "k", "v", "o", "gate", "up", "down")}
+
+
+def small(**kw):
+    from quantibbler_b200.decoder import DecoderConfig, random_model
+    base = dict(n_layers=2, d_model=128, n_heads=4, n_kv_heads=2, head_dim=64, d_ff=128, vocab=160, max_seq=64, max_batch=3,
+                serving="float32")
+    base.update(kw)
+    cfg = DecoderConfig(**base)
+    return cfg, random_model(cfg, RANKS, seed=5)
+
+
+def int8_rows(values):
+    """What an int8 cache holds of k or v [kv heads x head_dim] (float32), heads of 64."""
+    from oracle.attention_np import quantize_per_token
+    x = np.asarray(values, np.float64).reshape(-1, 64)
+    peak = np.abs(x).max(-1, keepdims=True)
+    scale = np.where(peak > 0, peak / 127.0, 1.0).astype(np.float32).astype(np.float64)
+    assert quantize_per_token(x)[0].shape == x.shape
+    return (np.clip(np.rint(x / scale), -127, 127) * scale).astype(np.float32).reshape(-1)
+
+
+def reference_logits(cfg, weights, tokens):
+    from oracle import decoder_np
+    rounding = {"float32": None, "bfloat16": decoder_np._bf16, "int8": int8_rows}[cfg.kv_dtype]
+    s = decoder_np.Session(cfg, weights, kv_round=rounding)
+    return np.array([s.step(t)[1] for t in tokens])
+
+
+# The tolerances are those of the decoder's other tests: float32 arithmetic in another order moves logits by less than
+# 2e-4 of their largest; a code of an int8 row that such a difference tips over moves a value by 1/127 of its row's largest,
+# one entry of 64 in one row, less than 5e-3 of the logits.
+TOL = {"float32": 2e-4, "bfloat16": 5e-3, "int8": 5e-3}
+
+
+@pytest.mark.parametrize("kv_dtype", ["float32", "bfloat16", "int8"])
+@pytest.mark.parametrize("graph", [False, True])
+def test_decoder_behind_a_shared_prefix(gpu_ctx, kv_dtype, graph):
+    """Three sequences continue one prefix in different ways: step by step, captured, against the forward of each
+    whole sequence."""
+    from quantibbler_b200.decoder import Decoder
+    cfg, weights = small(kv_dtype=kv_dtype, max_prefix=40)
+    dec = Decoder(gpu_ctx, cfg, weights)
+    rng = np.random.default_rng(1)
+    prefix = rng.integers(0, cfg.vocab, 37).tolist()
+    conts = rng.integers(0, cfg.vocab, (3, 4)).tolist()
+    dec.set_prefix(prefix)
+    first = dec.logits.cpu().numpy()
+    want = [reference_logits(cfg, weights, prefix + c) for c in conts]
+    scale, tol = np.abs(np.array(want)).max(), TOL[kv_dtype]
+    for b in range(3):
+        assert np.abs(first[b] - want[b][len(prefix) - 1]).max() <= tol * scale
+    if graph:
+        dec.capture()
+    for j in range(4):
+        dec.start([c[j] for c in conts], [len(prefix) + j] * 3)
+        if graph:
+            dec.graph.replay()
+        else:
+            dec.step()
+        torch.cuda.synchronize()
+        gpu_ctx.synchronize()
+        got = dec.logits.cpu().numpy()
+        for b in range(3):
+            assert np.abs(got[b] - want[b][len(prefix) + j]).max() <= tol * scale
+    for call, text in [(lambda: dec.start([1, 1, 1], [36, 40, 40]), "lies in the shared prefix"),
+                       (lambda: dec.prefill([1, 2], first_position=5), "lies in the shared prefix"),
+                       (lambda: dec.start([1] * 3, [37 + 64] * 3), "does not fit the KV cache"),
+                       (lambda: dec.set_prefix([]), "does not fit"), (lambda: dec.set_prefix([1] * 41), "does not fit"),
+                       (lambda: dec.set_prefix([cfg.vocab]), "out of range")]:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+@pytest.mark.parametrize("kv_dtype", ["bfloat16", "int8"])
+def test_prompts_behind_a_prefix_and_a_second_prefix(gpu_ctx, kv_dtype):
+    """Prompts of unequal length in portions behind a prefix; then another prefix with the same decoder."""
+    from quantibbler_b200.decoder import Decoder
+    cfg, weights = small(kv_dtype=kv_dtype, max_prefix=80, prefill_chunk=16)
+    dec = Decoder(gpu_ctx, cfg, weights)
+    rng = np.random.default_rng(2)
+    for length in (70, 21):
+        prefix = rng.integers(0, cfg.vocab, length).tolist()
+        dec.set_prefix(prefix)
+        prompts = [rng.integers(0, cfg.vocab, n).tolist() for n in (5, 33, 1)]
+        for b, p in enumerate(prompts):
+            got = dec.prefill(p, seq=b, want=[len(p) - 1]).cpu().numpy()[0]
+            want = reference_logits(cfg, weights, prefix + p)
+            assert np.abs(got - want[-1]).max() <= TOL[kv_dtype] * np.abs(want).max()
+        dec.start([1, 2, 3], [length + len(p) for p in prompts])
+        dec.step()
+        gpu_ctx.synchronize()
+        got = dec.logits.cpu().numpy()
+        for b, p in enumerate(prompts):
+            want = reference_logits(cfg, weights, prefix + p + [b + 1])
+            assert np.abs(got[b] - want[-1]).max() <= TOL[kv_dtype] * np.abs(want).max()
+
+
+def test_generate_over_an_int8_cache(gpu_ctx):
+    """Prompts on both sides of the batched prefill; alone and behind a prefix the same completion."""
+    from oracle import decoder_np
+    from quantibbler_b200.decoder import Decoder
+    for n in (5, 30):
+        prompt = np.random.default_rng(n).integers(0, 160, n).tolist()
+        cfg, weights = small(kv_dtype="int8", max_batch=1)
+        plain = Decoder(gpu_ctx, cfg, weights).generate(prompt, 6)
+        s = decoder_np.Session(cfg, weights, kv_round=int8_rows)
+        for t in prompt:
+            nxt, _ = s.step(t)
+        want = []
+        for _ in range(6):
+            want.append(nxt)
+            nxt, _ = s.step(nxt)
+        assert plain["completion_tokens"] == want
+        cfg, _ = small(kv_dtype="int8", max_batch=1, max_prefix=4)
+        behind = Decoder(gpu_ctx, cfg, weights)
+        behind.set_prefix(prompt[:4])
+        assert behind.generate(prompt[4:], 6)["completion_tokens"] == want
+
+
+@pytest.mark.parametrize("kv_dtype", ["float32", "int8"])
+def test_score(gpu_ctx, kv_dtype):
+    from quantibbler_b200.decoder import Decoder
+    cfg, weights = small(kv_dtype=kv_dtype, max_prefix=20, max_batch=4, max_seq=8)
+    dec = Decoder(gpu_ctx, cfg, weights)
+    rng = np.random.default_rng(3)
+    prompt = rng.integers(0, cfg.vocab, 17).tolist()
+    conts = [rng.integers(0, cfg.vocab, n).tolist() for n in (3, 9, 1)]
+    for _ in range(2):    # (a decoder scores again)
+        got = dec.score(prompt, conts, top=4)
+        for c, item in zip(conts, got):
+            x = reference_logits(cfg, weights, prompt + c[:-1])[len(prompt) - 1:].astype(np.float64)
+            tol = 2 * TOL[kv_dtype] * np.abs(x).max() + 1e-6
+            p = x - np.log(np.exp(x - x.max(-1, keepdims=True)).sum(-1, keepdims=True)) - x.max(-1, keepdims=True)
+            want = p[np.arange(len(c)), c]
+            assert np.abs(np.array(item["logprobs"]) - want).max() <= tol
+            assert abs(item["total"] - want.sum()) <= tol * len(c)
+            assert np.abs(np.array(item["entropy"]) + (np.exp(p) * p).sum(-1)).max() <= 8 * tol
+            best = -np.sort(-p, axis=-1)[:, :4]
+            assert np.abs(np.array(item["top_logprobs"]) - best).max() <= tol
+            assert np.abs(np.take_along_axis(p, np.array(item["top_ids"]), 1) - best).max() <= tol
+    for call, text in [(lambda: dec.score(prompt, []), "1 to 4 continuations"), (lambda: dec.score(prompt, [[]]), "1 to 4"),
+                       (lambda: dec.score(prompt, [[1]] * 5), "1 to 4"), (lambda: dec.score(prompt, [[1] * 10]), "does not fit"),
+                       (lambda: dec.score(prompt, [[cfg.vocab]]), "out of range")]:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_score_on_the_command_line(gpu_ctx, capsys):
+    import json
+    import os
+    from conftest import GOLDEN
+    from quantibbler_b200.__main__ import main
+    path = os.path.join(GOLDEN, "parity-tiny")
+    with open(os.path.join(path, "goldens.json")) as f:
+        g = json.load(f)
+    ids, k = g["input_ids"], 4
+    assert main(["score", "--model", path, "--prompt", ",".join(map(str, ids[:k])), "--continuation",
+                 ",".join(map(str, ids[k:])), "--continuation", "1", "--top", "2", "--kv-dtype", "float32"]) == 0
+    got = json.loads(capsys.readouterr().out)
+    x = np.array(g["logits"], np.float64)[k - 1:-1]
+    p = x - np.log(np.exp(x).sum(-1, keepdims=True))
+    # (the goldens' own budget is 1e-2 a logit)
+    assert np.abs(np.array(got[0]["logprobs"]) - p[np.arange(len(p)), ids[k:]]).max() <= 2e-2
+    assert len(got) == 2 and len(got[1]["logprobs"]) == 1 and len(got[0]["top_ids"][0]) == 2
