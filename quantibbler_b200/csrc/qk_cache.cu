@@ -269,16 +269,18 @@ attend_plain_kernel(CacheView c, CacheView p, qk::AttendArgs a) {
 // ------------------------------------------------------------------ attention of few query rows
 // How a call is dealt out: blocks over the prefix first (all queries of a kv head in rows of eight, splits of the
 // prefix), then blocks over the sequences' own rows.  A split of a sequence's rows is the same part of every
-// sequence, so that unequal lengths keep all blocks at work.
+// sequence, so that unequal lengths keep all blocks at work.  The blocks of a cluster are neighbouring splits, whose
+// results they join themselves.
 struct Plan {
     uint32_t prefix_subs, prefix_splits, prefix_chunk, prefix_blocks;
     uint32_t own_subs, own_splits, own_rows;  // own_rows: query rows of a block
-    uint32_t n_slots;                         // partial results per (query, head); 1: none, the output is written
+    uint32_t cluster;                         // blocks of a cluster; the splits are whole numbers of clusters
+    uint32_t prefix_slots, n_slots;           // partial results per (query, head); n_slots 1: none, the output is written
 };
 
 // kMost: column tiles of four query rows that a block needs at most.
 template <bool kI8, int D, int kMost>
-__global__ void __launch_bounds__(128, kI8 ? (kMost == 1 ? 4 : 3) : 2)
+__global__ void __launch_bounds__(128, kI8 ? (kMost == 1 ? 4 : 3) : (kMost == 1 ? 3 : 2))
 attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     qk::pdl_launch();
     qk::pdl_wait();
@@ -288,30 +290,35 @@ attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     uint32_t id = blockIdx.x, kvh;
     const CacheView *src;
     size_t line;
+    const uint32_t rank = id % pl.cluster;
     if (id < pl.prefix_blocks) {
         src = &p;
-        const uint32_t sub = id % pl.prefix_subs, split = id / pl.prefix_subs % pl.prefix_splits;
-        kvh = id / pl.prefix_subs / pl.prefix_splits;
+        id /= pl.cluster;
+        const uint32_t sub = id % pl.prefix_subs, part = id / pl.prefix_subs % pl.prefix_slots;
+        const uint32_t split = part * pl.cluster + rank;
+        kvh = id / pl.prefix_subs / pl.prefix_slots;
         line = (a.prefix_seq * p.n_kv + kvh) * p.rows;
-        s.begin = (int)(split * pl.prefix_chunk);
+        s.begin = (int)min(a.prefix_len, split * pl.prefix_chunk);
         s.end = (int)min(a.prefix_len, (split + 1) * pl.prefix_chunk);
         s.first_row = sub * 8;
         s.n_rows = min(8u, a.n_queries * group - s.first_row);
-        s.slot = split;
+        s.slot = part;
     } else {
-        id -= pl.prefix_blocks;
+        id = (id - pl.prefix_blocks) / pl.cluster;
         src = &c;
-        const uint32_t sub = id % pl.own_subs;
+        const uint32_t sub = id % pl.own_subs, parts = pl.own_splits / pl.cluster;
         kvh = id / pl.own_subs % c.n_kv;
-        const uint32_t split = id / pl.own_subs / c.n_kv % pl.own_splits, b = id / pl.own_subs / c.n_kv / pl.own_splits;
-        line = ((size_t)b * c.n_kv + kvh) * c.rows;
-        const uint32_t len = (uint32_t)min(max(a.kv_len[b], 0), (int)c.rows);
+        const uint32_t part = id / pl.own_subs / c.n_kv % parts, b = id / pl.own_subs / c.n_kv / parts;
+        const uint32_t split = part * pl.cluster + rank;
+        line = ((a.kv_len ? b : a.seq) * c.n_kv + kvh) * c.rows;
+        // (without lengths: the one query of a portion of one token)
+        const uint32_t len = a.kv_len ? (uint32_t)min(max(a.kv_len[b], 0), (int)c.rows) : a.first_row + 1;
         const uint32_t chunk = ((len + pl.own_splits - 1) / pl.own_splits + 63) / 64 * 64;
         s.begin = (int)min(len, split * chunk);
         s.end = (int)min(len, (split + 1) * chunk);
         s.first_row = b * group + sub * pl.own_rows;
         s.n_rows = min(pl.own_rows, group - sub * pl.own_rows);
-        s.slot = pl.prefix_splits + split;
+        s.slot = pl.prefix_slots + part;
     }
     s.k = static_cast<const uint8_t *>(src->k) + line * row_bytes;
     s.v = static_cast<const uint8_t *>(src->v) + line * row_bytes;
@@ -319,11 +326,11 @@ attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     s.v_scale = kI8 ? src->v_scale + line : nullptr;
     if constexpr (kMost > 1) {
         if (s.n_rows > 4) {
-            attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+            attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, attend_smem);
             return;
         }
     }
-    attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, attend_smem);
+    attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, attend_smem);
 }
 
 // Partial results of a (query, head) joined: outputs [slot][D], then {maximum (log2 units), sum} [slot] of all rows.
@@ -475,7 +482,7 @@ bool takes_rows(const qk_kv_cache *c) { return c->dtype != QK_F32 && (c->head_di
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned_rows(const CacheView &v) { return aligned(v.k) && aligned(v.v); }
 
-constexpr size_t kWantBlocks = 148 * 8, kMinChunk = 128;
+constexpr size_t kWantBlocks = 148 * 8, kMinChunk = 256, kResident = 148 * 2;
 
 // The tile kernel takes 128 query rows to an SM: how often the keys (64 to a block, two blocks at a time) are split so
 // that the SMs have work.
@@ -486,28 +493,46 @@ uint32_t tile_splits(size_t tiles, size_t keys) {
 size_t tiles_of(const qk_kv_cache *c, size_t queries, size_t n_heads) {
     return qk::ceil_div(queries * (n_heads / c->n_kv_heads), 128) * c->n_kv_heads;
 }
-// More query rows than this on a prefix go through the tile kernel.  (A block of the other kernel takes eight rows.)
-constexpr size_t kTileRows = 16;
+// Whether the query rows on a prefix go eight at a time through attend_rows_kernel, or 128 at a time through the tile
+// kernel.  A block of the former costs the same for one row as for eight, 16 keys of a kv head about 0.7 ns of the whole
+// device; one of the latter costs 64 keys 9 ns whatever its rows, and the launch 10 us more.  Eight sequences of four rows
+// behind 4001 INT8 rows: 21 against 25 us; 64 of them behind 8192 bfloat16 rows: 131 against 49.
+bool prefix_by_rows(const qk_kv_cache *c, size_t rows, size_t prefix_len) {
+    return rows <= 16 || qk::ceil_div(rows, 8) * prefix_len * c->n_kv_heads <= (1u << 18);
+}
 
 Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_heads) {
     Plan pl{};
     const size_t group = n_heads / c->n_kv_heads;
     auto splits = [](size_t blocks, size_t rows) {
-        const size_t most = std::min<size_t>(128, qk::ceil_div(rows, kMinChunk));
-        return (uint32_t)std::max<size_t>(1, std::min(most, qk::ceil_div(kWantBlocks, blocks)));
+        return std::max<size_t>(1, std::min({(size_t)128, qk::ceil_div(rows, kMinChunk), qk::ceil_div(kWantBlocks, blocks)}));
     };
-    if (prefix_len && batch * group > kTileRows) {
-        pl.prefix_splits = tile_splits(tiles_of(c, batch, n_heads), prefix_len);
-    } else if (prefix_len) {
-        pl.prefix_subs = (uint32_t)qk::ceil_div(batch * group, 8);
-        pl.prefix_splits = splits(pl.prefix_subs * c->n_kv_heads, prefix_len);
-        pl.prefix_chunk = (uint32_t)(qk::ceil_div(qk::ceil_div(prefix_len, pl.prefix_splits), 64) * 64);
-        pl.prefix_blocks = (uint32_t)(pl.prefix_subs * pl.prefix_splits * c->n_kv_heads);
-    }
+    const bool by_rows = prefix_len && prefix_by_rows(c, batch * group, prefix_len);
     pl.own_rows = (uint32_t)std::min<size_t>(group, 8);
     pl.own_subs = (uint32_t)qk::ceil_div(group, pl.own_rows);
-    pl.own_splits = splits(batch * c->n_kv_heads * pl.own_subs, c->rows);
-    pl.n_slots = pl.prefix_splits + pl.own_splits;
+    pl.prefix_subs = (uint32_t)qk::ceil_div(batch * group, 8);
+    const size_t own_blocks = batch * c->n_kv_heads * pl.own_subs, pre_blocks = by_rows ? pl.prefix_subs * c->n_kv_heads : 0;
+    size_t own = splits(own_blocks, c->rows), pre = by_rows ? splits(pre_blocks, prefix_len) : 1;
+    // While all blocks are resident at once, the splits are the blocks of a cluster (up to 32 of them become eight), and
+    // there is no second launch: one sequence of 2048 INT8 rows, 32 heads: 14 -> 11.6 us a call on the host, the device's
+    // time the same.  Where blocks queue, clusters make them wait for one another: 64 sequences 42 -> 47 us.
+    pl.cluster = 1;
+    const size_t most = std::max(own, pre);
+    const size_t size = most > 4 ? 8 : most > 2 ? 4 : most;
+    if (most <= 32 && (own_blocks + pre_blocks) * size <= kResident) {
+        pl.cluster = (uint32_t)size;
+        own = pre = size;
+    }
+    pl.own_splits = (uint32_t)(qk::ceil_div(own, pl.cluster) * pl.cluster);
+    if (by_rows) {
+        pl.prefix_splits = (uint32_t)(qk::ceil_div(pre, pl.cluster) * pl.cluster);
+        pl.prefix_slots = pl.prefix_splits / pl.cluster;
+        pl.prefix_chunk = (uint32_t)(qk::ceil_div(qk::ceil_div(prefix_len, pl.prefix_splits), 64) * 64);
+        pl.prefix_blocks = (uint32_t)(pl.prefix_subs * pl.prefix_splits * c->n_kv_heads);
+    } else if (prefix_len) {
+        pl.prefix_slots = tile_splits(tiles_of(c, batch, n_heads), prefix_len);
+    }
+    pl.n_slots = pl.prefix_slots + pl.own_splits / pl.cluster;
     return pl;
 }
 
@@ -552,7 +577,8 @@ qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, con
     qk_status st = qk::allow_smem(c, attend_rows_kernel<kI8, D, kMost>, smem);
     if (st != QK_OK) return st;
     const unsigned blocks = pl.prefix_blocks + a.n_queries * own.n_kv * pl.own_subs * pl.own_splits;
-    QK_PDL(c, (attend_rows_kernel<kI8, D, kMost>), dim3(blocks), dim3(128), smem, own, pre, a, pl);
+    (void)qk::launch_pdl_cluster(c->pdl, attend_rows_kernel<kI8, D, kMost>, dim3(blocks), dim3(128), pl.cluster, smem, c->stream,
+                                 own, pre, a, pl);
     QK_CUDA(cudaGetLastError());
     c->launches++;
     return join(c, a, pl.n_slots, D);
@@ -560,7 +586,7 @@ qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, con
 template <bool kI8, int D>
 qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, const qk::AttendArgs &a, const Plan &pl) {
     if (a.prefix_len && !pl.prefix_blocks) {
-        qk_status st = prefix_tiles(c, pre, a, pl.prefix_splits, pl.n_slots);
+        qk_status st = prefix_tiles(c, pre, a, pl.prefix_slots, pl.n_slots);
         if (st != QK_OK) return st;
     }
     const uint32_t rows = pl.prefix_blocks ? std::max(pl.own_rows, std::min(8u, a.n_queries * (a.n_heads / own.n_kv))) : pl.own_rows;
@@ -576,7 +602,7 @@ qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefi
     const CacheView own = view(cache), pre = view(a.prefix_len ? prefix : nullptr);
     if (takes_rows(cache) && aligned_rows(own) && aligned_rows(pre) && aligned(a.q) && a.q_stride % 4 == 0) {
         if ((st = ready_error_word(c)) != QK_OK) return st;
-        if (!a.kv_len) {
+        if (!a.kv_len && a.n_queries > 1) {
             const PortionPlan pp = plan_portion(cache, a.first_row, a.prefix_len, a.n_queries, a.n_heads);
             const uint32_t slots = pp.prefix_splits + pp.own_splits;
             if (a.prefix_len && (st = prefix_tiles(c, pre, a, pp.prefix_splits, slots)) != QK_OK) return st;
@@ -741,6 +767,7 @@ qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cac
 size_t qk_cache_portion_scratch(const qk_kv_cache *cache, size_t first_row, size_t prefix_len, size_t n_tokens,
                                 size_t n_heads) {
     if (!cache || cache->n_kv_heads == 0 || n_heads < cache->n_kv_heads || !n_tokens || !takes_rows(cache)) return 0;
+    if (n_tokens == 1) return qk_cache_attend_scratch(cache, prefix_len, 1, n_heads);
     const PortionPlan pp = plan_portion(cache, first_row, prefix_len, n_tokens, n_heads);
     return partial_bytes(n_tokens, n_heads, pp.prefix_splits + pp.own_splits, cache->head_dim);
 }

@@ -97,6 +97,21 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b, int i) {
     return r;
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A shared-memory address of this block in the cluster's block `rank`.
+__device__ __forceinline__ uint32_t of_block(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float load_shared(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+
 // What a block works on: its query rows and its span of keys.
 struct Span {
     const void *k, *v;              // the kv head's rows, from row 0
@@ -110,10 +125,12 @@ template <bool kI8, int D>
 struct AttendShape {
     static constexpr int kRowBytes = kI8 ? D : 2 * D, kPieces = kRowBytes / 16;
     static constexpr int kStageBytes = 2 * 16 * kRowBytes + (kI8 ? 128 : 0);
-    static constexpr int kStages = kI8 && D == 64 ? 4 : 3;
+    static constexpr int kStages = kI8 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kQPitch = kRowBytes + 16;                     // bytes of one term of a query row
-    static constexpr int kSmem = 4 * kWarpBytes + 8 * 3 * kQPitch + 32;
+    static constexpr int kQBytes = 8 * 3 * kQPitch, kResultBytes = (8 * D + 16) * 4;  // (the block's results follow q's terms)
+    static constexpr int kTermBytes = kQBytes > kResultBytes ? kQBytes : kResultBytes;
+    static constexpr int kSmem = 4 * kWarpBytes + kTermBytes + 32;
     static_assert(kWarpBytes >= (8 * D + 16) * 4, "a warp's results lie in its ring");
     // (pieces of 16 bytes of a row change places so that fragment loads meet no bank twice)
     __device__ static uint32_t swizzle(uint32_t row, uint32_t piece) {
@@ -128,7 +145,7 @@ struct AttendShape {
 // kTiles: column tiles of query rows, four rows each.
 template <bool kI8, int D, int kTiles>
 __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &a, uint32_t kvh, uint32_t n_kv, uint32_t n_slots,
-                                            uint8_t *smem) {
+                                            uint32_t n_cluster, uint8_t *smem) {
     using Shape = AttendShape<kI8, D>;
     constexpr int kRowBytes = Shape::kRowBytes, kPieces = Shape::kPieces, kStages = Shape::kStages;
     constexpr int kQTiles = kTiles + 1;                              // column tiles of q: (first, second) term per row, then the thirds
@@ -181,7 +198,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
 
     // ---- q's terms, a warp per row: lines of [row][term] in shared memory
     uint8_t *q_lines = smem + 4 * Shape::kWarpBytes;
-    float *q_factor = reinterpret_cast<float *>(q_lines + 8 * 3 * Shape::kQPitch);  // what turns a row's sums into log2 units
+    float *q_factor = reinterpret_cast<float *>(q_lines + Shape::kTermBytes);  // what turns a row's sums into log2 units
     const float unit = kLog2E / sqrtf((float)D);
     for (uint32_t r = warp; r < 4 * kTiles; r += 4) {
         constexpr uint32_t kLanes = D / 4;  // lanes with four channels each
@@ -432,6 +449,22 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                 mine[r * D + (kI8 ? (D / 8) * g + 2 * i + h : 16 * i + 8 * h + g)] = o[n][i][h] * undo;
     }
     __syncthreads();
+    const bool alone = n_cluster == 1;
+    float *result = reinterpret_cast<float *>(q_lines);  // [8][D] outputs, [8] maxima, [8] sums: for the cluster's blocks
+    auto put = [&](uint32_t r, uint32_t c, float top, float sum, float val) {
+        const uint32_t row = s.first_row + r, query = row / group, head = kvh * group + row % group;
+        if (n_slots == 1) {
+            a.out[query * a.out_stride + (size_t)head * D + c] = sum == 0.f ? 0.f : val / sum;
+        } else {
+            const size_t at_slot = ((size_t)query * a.n_heads + head) * n_slots + s.slot;
+            a.scratch[at_slot * D + c] = val;
+            if (c == 0)
+                *reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * n_slots * D + 2 * at_slot) =
+                    make_float2(top, sum);
+        }
+    };
+    // (a warp without keys has the sum 0; a NaN stays)
+    auto share_of = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top); };
     for (uint32_t at = threadIdx.x; at < s.n_rows * D; at += 128) {
         const uint32_t r = at / D, c = at % D;
         float mw[4], top = -INFINITY, sum = 0.f, val = 0.f;
@@ -443,22 +476,49 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float *src = reinterpret_cast<const float *>(smem + w * Shape::kWarpBytes);
-            // (a warp without keys has nothing; NaN sums stay)
-            const float weight = mw[w] == -INFINITY ? (src[8 * D + 8 + r] == 0.f ? 0.f : 1.f) : ex2(mw[w] - top);
+            const float weight = share_of(mw[w], src[8 * D + 8 + r], top);
             sum = fmaf(src[8 * D + 8 + r], weight, sum);
             val = fmaf(src[r * D + c], weight, val);
         }
-        const uint32_t row = s.first_row + r, query = row / group, head = kvh * group + row % group;
-        if (n_slots == 1) {
-            a.out[query * a.out_stride + (size_t)head * D + c] = sum == 0.f ? 0.f : val / sum;
+        if (alone) {
+            put(r, c, top, sum, val);
         } else {
-            const size_t at_slot = ((size_t)query * a.n_heads + head) * n_slots + s.slot;
-            a.scratch[at_slot * D + c] = val;
-            if (c == 0)
-                *reinterpret_cast<float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * n_slots * D + 2 * at_slot) =
-                    make_float2(top, sum);
+            result[r * D + c] = val;
+            if (c == 0) result[8 * D + r] = top, result[8 * D + 8 + r] = sum;
         }
     }
+    if (alone) return;
+    // ---- the splits of a cluster join through distributed shared memory, every block a part of the outputs
+    cluster_sync();
+    uint32_t rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t here = smem_addr(result);
+    for (uint32_t at = rank * 128 + threadIdx.x; at < s.n_rows * D; at += n_cluster * 128) {
+        const uint32_t r = at / D, c = at % D;
+        float m[8], l[8], v[8], top = -INFINITY, sum = 0.f, val = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (i >= n_cluster) break;
+            const uint32_t there = of_block(here, i);
+            v[i] = load_shared(there + (r * D + c) * 4);
+            m[i] = load_shared(there + (8 * D + r) * 4);
+            l[i] = load_shared(there + (8 * D + 8 + r) * 4);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (i >= n_cluster) break;
+            top = fmaxf(top, m[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (i >= n_cluster) break;
+            const float weight = share_of(m[i], l[i], top);
+            sum = fmaf(l[i], weight, sum);
+            val = fmaf(v[i], weight, val);
+        }
+        put(r, c, top, sum, val);
+    }
+    cluster_sync();  // (no block ends while another reads its results)
 }
 
 }  // namespace
