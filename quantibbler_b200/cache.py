@@ -93,7 +93,7 @@ class KvCache:
 
     def __init__(self, ctx: GpuContext, k, v, k_scale=None, v_scale=None, first_position: int = 0):
         import torch
-        self._torch, self._f32, self.ctx = torch, torch.float32, ctx
+        self._torch, self._f32, self._i32, self.ctx = torch, torch.float32, torch.int32, ctx
         names = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.int8: "int8"}
         if k.dtype not in names:
             raise KernelError(f"a cache holds float32, bfloat16 or int8, got {str(k.dtype).replace('torch.', '')}")
@@ -159,9 +159,14 @@ class KvCache:
         return t.shape[0], (t.stride(0) if t.shape[0] > 1 else width)
 
     def _places(self, positions, seq_index, tokens: int | None = None) -> int:
-        n = positions.shape[0] if positions.dim() == 1 else -1
+        shape = positions.shape
+        if (positions.dtype is self._i32 and seq_index.dtype is self._i32 and len(shape) == 1 and seq_index.shape == shape
+                and (tokens is None or shape[0] == tokens) and positions.device == self.device
+                and seq_index.device == self.device and positions.is_contiguous() and seq_index.is_contiguous()):
+            return shape[0]
+        n = shape[0] if len(shape) == 1 else -1
         for what, t in (("positions", positions), ("seq_index", seq_index)):
-            check_tensor(what, t, self._torch.int32, self.device, (n if tokens is None else tokens,))
+            check_tensor(what, t, self._i32, self.device, (n if tokens is None else tokens,))
             if not t.is_contiguous():
                 raise KernelError(f"{what} must be contiguous")
         return n
@@ -206,8 +211,7 @@ class KvCache:
         if dtype not in ("float32", "bfloat16"):
             raise KernelError(f"rows are read as float32 or bfloat16, got {dtype!r}")
         n = self._places(positions, seq_index)
-        k, v = (torch.empty((n, self.n_kv_heads, self.head_dim), dtype=getattr(torch, dtype), device=self.device)
-                for _ in range(2))
+        k, v = torch.empty((2, n, self.n_kv_heads, self.head_dim), dtype=getattr(torch, dtype), device=self.device).unbind(0)
         if n:
             with ordered(self.ctx, self.device):
                 check(_lib.lib().qk_cache_read(self.ctx.handle, self._ref, positions.data_ptr(), seq_index.data_ptr(),
@@ -237,7 +241,7 @@ class KvCache:
         nothing gets zeros.  Returns ``out`` (default: a new tensor)."""
         n, q_stride = self._rows("q", q, None)
         heads = q.shape[1]
-        check_tensor("kv_len", kv_len, self._torch.int32, self.device, (n,))
+        check_tensor("kv_len", kv_len, self._i32, self.device, (n,))
         if not kv_len.is_contiguous():
             raise KernelError("kv_len must be contiguous")
         ref = self._prefix(prefix, prefix_len, prefix_seq)

@@ -1,6 +1,7 @@
 // Key/value caches in float32, bfloat16 and INT8: appending with rotation and quantisation, reading back, the
 // attention of a step and of a prompt's portion, both with rows in front that all sequences share.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -10,23 +11,27 @@
 namespace {
 
 // ------------------------------------------------------------------ append
-// x / scale, rounded to the nearest integer (ties to even) as 64-bit arithmetic does it: the 32-bit quotient is
-// off by less than 1e-4 (127 * 2^-22 from x and its division), so only next to a border is the division done in
-// 64 bits.
-__device__ __forceinline__ int quantise(double x, float scale, float inv) {
-    const float t = (float)x * inv;
-    if (fabsf(fabsf(t - truncf(t)) - 0.5f) > 1e-3f) return min(127, max(-127, __float2int_rn(t)));
-    return min(127, max(-127, __double2int_rn(x / (double)scale)));
-}
-
-// Whether a later token of the call names the same row.  All threads of the block take part.
-__device__ __forceinline__ bool superseded(const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index,
-                                           uint32_t tok, uint32_t n_tokens) {
-    const int pos = positions[tok], seq = seq_index[tok];
-    int later = 0;
-    for (uint32_t i = tok + 1 + threadIdx.x; i < n_tokens; i += blockDim.x)
-        later |= positions[i] == pos && seq_index[i] == seq;
-    return __syncthreads_or(later) != 0;
+// Whether a later token of the call names the same row, as far as this thread looks: the block's threads share the
+// tokens, four at a time where the lists lie on 16 bytes.
+__device__ __forceinline__ bool named_again(const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index,
+                                            uint32_t tok, int pos, int seq, uint32_t n_tokens) {
+    bool later = false;
+    if ((((uintptr_t)positions | (uintptr_t)seq_index) & 15) == 0) {
+        const uint32_t whole = n_tokens / 4;
+        const int4 *p4 = reinterpret_cast<const int4 *>(positions), *s4 = reinterpret_cast<const int4 *>(seq_index);
+#pragma unroll 2
+        for (uint32_t i = (tok + 1) / 4 + threadIdx.x; i < whole; i += blockDim.x) {
+            const int4 p = p4[i], s = s4[i];
+            const uint32_t t = 4 * i;
+            later |= (p.x == pos && s.x == seq && t > tok) | (p.y == pos && s.y == seq && t + 1 > tok) |
+                     (p.z == pos && s.z == seq && t + 2 > tok) | (p.w == pos && s.w == seq && t + 3 > tok);
+        }
+        const uint32_t i = 4 * whole + threadIdx.x;
+        if (i < n_tokens) later |= positions[i] == pos && seq_index[i] == seq && i > tok;
+    } else {
+        for (uint32_t i = tok + 1 + threadIdx.x; i < n_tokens; i += blockDim.x) later |= positions[i] == pos && seq_index[i] == seq;
+    }
+    return later;
 }
 
 // The largest of the lanes' non-negative numbers (their bits are in their order).
@@ -36,6 +41,14 @@ __device__ __forceinline__ double warp_peak(double x) {
     return __hiloint2double((int)top, (int)lo);
 }
 
+// Four codes, clipped to -127 .. 127.
+__device__ __forceinline__ uint32_t pack_codes(const int (&n)[4]) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= (uint32_t)(min(127, max(-127, n[e])) & 0xff) << (8 * e);
+    return w;
+}
+
 // n consecutive values.
 template <int kN, typename T>
 __device__ __forceinline__ void load_n(const T *p, T (&v)[kN]) {
@@ -43,128 +56,239 @@ __device__ __forceinline__ void load_n(const T *p, T (&v)[kN]) {
     *reinterpret_cast<V *>(v) = *reinterpret_cast<const V *>(p);
 }
 
-// One block per token and share of its rows; a warp per row (a head of q, k or v) at a time.  A lane rotates pairs
-// (i, i + d/2) and keeps their angles for all rows of the token.  kPairs > 0: a lane has kPairs neighbouring pairs and
-// loads them as vectors; 0: any even head size, addresses of any alignment.
-// What bounds it: a long prompt's bytes (q read and written in float32 are most of them); a step's few rows are latency.
-template <typename KV, int kPairs>  // KV: float, uint16_t (bfloat16), int8_t
+// Any even head size, addresses of any alignment: a warp per row (a head of q, k or v), a lane has the pairs (i, i + d/2),
+// i = lane, lane + 32, ..
+template <typename KV>  // float, uint16_t (bfloat16), int8_t
 __global__ void __launch_bounds__(256)
-append_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t q_out_stride,
-              uint32_t n_heads, const float *__restrict__ k, size_t k_stride, const float *__restrict__ v, size_t v_stride,
+append_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t q_out_stride, uint32_t n_heads,
+              const float *__restrict__ k, size_t k_stride, const float *__restrict__ v, size_t v_stride,
               const float *__restrict__ cos_sin, uint32_t n_positions, const int32_t *__restrict__ positions,
               const int32_t *__restrict__ seq_index, uint32_t first_position, uint32_t n_tokens, int *__restrict__ error) {
     qk::pdl_launch();
     qk::pdl_wait();
-    constexpr int kMine = kPairs ? kPairs : 4;  // pairs of a lane (head_dim <= 256)
-    const uint32_t tok = blockIdx.x, half = c.d / 2, lane = threadIdx.x % 32, warps = gridDim.y * (blockDim.x / 32);
-    const uint32_t warp = blockIdx.y * (blockDim.x / 32) + threadIdx.x / 32;
+    constexpr int kMine = 4;  // (head_dim <= 256)
+    const uint32_t tok = blockIdx.x, d = c.d, half = d / 2, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t pos = positions[tok], seq = seq_index[tok], row = pos - (int64_t)first_position;
     if (row < 0 || row >= (int64_t)c.rows || pos >= (int64_t)n_positions || seq < 0 || seq >= (int64_t)c.n_seq) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(error, 4);
+        if (threadIdx.x == 0) atomicOr(error, 4);
         return;
     }
-    auto pair_of = [&](int e) { return kPairs ? lane * kPairs + e : lane + 32 * e; };
-    auto load_pairs = [&](const float *src, float (&a)[kMine], float (&b)[kMine]) {
-        if constexpr (kPairs > 0) {
-            load_n<kPairs>(src + lane * kPairs, a);
-            load_n<kPairs>(src + half + lane * kPairs, b);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kMine; ++e) {
-                const uint32_t i = pair_of(e);
-                a[e] = i < half ? src[i] : 0.f, b[e] = i < half ? src[half + i] : 0.f;
+    const float *cs = cos_sin + (size_t)pos * d;
+    if (q)
+        for (uint32_t h = warp; h < n_heads; h += 8) {
+            const float *src = q + tok * q_stride + (size_t)h * d;
+            float *dst = q_out + tok * q_out_stride + (size_t)h * d;
+            for (uint32_t i = lane; i < half; i += 32) {
+                const float a = src[i], b = src[half + i], co = cs[2 * i], si = cs[2 * i + 1];
+                dst[i] = rope_first(a, b, co, si);
+                dst[half + i] = rope_second(a, b, co, si);
             }
         }
-    };
-    auto store_pairs = [&](auto *dst, const auto &a, const auto &b) {
-        using T = std::remove_reference_t<decltype(*dst)>;
-        if constexpr (kPairs > 0 && (kPairs * sizeof(T) == 2 || kPairs * sizeof(T) == 4 || kPairs * sizeof(T) >= 8)) {
-            using V = std::conditional_t<kPairs * sizeof(T) == 16, uint4,
-                                         std::conditional_t<kPairs * sizeof(T) == 8, uint2,
-                                                            std::conditional_t<kPairs * sizeof(T) == 4, uint32_t, uint16_t>>>;
-            *reinterpret_cast<V *>(dst + lane * kPairs) = *reinterpret_cast<const V *>(a);
-            *reinterpret_cast<V *>(dst + half + lane * kPairs) = *reinterpret_cast<const V *>(b);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kMine; ++e) {
-                const uint32_t i = pair_of(e);
-                if (i < half) dst[i] = a[e], dst[half + i] = b[e];
-            }
-        }
-    };
-    float co[kMine], si[kMine];
-    {
-        const float *cs = cos_sin + (size_t)pos * c.d;
-#pragma unroll
-        for (int e = 0; e < kMine; ++e) {
-            const uint32_t i = pair_of(e);
-            const float2 t = i < half ? make_float2(cs[2 * i], cs[2 * i + 1]) : make_float2(1.f, 0.f);
-            co[e] = t.x, si[e] = t.y;
-        }
-    }
-    if (q) {
-        constexpr uint32_t kRows = 2;  // rows in flight
-        for (uint32_t h0 = warp; h0 < n_heads; h0 += kRows * warps) {
-            alignas(16) float a[kRows][kMine], b[kRows][kMine];
-#pragma unroll
-            for (uint32_t u = 0; u < kRows; ++u)
-                if (h0 + u * warps < n_heads) load_pairs(q + tok * q_stride + (size_t)(h0 + u * warps) * c.d, a[u], b[u]);
-#pragma unroll
-            for (uint32_t u = 0; u < kRows; ++u) {
-                if (h0 + u * warps >= n_heads) break;
-                alignas(16) float x[kMine], y[kMine];
-#pragma unroll
-                for (int e = 0; e < kMine; ++e) {
-                    x[e] = rope_first(a[u][e], b[u][e], co[e], si[e]);
-                    y[e] = rope_second(a[u][e], b[u][e], co[e], si[e]);
-                }
-                store_pairs(q_out + tok * q_out_stride + (size_t)(h0 + u * warps) * c.d, x, y);
-            }
-        }
-    }
-    if (superseded(positions, seq_index, tok, n_tokens)) return;
-    // (the warps that had fewer rows of q first)
-    for (uint32_t r = warps - 1 - warp; r < 2 * c.n_kv; r += warps) {
+    if (__syncthreads_or(named_again(positions, seq_index, tok, (int)pos, (int)seq, n_tokens))) return;  // (that one stays)
+    for (uint32_t r = warp; r < 2 * c.n_kv; r += 8) {
         const bool is_k = r < c.n_kv;
         const uint32_t h = is_k ? r : r - c.n_kv;
-        alignas(16) float a[kMine], b[kMine];
-        load_pairs((is_k ? k + tok * k_stride : v + tok * v_stride) + (size_t)h * c.d, a, b);
+        const float *src = (is_k ? k + tok * k_stride : v + tok * v_stride) + (size_t)h * d;
         const size_t line = ((size_t)seq * c.n_kv + h) * c.rows + (size_t)row;
-        KV *dst = static_cast<KV *>(is_k ? c.k : c.v) + line * c.d;
-        alignas(16) KV x[kMine], y[kMine];
+        KV *dst = static_cast<KV *>(is_k ? c.k : c.v) + line * d;
         if constexpr (sizeof(KV) != 1) {
-#pragma unroll
-            for (int e = 0; e < kMine; ++e) {
-                store_from_float<KV>(x, e, is_k ? rope_first(a[e], b[e], co[e], si[e]) : a[e]);
-                store_from_float<KV>(y, e, is_k ? rope_second(a[e], b[e], co[e], si[e]) : b[e]);
+            for (uint32_t i = lane; i < half; i += 32) {
+                const float a = src[i], b = src[half + i], co = cs[2 * i], si = cs[2 * i + 1];
+                store_from_float<KV>(dst, i, is_k ? rope_first(a, b, co, si) : a);
+                store_from_float<KV>(dst, half + i, is_k ? rope_second(a, b, co, si) : b);
             }
         } else {
-            // In 64 bits, where products of two float32 are exact.
-            double p[kMine], s[kMine], peak = 0.0;
+            double x[2][kMine], peak = 0.0;  // in 64 bits, where products of two float32 are exact
             bool finite = true;
 #pragma unroll
             for (int e = 0; e < kMine; ++e) {
-                p[e] = a[e], s[e] = b[e];
-                if (is_k) {
-                    const double x0 = p[e], y0 = s[e];
-                    p[e] = fma(x0, (double)co[e], -(y0 * (double)si[e]));
-                    s[e] = fma(y0, (double)co[e], x0 * (double)si[e]);
+                const uint32_t i = lane + 32 * e;
+                x[0][e] = x[1][e] = 0.0;
+                if (i >= half) continue;
+                const double a = src[i], b = src[half + i], co = is_k ? cs[2 * i] : 1.0, si = is_k ? cs[2 * i + 1] : 0.0;
+                x[0][e] = is_k ? fma(a, co, -(b * si)) : a;
+                x[1][e] = is_k ? fma(b, co, a * si) : b;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    finite = finite && fabs(x[w][e]) <= (double)FLT_MAX;
+                    peak = fmax(peak, fabs(x[w][e]));
                 }
-                finite = finite && fabs(p[e]) < INFINITY && fabs(s[e]) < INFINITY;
-                peak = fmax(peak, fmax(fabs(p[e]), fabs(s[e])));
             }
             finite = __all_sync(0xffffffffu, finite);
             float scale = (float)(warp_peak(peak) / 127.0);
             if (scale == 0.f) scale = 1.f;
-            const float inv = 1.f / scale;  // (infinite for the smallest scales: then every code takes the division)
 #pragma unroll
             for (int e = 0; e < kMine; ++e) {
-                x[e] = (int8_t)(finite ? quantise(p[e], scale, inv) : 0);
-                y[e] = (int8_t)(finite ? quantise(s[e], scale, inv) : 0);
+                const uint32_t i = lane + 32 * e;
+                if (i >= half) continue;
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    dst[w * half + i] =
+                        (int8_t)(finite ? min(127, max(-127, __double2int_rn(x[w][e] / (double)scale))) : 0);
             }
             if (lane == 0) (is_k ? c.k_scale : c.v_scale)[line] = finite ? scale : __int_as_float(0x7fffffff);
         }
-        store_pairs(dst, x, y);
+    }
+}
+
+// Head sizes 64 kGroups on 16-byte boundaries: eight lanes to a row, four rows to a warp at once (what a row
+// costs beside its entries - the reductions, the division that gives the scale - is paid once for four), kGroups vectors
+// of four pairs a lane.  2048 tokens, 32 / 8 heads of 128: 26 us with a row to a warp, most of it issue.
+template <typename KV, int kGroups>
+__global__ void __launch_bounds__(128, kGroups == 4 ? 4 : 8)
+append_wide_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t q_out_stride, uint32_t n_heads,
+                   const float *__restrict__ k, size_t k_stride, const float *__restrict__ v, size_t v_stride,
+                   const float *__restrict__ cos_sin, uint32_t n_positions, const int32_t *__restrict__ positions,
+                   const int32_t *__restrict__ seq_index, uint32_t first_position, uint32_t n_tokens, uint32_t kv_blocks,
+                   int *__restrict__ error) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    constexpr uint32_t d = 64 * kGroups, half = d / 2;
+    constexpr int kMine = 4 * kGroups;  // pairs of a lane: 32 g + 4 (lane % 8) ..
+    const uint32_t tok = blockIdx.x, lane = threadIdx.x % 32, i0 = 4 * (lane % 8);
+    const bool is_q = blockIdx.y >= kv_blocks;
+    const uint32_t r = (is_q ? blockIdx.y - kv_blocks : blockIdx.y) * 16 + threadIdx.x / 8;
+    const bool is_k = r < c.n_kv, live = r < (is_q ? n_heads : 2 * c.n_kv);
+    const uint32_t h = is_q || is_k ? r : r - c.n_kv;
+    const int64_t pos = positions[tok], seq = seq_index[tok], row = pos - (int64_t)first_position;
+    const float *src = (is_q ? q + tok * q_stride : is_k ? k + tok * k_stride : v + tok * v_stride) + h * d + i0;
+    float a[kMine], b[kMine];
+    if (live) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            *reinterpret_cast<float4 *>(a + 4 * g) = *reinterpret_cast<const float4 *>(src + 32 * g);
+            *reinterpret_cast<float4 *>(b + 4 * g) = *reinterpret_cast<const float4 *>(src + half + 32 * g);
+        }
+    }
+    if (row < 0 || row >= (int64_t)c.rows || pos >= (int64_t)n_positions || seq < 0 || seq >= (int64_t)c.n_seq) {
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(error, 4);
+        return;
+    }
+    // (a later token of the call with the same row stays; its list is read while the row's entries are on their way)
+    const bool later = !is_q && named_again(positions, seq_index, tok, (int)pos, (int)seq, n_tokens);
+    const bool turned = is_q || is_k;
+    float co[kMine], si[kMine];
+    if (live && turned) {
+        const float *cs = cos_sin + (size_t)pos * d + 2 * i0;
+#pragma unroll
+        for (int e = 0; e < kMine; e += 2) {
+            const float4 t = *reinterpret_cast<const float4 *>(cs + e / 4 * 64 + e % 4 * 2);
+            co[e] = t.x, si[e] = t.y, co[e + 1] = t.z, si[e + 1] = t.w;
+        }
+    }
+    float p[2][kMine];
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        p[0][e] = !live ? 0.f : turned ? rope_first(a[e], b[e], co[e], si[e]) : a[e];
+        p[1][e] = !live ? 0.f : turned ? rope_second(a[e], b[e], co[e], si[e]) : b[e];
+    }
+    if (is_q) {
+        float *dst = q_out + tok * q_out_stride + h * d + i0;
+        if (live)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                *reinterpret_cast<float4 *>(dst + 32 * g) = *reinterpret_cast<const float4 *>(p[0] + 4 * g);
+                *reinterpret_cast<float4 *>(dst + half + 32 * g) = *reinterpret_cast<const float4 *>(p[1] + 4 * g);
+            }
+        return;
+    }
+    if (__syncthreads_or(later)) return;
+    const size_t line = ((size_t)seq * c.n_kv + h) * c.rows + (size_t)row;
+    KV *dst = static_cast<KV *>(is_k ? c.k : c.v) + line * d + i0;
+    if constexpr (sizeof(KV) == 4) {
+        if (live)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                *reinterpret_cast<float4 *>(dst + 32 * g) = *reinterpret_cast<const float4 *>(p[0] + 4 * g);
+                *reinterpret_cast<float4 *>(dst + half + 32 * g) = *reinterpret_cast<const float4 *>(p[1] + 4 * g);
+            }
+    } else if constexpr (sizeof(KV) == 2) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                uint16_t x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = float_to_bf16_bits(p[w][4 * g + e]);
+                if (live)
+                    *reinterpret_cast<uint2 *>(dst + w * half + 32 * g) =
+                        make_uint2((uint32_t)x[1] << 16 | x[0], (uint32_t)x[3] << 16 | x[2]);
+            }
+    } else {
+        // The codes are those of 64-bit arithmetic (products of two float32 are exact there).  float32 gives an entry to
+        // 2^-22 of the row's largest, 3e-5 of a code's width: the largest entry, and entries as near as 1e-3 to the border
+        // between two codes, are formed again in 64 bits.
+        auto exactly = [&](int e, int w) {
+            // (seldom: read again, not kept)
+            const uint32_t at = e / 4 * 32 + e % 4;
+            if (!is_k) return (double)src[w * half + at];
+            const float2 turn = *reinterpret_cast<const float2 *>(cos_sin + (size_t)pos * d + 2 * (i0 + at));
+            const double x = src[at], y = src[half + at], co64 = turn.x, si64 = turn.y;
+            return w ? fma(y, co64, x * si64) : fma(x, co64, -(y * si64));
+        };
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e)
+            mine = max(mine, max(__float_as_uint(fabsf(p[0][e])), __float_as_uint(fabsf(p[1][e]))));
+        uint32_t top = mine;
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const bool finite = top < 0x7f800000u;  // (an infinity or NaN is larger than any number)
+        const float near_top = __uint_as_float(top) * (1.f - 0x1p-20f);
+        double peak = (double)__uint_as_float(mine);
+        if (is_k) {
+            peak = 0.0;  // (unless another lane has the largest)
+            if (live && __uint_as_float(mine) >= near_top) {
+                int which = 0, several = 0;  // entries that may be the largest: nearly always one
+#pragma unroll
+                for (int e = 0; e < 2 * kMine; ++e)
+                    if (fabsf(p[e / kMine][e % kMine]) >= near_top) which = e, ++several;
+                if (several == 1)
+                    peak = fabs(exactly(which % kMine, which / kMine));
+                else
+                    for (int e = 0; e < 2 * kMine; ++e) peak = fmax(peak, fabs(exactly(e % kMine, e / kMine)));
+            }
+        }
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) peak = fmax(peak, __shfl_xor_sync(0xffffffffu, peak, off));
+        float scale = (float)(peak / 127.0);
+        if (scale == 0.f) scale = 1.f;
+        const float inv = 1.f / scale;
+        uint32_t codes[2][kGroups];
+        float off_code = 0.f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                uint32_t n[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // (1.5 2^23 more: the nearest integer, ties to even, in the low bits)
+                    const float x = p[w][4 * g + e] * inv, more = x + 12582912.f;
+                    off_code = fmaxf(off_code, fabsf(x - (more - 12582912.f)));
+                    n[e] = __float_as_uint(more);
+                }
+                codes[w][g] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+            }
+        // (the smallest scales, whose reciprocal may be infinite and who may round by much, too)
+        if (live && finite && (off_code > 0.499f || !(inv < 0x1p120f))) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    int n[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) n[e] = __double2int_rn(exactly(4 * g + e, w) / (double)scale);
+                    codes[w][g] = pack_codes(n);
+                }
+        }
+        if (!live) return;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            *reinterpret_cast<uint32_t *>(dst + 32 * g) = finite ? codes[0][g] : 0u;
+            *reinterpret_cast<uint32_t *>(dst + half + 32 * g) = finite ? codes[1][g] : 0u;
+        }
+        if (lane % 8 == 0) (is_k ? c.k_scale : c.v_scale)[line] = finite ? scale : __int_as_float(0x7fffffff);
     }
 }
 
@@ -394,6 +518,50 @@ join_kernel(qk::AttendArgs a, uint32_t n_slots) {
     }
 }
 
+// The same for up to 32 slots: a warp each, no barriers; the first outputs are on their way with the maxima and sums.
+template <int D>
+__global__ void __launch_bounds__(128)
+join_few_kernel(qk::AttendArgs a, uint32_t n_slots) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    using V = std::conditional_t<D == 128, float4, float2>;
+    constexpr uint32_t kMine = D / 32, kAhead = 4;
+    const uint32_t row = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (row >= a.n_queries * a.n_heads) return;
+    const V *outs = reinterpret_cast<const V *>(a.scratch + (size_t)row * n_slots * D) + lane;
+    const float2 *stats = reinterpret_cast<const float2 *>(a.scratch + (size_t)a.n_queries * a.n_heads * n_slots * D) +
+                          (size_t)row * n_slots;
+    V x[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) x[i] = outs[(size_t)min(i, n_slots - 1) * 32];
+    const float2 st = lane < n_slots ? stats[lane] : make_float2(-INFINITY, 0.f);
+    float top = st.x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    // (a span without keys has the sum 0; a NaN stays)
+    const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : ex2(st.x - top);
+    float sum = st.y * w, v[kMine] = {};
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (uint32_t s0 = 0; s0 < n_slots; s0 += kAhead) {
+        V y[kAhead];
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) y[i] = outs[(size_t)min(s0 + kAhead + i, n_slots - 1) * 32];
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const float ws = __shfl_sync(0xffffffffu, w, (s0 + i) & 31);
+            const float *xs = reinterpret_cast<const float *>(&x[i]);
+            if (s0 + i < n_slots)
+#pragma unroll
+                for (uint32_t e = 0; e < kMine; ++e) v[e] = fmaf(xs[e], ws, v[e]);
+            x[i] = y[i];
+        }
+    }
+    float *dst = a.out + (size_t)(row / a.n_heads) * a.out_stride + (size_t)(row % a.n_heads) * D + lane * kMine;
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) dst[e] = sum == 0.f ? 0.f : v[e] / sum;
+}
+
 // ------------------------------------------------------------------ host side
 using qk::DeviceGuard;
 
@@ -550,8 +718,10 @@ size_t partial_bytes(size_t queries, size_t n_heads, size_t slots, size_t d) {
 
 qk_status join(qk_ctx *c, const qk::AttendArgs &a, uint32_t n_slots, uint32_t d) {
     if (n_slots == 1) return QK_OK;
-    const dim3 grid(a.n_queries * a.n_heads);
-    if (d == 128) QK_PDL(c, join_kernel<128>, grid, dim3(128), 0, a, n_slots);
+    const dim3 grid(a.n_queries * a.n_heads), few((unsigned)qk::ceil_div((size_t)a.n_queries * a.n_heads, 4));
+    if (n_slots <= 32 && d == 128) QK_PDL(c, join_few_kernel<128>, few, dim3(128), 0, a, n_slots);
+    else if (n_slots <= 32) QK_PDL(c, join_few_kernel<64>, few, dim3(128), 0, a, n_slots);
+    else if (d == 128) QK_PDL(c, join_kernel<128>, grid, dim3(128), 0, a, n_slots);
     else QK_PDL(c, join_kernel<64>, grid, dim3(128), 0, a, n_slots);
     QK_CUDA(cudaGetLastError());
     c->launches++;
@@ -664,28 +834,30 @@ qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q,
     if (n_tokens == 0) return QK_OK;
     std::lock_guard<std::mutex> lock(c->mu);
     if ((st = ready_error_word(c)) != QK_OK) return st;
-    const size_t rows = (q ? n_heads : 0) + 2 * cache->n_kv_heads;
-    const size_t most = qk::ceil_div(rows, 8), want = qk::ceil_div((size_t)c->sm_count * 4, n_tokens);
-    const dim3 grid((unsigned)n_tokens, (unsigned)std::min(most, want));
     const CacheView cv = view(cache);
     int *err = (int *)c->d_err.ptr;
     // (a row's vectors lie on their boundaries where the tensors' addresses and strides do)
     const size_t mask = ((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cv.k | (uintptr_t)cv.v) |
                         (q ? (q_stride | q_out_stride) * 4 : 0) | (k_stride | v_stride) * 4;
-    const int pairs = mask % 16 ? 0 : d == 128 ? 2 : d == 256 ? 4 : 0;
-#define QK_APPEND_N(KV, N)                                                                                                  \
-    QK_PDL(c, (append_kernel<KV, N>), grid, dim3(256), 0, cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, \
-           v, v_stride, cos_sin, (uint32_t)n_positions, positions, seq_index, (uint32_t)first_position, (uint32_t)n_tokens, err)
-#define QK_APPEND(KV)                          \
-    do {                                       \
-        if (pairs == 2) QK_APPEND_N(KV, 2);    \
-        else if (pairs == 4) QK_APPEND_N(KV, 4); \
-        else QK_APPEND_N(KV, 0);               \
+    const int groups = mask % 16 || (uintptr_t)cos_sin % 16 ? 0 : d == 64 ? 1 : d == 128 ? 2 : d == 256 ? 4 : 0;
+#define QK_APPEND_ARGS                                                                                                    \
+    cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, v, v_stride, cos_sin, (uint32_t)n_positions, positions, \
+        seq_index, (uint32_t)first_position, (uint32_t)n_tokens
+#define QK_APPEND_WIDE(KV, N) QK_PDL(c, (append_wide_kernel<KV, N>), wide, dim3(128), 0, QK_APPEND_ARGS, wide_kv, err)
+#define QK_APPEND(KV)                                                                                        \
+    do {                                                                                                     \
+        if (groups == 1) QK_APPEND_WIDE(KV, 1);                                                              \
+        else if (groups == 2) QK_APPEND_WIDE(KV, 2);                                                         \
+        else if (groups == 4) QK_APPEND_WIDE(KV, 4);                                                         \
+        else QK_PDL(c, append_kernel<KV>, dim3((unsigned)n_tokens), dim3(256), 0, QK_APPEND_ARGS, err);      \
     } while (0)
+    const uint32_t wide_kv = (uint32_t)qk::ceil_div(2 * cache->n_kv_heads, 16);
+    const dim3 wide((unsigned)n_tokens, wide_kv + (unsigned)(q ? qk::ceil_div(n_heads, 16) : 0));
     if (cv.dtype == QK_I8) QK_APPEND(int8_t);
     else if (cv.dtype == QK_BF16) QK_APPEND(uint16_t);
     else QK_APPEND(float);
-#undef QK_APPEND_N
+#undef QK_APPEND_WIDE
+#undef QK_APPEND_ARGS
 #undef QK_APPEND
     QK_CUDA(cudaGetLastError());
     c->launches++;

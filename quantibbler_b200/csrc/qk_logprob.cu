@@ -17,7 +17,7 @@ namespace {
 constexpr uint32_t kMaxTop = 32, kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMinSlice = 2048;   // entries a block takes at least
 constexpr uint32_t kHeld = 8;          // vectors of four entries that a thread keeps in registers
-constexpr uint32_t kCandidates = 256;  // places for entries that may be among the best of a slice
+constexpr uint32_t kCandidates = 512;  // places for entries that may be among the best of a slice
 constexpr uint32_t kWantBlocks = 148 * 8;
 constexpr float kLog2E = 1.4426950408889634f;
 
@@ -195,24 +195,28 @@ log_probs_kernel(LogProbArgs a) {
 }
 
 // With the most probable entries: a slice of at most 32 entries a thread (and a single one) stays in registers.  The
-// n_top-th of the 256 threads' best entries is no better than the slice's n_top-th entry: what is as good as that, a
-// few more than n_top entries, one warp sorts.  (64 rows of 128256, 20 places: whatever beats a running last place
-// sorted warp by warp 93 us; the bound from each warp's 32 threads 44.)
-__global__ void __launch_bounds__(kThreads)
+// n_top-th of the largest values of 32 groups of eight threads is no better than the slice's n_top-th entry: what is as
+// good as that, 30 to 110 entries of a slice of 8192 without ties, goes into a list whose places are found by counting.
+// Where the list overflows because many entries equal the bound (masked vocabularies), those of the lowest indices are
+// taken; where it overflows without them, the warps sort.
+// (64 rows of 128256, 20 places: whatever beats a running last place sorted warp by warp 93 us; the bound from the 256
+// threads' best, sorted, and a sorted list 26.)
+__global__ void __launch_bounds__(kThreads, 3)
 log_probs_top_kernel(LogProbArgs a) {
     qk::pdl_launch();
     qk::pdl_wait();
-    __shared__ Stats part[kWarps];
-    __shared__ uint64_t bound_key, candidates[kCandidates];
-    __shared__ uint64_t best_of[kWarps][32];
-    __shared__ uint32_t n_candidates;
+    __shared__ float2 part[kWarps];
+    __shared__ float group_best[32], bound_value;
+    __shared__ uint64_t candidates[kCandidates], best_of[kWarps][32];
+    __shared__ uint32_t n_candidates, n_better, warp_count[kWarps];
     const uint32_t row = blockIdx.x / a.n_slices, slice = blockIdx.x % a.n_slices;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const float *x = a.logits + row * a.stride;
     const Extent ext(x, a, slice);
     const float4 *xv = reinterpret_cast<const float4 *>(x + ext.lo + ext.head);
     const uint32_t first = ext.lo + ext.head, single = ext.single();
-    if (threadIdx.x == 0) n_candidates = 0;
+    if (threadIdx.x == 0) n_candidates = 0, n_better = 0;
+    if (threadIdx.x < 32) best_of[0][threadIdx.x] = 0;
     float v[kHeld * 4 + 1];
 #pragma unroll
     for (uint32_t u = 0; u < kHeld; ++u) {
@@ -227,80 +231,137 @@ log_probs_top_kernel(LogProbArgs a) {
     float m = -INFINITY;
 #pragma unroll
     for (uint32_t i = 0; i <= kHeld * 4; ++i) m = fmaxf(m, v[i]);
-    float s = 0.f, t = 0.f;
-    const float base = m > -INFINITY ? m : 0.f;
-    uint32_t which = kHeld * 4;  // the first of the thread's entries that has its best value
+    float top = m;
 #pragma unroll
-    for (int i = kHeld * 4 - 1; i >= 0; --i) {
+    for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (lane % 8 == 0) group_best[warp * 4 + lane / 8] = top;
+    __syncthreads();
+    float key = group_best[lane], m_block = key;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m_block = fmaxf(m_block, __shfl_xor_sync(0xffffffffu, m_block, off));
+    if (warp == 0) {  // ---- the bound: the groups' values in falling order, the n_top-th of them
+#pragma unroll
+        for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+            for (int bit = size / 2; bit > 0; bit /= 2) {
+                const float other = __shfl_xor_sync(0xffffffffu, key, bit);
+                key = ((lane & bit) == 0) == ((lane & size) == 0 || size == 32) ? fmaxf(key, other) : fminf(key, other);
+            }
+        if (lane == a.n_top - 1) bound_value = key;
+    }
+    // ---- sums against the slice's maximum
+    float s = 0.f, t = 0.f;
+    const float base = m_block > -INFINITY ? m_block : 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i <= kHeld * 4; ++i) {
         const float d = floored(v[i] - base), w = ex2(d * kLog2E);
         s += w;
         t = fmaf(d, w, t);
-        if (v[i] == m) which = i;
     }
-    {
-        const float d = floored(v[kHeld * 4] - base), w = ex2(d * kLog2E);
-        s += w;
-        t = fmaf(d, w, t);
-    }
-    uint32_t at = which < kHeld * 4 && there(which) ? index_of(which) : 0xffffffffu;
-    if (v[kHeld * 4] == m) at = min(at, single);  // (the single entry may lie in front of or behind the others; none: no index)
-    // the threads' best entries, sorted: the n_top-th of them is no better than the slice's n_top-th entry
-    uint64_t list = sorted(at != 0xffffffffu ? rank_key(m, at) : 0ull, lane);
-    best_of[warp][lane] = list;
-    share(Stats{m, s, t}, part);
 #pragma unroll
-    for (uint32_t half = kWarps / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (warp < half) {
-            list = merged(list, best_of[warp + half][lane], lane);
-            best_of[warp][lane] = list;
-        }
+    for (int off = 16; off > 0; off >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, off);
+        t += __shfl_xor_sync(0xffffffffu, t, off);
     }
-    if (warp == 0 && lane == a.n_top - 1) bound_key = list;
+    if (lane == 0) part[warp] = make_float2(s, t);
     __syncthreads();
-    const uint64_t bound = bound_key;
-    const float bound_value = bound ? key_value(bound) : -INFINITY;
-    const uint32_t bound_index = bound ? key_index(bound) : 0xffffffffu;
-    auto enters = [&](uint32_t i) { return v[i] >= bound_value && there(i) && (v[i] > bound_value || index_of(i) <= bound_index); };
-    if (m >= bound_value) {
-        uint32_t as_good = 0;  // (most threads have one such entry at most, the one they know)
+    const float bound = bound_value;
+    auto push = [&](uint32_t i) {
+        const uint32_t place = atomicAdd(&n_candidates, 1u);
+        if (place < kCandidates) candidates[place] = rank_key(v[i], index_of(i));
+    };
+    if (m >= bound && bound > -INFINITY) {
 #pragma unroll
-        for (uint32_t i = 0; i <= kHeld * 4; ++i) as_good += v[i] >= bound_value;
-        if (as_good == 1 && at != 0xffffffffu) {
-            if (m > bound_value || at <= bound_index) {
-                const uint32_t place = atomicAdd(&n_candidates, 1u);
-                if (place < kCandidates) candidates[place] = rank_key(m, at);
-            }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i <= kHeld * 4; ++i)
-                if (enters(i)) {
-                    const uint32_t place = atomicAdd(&n_candidates, 1u);
-                    if (place < kCandidates) candidates[place] = rank_key(v[i], index_of(i));
-                }
-        }
+        for (uint32_t i = 0; i <= kHeld * 4; ++i)
+            if (v[i] >= bound) push(i);
     }
     __syncthreads();
-    const uint32_t n = n_candidates;
+    uint32_t n = n_candidates;
     uint64_t best = 0;
-    if (n > kCandidates) {  // too many for the list: every warp sorts its own, then they join
-        for (uint32_t i = 0; i <= kHeld * 4; ++i) {
-            uint64_t key = 0;
-#pragma unroll
-            for (uint32_t e = 0; e <= kHeld * 4; ++e)
-                if (e == i && enters(e)) key = rank_key(v[e], index_of(e));
-            if (__any_sync(0xffffffffu, key != 0)) best = merged(best, sorted(key, lane), lane);
-        }
-        best_of[warp][lane] = best;
+    if (n > kCandidates || bound == -INFINITY) {  // (the same for all threads)
         __syncthreads();
+        if (threadIdx.x == 0) n_candidates = 0;
+        __syncthreads();
+        uint32_t better = 0;
+#pragma unroll
+        for (uint32_t i = 0; i <= kHeld * 4; ++i) {
+            if (v[i] > bound) {
+                push(i);
+                ++better;
+            }
+        }
+        if (better) atomicAdd(&n_better, better);
+        __syncthreads();
+        n = n_better;
+        if (n <= kCandidates) {
+            // entries equal to the bound, in the order of their indices: the single ones in front, the vectors' rounds, the
+            // single ones behind; as many as there are places left
+            uint32_t left = a.n_top > n ? a.n_top - n : 0;
+#pragma unroll
+            for (int round = -1; round <= (int)kHeld; ++round) {
+                if (left == 0) break;
+                const bool lone = round < 0 || round == (int)kHeld;
+                auto equal = [&](uint32_t e) {
+                    const uint32_t i = lone ? kHeld * 4 : 4 * round + e;
+                    return there(i) && v[i] == bound && (!lone || ((threadIdx.x < ext.head) == (round < 0)));
+                };
+                uint32_t count = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < (lone ? 1u : 4u); ++e) count += equal(e);
+                uint32_t before = count;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const uint32_t o = __shfl_up_sync(0xffffffffu, before, off);
+                    if (lane >= (uint32_t)off) before += o;
+                }
+                if (lane == 31) warp_count[warp] = before;
+                __syncthreads();
+                before -= count;
+                uint32_t all = 0;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) {
+                    before += w < warp ? warp_count[w] : 0;
+                    all += warp_count[w];
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < (lone ? 1u : 4u); ++e)
+                    if (equal(e)) {
+                        if (before < left) push(lone ? kHeld * 4 : 4 * round + e);
+                        ++before;
+                    }
+                left -= min(left, all);
+                __syncthreads();
+            }
+            n = min(n_candidates, kCandidates);
+        } else {  // every warp sorts its own, then they join
+            for (uint32_t i = 0; i <= kHeld * 4; ++i) {
+                uint64_t key = 0;
+#pragma unroll
+                for (uint32_t e = 0; e <= kHeld * 4; ++e)
+                    if (e == i && v[e] >= bound && there(e)) key = rank_key(v[e], index_of(e));
+                if (__any_sync(0xffffffffu, key != 0)) best = merged(best, sorted(key, lane), lane);
+            }
+            best_of[warp][lane] = best;
+            __syncthreads();
+            if (warp == 0) {
+                for (uint32_t w = 1; w < kWarps; ++w) best = merged(best, best_of[w][lane], lane);
+                best_of[0][lane] = best;
+            }
+            n = 0;
+        }
     }
+    // ---- a candidate's place is the number of better ones
+    for (uint32_t at = threadIdx.x; at < n; at += kThreads) {
+        const uint64_t key = candidates[at];
+        uint32_t place = 0;
+        for (uint32_t i = 0; i < n; ++i) place += candidates[i] > key;
+        if (place < 32) best_of[0][place] = key;
+    }
+    __syncthreads();
     if (warp != 0) return;
-    if (n > kCandidates) {
-        for (uint32_t w = 1; w < kWarps; ++w) best = merged(best, best_of[w][lane], lane);
-    } else {
-        for (uint32_t i = 0; i < n; i += 32) best = merged(best, sorted(i + lane < n ? candidates[i + lane] : 0ull, lane), lane);
-    }
-    const Stats st = of_block(part);
+    best = best_of[0][lane];
+    Stats st{m_block, 0.f, 0.f};
+    for (uint32_t w = 0; w < kWarps; ++w) st.s += part[w].x, st.t += part[w].y;
     if (a.n_slices == 1) {
         finish(a, row, st, best, lane);
         return;
@@ -329,12 +390,16 @@ log_probs_join_kernel(LogProbArgs a) {
         for (uint32_t i = warp; i < a.n_slices; i += kWarps)
             best = merged(best, a.keys[((size_t)row * a.n_slices + i) * 32 + lane], lane);
         best_of[warp][lane] = best;
+#pragma unroll
+        for (uint32_t half = kWarps / 2; half > 0; half /= 2) {
+            __syncthreads();
+            if (warp < half) best_of[warp][lane] = best = merged(best, best_of[warp + half][lane], lane);
+        }
+    } else {
+        __syncthreads();
     }
-    __syncthreads();
     if (warp != 0) return;
     st = of_block(part);
-    if constexpr (kTop)
-        for (uint32_t w = 1; w < kWarps; ++w) best = merged(best, best_of[w][lane], lane);
     finish(a, row, st, best, lane);
 }
 

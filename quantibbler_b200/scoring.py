@@ -44,10 +44,9 @@ def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
         if not targets.is_contiguous():
             raise KernelError("targets must be contiguous")
     dev, f32 = logits.device, torch.float32
-    # (one allocation for the float outputs: lse, entropy, logprob, top_logprob)
-    flat = torch.empty(n * (3 + top), dtype=f32, device=dev)
-    lse, entropy, logprob = flat[:n], flat[n:2 * n], flat[2 * n:3 * n]
-    top_logprob, top_ids = flat[3 * n:].view(n, top), torch.empty((n, top), dtype=torch.int32, device=dev)
+    lse, entropy, logprob = torch.empty((3, n), dtype=f32, device=dev).unbind(0)
+    top_logprob = torch.empty((n, top), dtype=f32, device=dev)
+    top_ids = torch.empty((n, top), dtype=torch.int32, device=dev)
     lib = _lib.lib()
     if n:
         scratch = workspace(ctx, lib.qk_log_probs_scratch(n, vocab, top), dev)
