@@ -116,6 +116,7 @@ class KvCache:
             if not t.is_contiguous():
                 raise KernelError(f"{what} must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._like = {name: torch.empty(0, dtype=getattr(torch, name), device=k.device) for name in ("float32", "bfloat16")}
         self.n_seq, self.n_kv_heads, self.rows, self.head_dim = (int(n) for n in k.shape)
         self.first_position = int(first_position)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
@@ -191,7 +192,7 @@ class KvCache:
             _, q_stride = self._rows("q", q, None, n)
             heads = q.shape[1]
             if q_out is None:
-                q_out = torch.empty((n, heads, self.head_dim), dtype=torch.float32, device=self.device)
+                q_out = q.new_empty(q.shape)
             _, out_stride = self._rows("q_out", q_out, heads, n)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
@@ -207,20 +208,20 @@ class KvCache:
     def read(self, positions, seq_index, dtype: str = "float32"):
         """The rows of the named tokens as values: k, v ``[tokens, kv heads, head_dim]`` in float32 or bfloat16.
         A row that does not exist reads as zeros and is reported by ``ctx.synchronize()``."""
-        torch = self._torch
         if dtype not in ("float32", "bfloat16"):
             raise KernelError(f"rows are read as float32 or bfloat16, got {dtype!r}")
         n = self._places(positions, seq_index)
-        k, v = torch.empty((2, n, self.n_kv_heads, self.head_dim), dtype=getattr(torch, dtype), device=self.device).unbind(0)
+        shape, like = (n, self.n_kv_heads, self.head_dim), self._like[dtype]
+        k, v = like.new_empty(shape), like.new_empty(shape)
         if n:
             with ordered(self.ctx, self.device):
                 check(_lib.lib().qk_cache_read(self.ctx.handle, self._ref, positions.data_ptr(), seq_index.data_ptr(),
                                                self.first_position, n, _TAGS[dtype], k.data_ptr(), v.data_ptr()))
         return k, v
 
-    def _out(self, out, n: int, heads: int):
+    def _out(self, out, q, n: int, heads: int):
         if out is None:
-            out = self._torch.empty((n, heads, self.head_dim), dtype=self._torch.float32, device=self.device)
+            return q.new_empty(q.shape), heads * self.head_dim
         return out, self._rows("out", out, heads, n)[1]
 
     def _prefix(self, prefix, prefix_len: int, prefix_seq: int):
@@ -245,7 +246,7 @@ class KvCache:
         if not kv_len.is_contiguous():
             raise KernelError("kv_len must be contiguous")
         ref = self._prefix(prefix, prefix_len, prefix_seq)
-        out, out_stride = self._out(out, n, heads)
+        out, out_stride = self._out(out, q, n, heads)
         lib = _lib.lib()
         if n:
             scratch = workspace(self.ctx, lib.qk_cache_attend_scratch(self._ref, prefix_len, n, heads), self.device)
@@ -267,7 +268,7 @@ class KvCache:
                               f"{self.first_position}")
         ref = self._prefix(prefix, prefix_len, prefix_seq)
         row = first_position - self.first_position
-        out, out_stride = self._out(out, n, heads)
+        out, out_stride = self._out(out, q, n, heads)
         lib = _lib.lib()
         if n:
             scratch = workspace(self.ctx, lib.qk_cache_portion_scratch(self._ref, row, prefix_len, n, heads),

@@ -6,9 +6,10 @@
 // the i-th best; lists are sorted and merged by bitonic networks across the warp.
 //
 // What bounds it: the logits' bytes.  A row is cut into slices where there are fewer rows than blocks fit the
-// device; a second kernel joins the slices of a row.
+// device; up to sixteen slices are the blocks of a cluster, which joins them, more are joined by a second kernel.
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 
 #include "qk_common.h"
 
@@ -19,6 +20,7 @@ constexpr uint32_t kMinSlice = 2048;   // entries a block takes at least
 constexpr uint32_t kHeld = 8;          // vectors of four entries that a thread keeps in registers
 constexpr uint32_t kCandidates = 512;  // places for entries that may be among the best of a slice
 constexpr uint32_t kWantBlocks = 148 * 8;
+constexpr size_t kResident = 148 * 2, kMaxCluster = 16, kMaxSlice = 16384;  // (longer slices than that are for more blocks than a cluster has)
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct LogProbArgs {
@@ -28,8 +30,9 @@ struct LogProbArgs {
     const int32_t *targets;
     float *lse, *logprob, *entropy, *top_logprob;
     int32_t *top_ids;
-    float *stats;    // [n_tokens][n_slices][4]: m, S, T; where n_slices > 1
-    uint64_t *keys;  // [n_tokens][n_slices][32]; where also n_top > 0
+    uint32_t clustered;  // the slices of a row are the blocks of a cluster, which join them; else a second launch does:
+    float *stats;        // [n_tokens][n_slices][4]: m, S, T
+    uint64_t *keys;      // [n_tokens][n_slices][32]; where n_top > 0
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -126,6 +129,62 @@ __device__ __forceinline__ Stats of_block(const Stats *part) {
     return st;
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A shared-memory address of this block in the cluster's block `rank`.
+__device__ __forceinline__ uint32_t of_rank(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float load_float(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint64_t load_key(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(addr));
+    return v;
+}
+// The blocks of a cluster are the slices of a row: the first one joins their statistics and best entries (`best`, in
+// lanes; kTop) through distributed shared memory.  All threads; st and best are those of the first warp.
+template <bool kTop>
+__device__ __forceinline__ void join_cluster(const LogProbArgs &a, uint32_t row, uint32_t slice, Stats st, uint64_t best,
+                                             Stats *shared_stats, uint64_t (*lists)[32]) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 0) {
+        if (lane == 0) *shared_stats = st;
+        if constexpr (kTop) lists[0][lane] = best;
+    }
+    cluster_sync();
+    if (slice == 0) {
+        st = Stats{-INFINITY, 0.f, 0.f};
+        if (warp == 0 && lane < a.n_slices) {
+            const uint32_t from = of_rank(shared_stats, lane);
+            st = Stats{load_float(from), load_float(from + 4), load_float(from + 8)};
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1)  // (every lane needs them)
+            st = joined(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, off), __shfl_xor_sync(0xffffffffu, st.s, off),
+                                  __shfl_xor_sync(0xffffffffu, st.t, off)});
+        best = 0;
+        if constexpr (kTop) {
+            for (uint32_t i = warp; i < a.n_slices; i += kWarps)
+                best = merged(best, load_key(of_rank(&lists[0][lane], i)), lane);
+#pragma unroll
+            for (uint32_t half = kWarps / 2; half > 0; half /= 2) {
+                if (warp >= half && warp < 2 * half) lists[warp][lane] = best;
+                __syncthreads();
+                if (warp < half) best = merged(best, lists[warp + half][lane], lane);
+            }
+        }
+        if (warp == 0) finish(a, row, st, best, lane);
+    }
+    cluster_sync();  // (no block ends while the first one reads it)
+}
+
 // Where a slice's 16-byte vectors lie: up to three single entries in front, up to three behind.
 struct Extent {
     uint32_t lo, hi, head, vectors, tail;
@@ -188,6 +247,11 @@ log_probs_kernel(LogProbArgs a) {
     if (single != 0xffffffffu) take(x[single], -INFINITY, -INFINITY, -INFINITY);
     share(Stats{m, s, t}, part);
     __syncthreads();
+    if (a.clustered) {
+        __shared__ Stats shared_stats;
+        join_cluster<false>(a, row, slice, of_block(part), 0, &shared_stats, nullptr);
+        return;
+    }
     if (threadIdx.x >= 32) return;
     const Stats st = of_block(part);
     if (a.n_slices == 1) finish(a, row, st, 0, threadIdx.x);
@@ -358,10 +422,16 @@ log_probs_top_kernel(LogProbArgs a) {
         if (place < 32) best_of[0][place] = key;
     }
     __syncthreads();
-    if (warp != 0) return;
+    if (warp != 0 && !a.clustered) return;
     best = best_of[0][lane];
     Stats st{m_block, 0.f, 0.f};
     for (uint32_t w = 0; w < kWarps; ++w) st.s += part[w].x, st.t += part[w].y;
+    if (a.clustered) {
+        __shared__ Stats shared_stats;
+        __syncthreads();
+        join_cluster<true>(a, row, slice, st, best, &shared_stats, best_of);
+        return;
+    }
     if (a.n_slices == 1) {
         finish(a, row, st, best, lane);
         return;
@@ -403,13 +473,19 @@ log_probs_join_kernel(LogProbArgs a) {
     finish(a, row, st, best, lane);
 }
 
-// How many slices a row is cut into, and their length (a multiple of four entries).
-void slices(size_t n_tokens, size_t vocab, size_t n_top, uint32_t *n, uint32_t *length) {
+// How many slices a row is cut into, their length (a multiple of four entries), and whether a cluster joins them: while
+// all blocks are resident at once.  (1 x 32768, 5 places: 24 -> 19 us a call.  Where blocks queue, clusters make them wait
+// for one another: 64 x 128256, 20 places, 18 -> 30 us.)
+bool slices(size_t n_tokens, size_t vocab, size_t n_top, uint32_t *n, uint32_t *length) {
+    const size_t held = n_top ? kThreads * kHeld * 4 : SIZE_MAX;  // (what stays in registers)
     const size_t most = qk::ceil_div(vocab, kMinSlice), want = std::max<size_t>(1, kWantBlocks / std::max<size_t>(1, n_tokens));
-    size_t len = (qk::ceil_div(vocab, std::min(most, want)) + 3) / 4 * 4;
-    if (n_top) len = std::min<size_t>(len, kThreads * kHeld * 4);  // (what stays in registers)
+    size_t count = std::min(most, want);
+    if (count > kMaxCluster && n_tokens * kMaxCluster <= kResident && qk::ceil_div(vocab, kMaxCluster) <= std::min(held, kMaxSlice))
+        count = kMaxCluster;
+    const size_t len = std::min((qk::ceil_div(vocab, count) + 3) / 4 * 4, held);
     *length = (uint32_t)len;
     *n = (uint32_t)qk::ceil_div(vocab, len);
+    return *n > 1 && *n <= kMaxCluster && n_tokens * *n <= kResident;
 }
 
 }  // namespace
@@ -419,8 +495,8 @@ extern "C" {
 size_t qk_log_probs_scratch(size_t n_tokens, size_t vocab, size_t n_top) {
     if (!n_tokens || !vocab) return 0;
     uint32_t n, length;
-    slices(n_tokens, vocab, n_top, &n, &length);
-    return n == 1 ? 0 : n_tokens * n * (16 + (n_top ? 256 : 0));
+    const bool clustered = slices(n_tokens, vocab, n_top, &n, &length);
+    return n == 1 || clustered ? 0 : n_tokens * n * (16 + (n_top ? 256 : 0));
 }
 
 qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t vocab, size_t stride,
@@ -446,18 +522,19 @@ qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t
     LogProbArgs a{};
     a.logits = logits, a.stride = stride, a.n_tokens = (uint32_t)n_tokens, a.vocab = (uint32_t)vocab, a.n_top = (uint32_t)n_top;
     a.targets = targets, a.lse = lse, a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob, a.top_ids = top_ids;
-    slices(n_tokens, vocab, n_top, &a.n_slices, &a.slice);
+    a.clustered = slices(n_tokens, vocab, n_top, &a.n_slices, &a.slice);
     a.keys = static_cast<uint64_t *>(scratch);
     a.stats = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + (n_top ? n_tokens * a.n_slices * 256 : 0));
-    auto go = [&](auto kernel, unsigned blocks) -> qk_status {
-        (void)qk::launch_pdl(c->pdl, kernel, dim3(blocks), dim3(kThreads), 0, c->stream, a);
+    auto go = [&](auto kernel, unsigned blocks, unsigned cluster) -> qk_status {
+        if (cluster > 8) QK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        (void)qk::launch_pdl_cluster(c->pdl, kernel, dim3(blocks), dim3(kThreads), cluster, 0, c->stream, a);
         QK_CUDA(cudaGetLastError());
         c->launches++;
         return QK_OK;
     };
-    st = go(n_top ? log_probs_top_kernel : log_probs_kernel, (unsigned)(n_tokens * a.n_slices));
-    if (st != QK_OK || a.n_slices == 1) return st;
-    return go(n_top ? log_probs_join_kernel<true> : log_probs_join_kernel<false>, (unsigned)n_tokens);
+    st = go(n_top ? log_probs_top_kernel : log_probs_kernel, (unsigned)(n_tokens * a.n_slices), a.clustered ? a.n_slices : 1);
+    if (st != QK_OK || a.n_slices == 1 || a.clustered) return st;
+    return go(n_top ? log_probs_join_kernel<true> : log_probs_join_kernel<false>, (unsigned)n_tokens, 1);
 }
 
 }  // extern "C"

@@ -29,23 +29,24 @@ def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
     -infinity, gives NaN (its ids: -1); entries of -infinity are impossible ones.  Runs on the context's stream,
     ordered with torch's current one."""
     import torch
-    if logits.dim() != 2:
-        raise KernelError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
-    if logits.device.type != "cuda" or logits.device.index != ctx.device_index:
-        raise KernelError(f"logits are on {logits.device}, the context on cuda:{ctx.device_index}")
-    check_tensor("logits", logits, torch.float32, logits.device)
-    n, vocab = (int(v) for v in logits.shape)
+    shape, dev = logits.shape, logits.device
+    if len(shape) != 2:
+        raise KernelError(f"logits must be [rows, vocab], got {tuple(shape)}")
+    if dev.type != "cuda" or dev.index != ctx.device_index:
+        raise KernelError(f"logits are on {dev}, the context on cuda:{ctx.device_index}")
+    if logits.dtype is not torch.float32:
+        check_tensor("logits", logits, torch.float32, dev)
+    n, vocab = shape
     if logits.stride(1) != 1 and vocab > 1:
         raise KernelError(f"a row of logits must be contiguous, got strides {logits.stride()}")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise KernelError(f"top must lie in 0 .. {min(MAX_TOP, vocab)}, got {top}")
     if targets is not None:
-        check_tensor("targets", targets, torch.int32, logits.device, (n,))
+        check_tensor("targets", targets, torch.int32, dev, (n,))
         if not targets.is_contiguous():
             raise KernelError("targets must be contiguous")
-    dev, f32 = logits.device, torch.float32
-    lse, entropy, logprob = torch.empty((3, n), dtype=f32, device=dev).unbind(0)
-    top_logprob = torch.empty((n, top), dtype=f32, device=dev)
+    lse, entropy, logprob = logits.new_empty((3, n)).unbind(0)
+    top_logprob = logits.new_empty((n, top))
     top_ids = torch.empty((n, top), dtype=torch.int32, device=dev)
     lib = _lib.lib()
     if n:

@@ -101,7 +101,7 @@ PREFIXES = [
 def test_attend(change, text):
     change = dict(change)
     if change.pop("wide", False):   # a shape whose keys are split over blocks
-        refused(attend(cache(rows=5000, d=128), q_stride=512, out_stride=512, **change), text)
+        refused(attend(cache(rows=200_000, d=128), q_stride=512, out_stride=512, **change), text)
     else:
         refused(attend(cache(), **change), text)
 
