@@ -34,8 +34,10 @@ def _joined(torch, handle, current):
     stream = torch.cuda.ExternalStream(handle, device=current.device) if handle > 2 else \
         torch.cuda.default_stream(current.device)
     stream.wait_stream(current)
-    yield
-    current.wait_stream(stream)
+    try:
+        yield
+    finally:
+        current.wait_stream(stream)
 
 
 _alone = contextlib.nullcontext()
@@ -59,14 +61,14 @@ def ordered(ctx: GpuContext, device):
 
 
 def workspace(ctx: GpuContext, size: int, device):
-    """Device memory of ``size`` bytes for one call on ``ctx``: the context's own, grown and kept (calls on a context
-    follow one another on its stream), but inside a stream capture a tensor of the graph's."""
+    """Device memory of ``size`` bytes for one call on ``ctx``: the context's own for its stream, grown and kept (calls
+    follow one another there), but inside a stream capture a tensor of the graph's."""
     import torch
     if not size:
         return None
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(size, dtype=torch.uint8, device=device)
-    kept = ctx.workspaces    # (the ones outgrown stay: work in flight may use them)
+    kept = ctx.workspaces.setdefault(ctx.stream_handle, [])    # (the ones outgrown stay: work in flight may use them)
     if not kept or kept[-1].numel() < size:
         with _growing:
             if not kept or kept[-1].numel() < size:

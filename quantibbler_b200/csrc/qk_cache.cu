@@ -650,6 +650,9 @@ bool takes_rows(const qk_kv_cache *c) { return c->dtype != QK_F32 && (c->head_di
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned_rows(const CacheView &v) { return aligned(v.k) && aligned(v.v); }
 
+// Tokens of one launch of append, whose blocks each look through those after their own; a later launch's writes come last
+// by the stream's order.  65536 INT8 tokens of 8 heads of 128: 990 us in one launch, 452 by 16384, 398 by 8192, 404 by 4096.
+constexpr size_t kAppendTokens = 8192;
 constexpr size_t kWantBlocks = 148 * 8, kMinChunk = 256, kResident = 148 * 2;
 
 // The tile kernel takes 128 query rows to an SM: how often the keys (64 to a block, two blocks at a time) are split so
@@ -842,26 +845,31 @@ qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q,
     const int groups = mask % 16 || (uintptr_t)cos_sin % 16 ? 0 : d == 64 ? 1 : d == 128 ? 2 : d == 256 ? 4 : 0;
 #define QK_APPEND_ARGS                                                                                                    \
     cv, q, q_stride, q_out, q_out_stride, (uint32_t)n_heads, k, k_stride, v, v_stride, cos_sin, (uint32_t)n_positions, positions, \
-        seq_index, (uint32_t)first_position, (uint32_t)n_tokens
+        seq_index, (uint32_t)first_position, (uint32_t)n
 #define QK_APPEND_WIDE(KV, N) QK_PDL(c, (append_wide_kernel<KV, N>), wide, dim3(128), 0, QK_APPEND_ARGS, wide_kv, err)
 #define QK_APPEND(KV)                                                                                        \
     do {                                                                                                     \
         if (groups == 1) QK_APPEND_WIDE(KV, 1);                                                              \
         else if (groups == 2) QK_APPEND_WIDE(KV, 2);                                                         \
         else if (groups == 4) QK_APPEND_WIDE(KV, 4);                                                         \
-        else QK_PDL(c, append_kernel<KV>, dim3((unsigned)n_tokens), dim3(256), 0, QK_APPEND_ARGS, err);      \
+        else QK_PDL(c, append_kernel<KV>, dim3((unsigned)n), dim3(256), 0, QK_APPEND_ARGS, err);      \
     } while (0)
     const uint32_t wide_kv = (uint32_t)qk::ceil_div(2 * cache->n_kv_heads, 16);
-    const dim3 wide((unsigned)n_tokens, wide_kv + (unsigned)(q ? qk::ceil_div(n_heads, 16) : 0));
-    if (cv.dtype == QK_I8) QK_APPEND(int8_t);
-    else if (cv.dtype == QK_BF16) QK_APPEND(uint16_t);
-    else QK_APPEND(float);
+    for (size_t done = 0; done < n_tokens; done += kAppendTokens) {
+        const size_t n = std::min(kAppendTokens, n_tokens - done);
+        const dim3 wide((unsigned)n, wide_kv + (unsigned)(q ? qk::ceil_div(n_heads, 16) : 0));
+        if (cv.dtype == QK_I8) QK_APPEND(int8_t);
+        else if (cv.dtype == QK_BF16) QK_APPEND(uint16_t);
+        else QK_APPEND(float);
+        QK_CUDA(cudaGetLastError());
+        c->launches++;
+        c->err_armed = true;
+        if (q) q += n * q_stride, q_out += n * q_out_stride;
+        k += n * k_stride, v += n * v_stride, positions += n, seq_index += n;
+    }
 #undef QK_APPEND_WIDE
 #undef QK_APPEND_ARGS
 #undef QK_APPEND
-    QK_CUDA(cudaGetLastError());
-    c->launches++;
-    c->err_armed = true;
     return QK_OK;
 }
 

@@ -11,7 +11,8 @@
 //
 // Exactness.  INT8 rows: codes as float16 are exact (three warps convert them on their way into shared memory); q is
 // two float16 terms after scaling by a power of two per row (22 bits), and so are the weights times the value scales,
-// which are taken relative to a power of two at their running maximum E and scaled to 2^14.  bfloat16 rows go in as
+// which are taken relative to a power of two at their running maximum E and scaled to 2^14 (in blocks that some row does
+// not see whole, at the row's own maximum).  bfloat16 rows go in as
 // they are; q and the weights are three bfloat16 terms.  A block's product with v starts from zero and is added to the
 // row's output in registers, in float32: the tensor core truncates.
 //
@@ -41,6 +42,7 @@ constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kSms = 148;
+constexpr uint32_t kEdges = 4;  // causal: the blocks that some row of a tile does not see whole are among the last four
 
 template <bool kI8, int D>
 struct TileShape {
@@ -51,7 +53,7 @@ struct TileShape {
     static constexpr uint32_t kStages = kI8 || D == 64 ? 4 : 3;        // of the keys' ring, and of the values'
     static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a block's key and value scales, and E
     static constexpr uint32_t kRingBytes = 2 * kStages * kTileBytes;
-    static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 384;
+    static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 512;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
     // Tensor memory.  INT8: q's terms (the A operand of the scores, so that shared memory is not read for them in every
     // block), a unit's scores, over which its weights lie (16 columns of scores become eight of either term), its
@@ -155,6 +157,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *never = reinterpret_cast<volatile int *>(tmem_slot + 2);
+    uint32_t *spoilt = tmem_slot + 3;  // [block from the last][2]: keys with an infinity or NaN among their values
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t kvh = blockIdx.x % c.n_kv, tile = gridDim.x / c.n_kv - 1 - blockIdx.x / c.n_kv, split = blockIdx.y;
     const uint32_t group = a.n_heads / c.n_kv, n_rows = a.n_queries * group;
@@ -180,6 +183,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         mbar_init(drain, 1);
         *abort_flag = 0;
         *never = 0;
+        for (uint32_t i = 0; i < 2 * kEdges; ++i) spoilt[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -195,6 +199,9 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     const uint32_t tmem = *tmem_slot;
     const size_t line0 = (a.seq * c.n_kv + kvh) * (size_t)c.rows + (size_t)block0 * kKeys;  // first key's row
     const uint32_t keys = n_blocks ? min(n_keys - block0 * kKeys, n_blocks * kKeys) : 0;    // of this CTA
+    // keys that every row of the tile sees: the blocks past them (at the end) are edges
+    const int seen0 = min((int)keys, a.causal ? (int)(a.first_row + row0 / group) + 1 - (int)(block0 * kKeys) : (int)keys);
+    auto at_edge = [&](uint32_t g) { return (int)((g + 1) * kKeys) > seen0; };
 
     if (warp >= kKeyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -251,6 +258,26 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     hand_over(fulls + s);
                 }
             } else {
+                // Values that some rows of the tile do not see: an infinity or NaN times their weight, zero, would reach them
+                // all the same.  It becomes zero, and its key is noted for the rows that do see it.  (A thread looks at what it
+                // copied itself.)
+                auto clean = [&](uint32_t g) {
+                    const uint32_t from_last = n_blocks - 1 - g;
+                    if (!is_v || !a.causal || from_last >= kEdges) return;
+                    uint8_t *tile_at = tiles + g % kStages * S::kTileBytes + piece / 8 * S::kChunkBytes;
+#pragma unroll 1
+                    for (uint32_t row = first; row < kKeys; row += kStep) {
+                        uint32_t *w = reinterpret_cast<uint32_t *>(tile_at + row * 128 + (((piece % 8) ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+                            if (lo || hi) {
+                                w[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+                                atomicOr(spoilt + 2 * from_last + row / 32, 1u << (row % 32));
+                            }
+                        }
+                    }
+                };
                 for (uint32_t g = 0; g < n_blocks; ++g) {
                     const uint32_t s = g % kStages;
                     ok = mbar_wait(empties + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
@@ -269,11 +296,15 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (g) {  // (a block is handed over when the next one is under way)
                         asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        clean(g - 1);
                         hand_over(fulls + (g - 1) % kStages);
                     }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
-                if (ok && n_blocks) hand_over(fulls + (n_blocks - 1) % kStages);
+                if (ok && n_blocks) {
+                    clean(n_blocks - 1);
+                    hand_over(fulls + (n_blocks - 1) % kStages);
+                }
             }
             if (!ok) *abort_flag = 1;
         } else if (warp == kScaleWarp) {
@@ -287,7 +318,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                                                                   (size_t)(kvh2 * group + which % group) * D + i % (D / 32) * 32));
                 }
             }
-            // ---- INT8: the scales, those of the values relative to the running maximum's power of two
+            // ---- INT8: the scales, those of the values relative to the running maximum's power of two; at an edge, where the
+            // maximum is a row's own affair, as they are
             if constexpr (kI8) {
                 float sc[4];  // key and value scales of keys lane, lane + 32 of the next block
                 auto load = [&](uint32_t g) {
@@ -305,12 +337,12 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     const uint32_t top = __reduce_max_sync(0xffffffffu,
                                                            max(__float_as_uint(fabsf(sc[2])), __float_as_uint(fabsf(sc[3]))));
                     e_max = max(e_max, exponent_of(top));
-                    const float mul = pow2(-1 - e_max);
+                    const float mul = at_edge(g) ? 1.f : pow2(-1 - e_max) * kWeightScale;
                     ok = mbar_wait(v_empty + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
                     if (!ok) break;
                     float *dst = scales + s * S::kScaleFloats;
                     dst[lane] = sc[0], dst[32 + lane] = sc[1];
-                    dst[kKeys + lane] = sc[2] * mul * kWeightScale, dst[kKeys + 32 + lane] = sc[3] * mul * kWeightScale;
+                    dst[kKeys + lane] = sc[2] * mul, dst[kKeys + 32 + lane] = sc[3] * mul;
                     if (lane == 0) reinterpret_cast<int *>(dst)[2 * kKeys] = e_max;
                     load(g + 1);
                     __syncwarp();
@@ -448,10 +480,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         const float f = row_factor[r];
         const uint32_t cols = tmem + S::score_col(u) + (((warp % 4) * 32) << 16);  // scores and weights
         const uint32_t outs = tmem + S::out_col(u) + (((warp % 4) * 32) << 16);
-        // keys of this CTA that this row sees, and its tile's first row
-        const int base_key = (int)(block0 * kKeys);
-        const int seen = a.causal ? (int)(a.first_row + query) + 1 - base_key : (int)keys;
-        const int seen0 = a.causal ? (int)(a.first_row + row0 / group) + 1 - base_key : (int)keys;
+        // keys of this CTA that this row sees
+        const int seen = a.causal ? (int)(a.first_row + query) + 1 - (int)(block0 * kKeys) : (int)keys;
         float m = -INFINITY, l = 0.f;
         int e_here = -100;
         float o[D];
@@ -486,10 +516,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             ok = ok && mbar_wait(s_full + u, it & 1, abort_flag, a.wait_limit);
             if (!ok) break;  // (a warp at a time: the others' waits end with the flag below)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const bool edge = key0 + (int)kKeys > min(seen0, (int)keys);  // some row of the tile does not see the whole block
-            const int limit = min(seen, (int)keys) - key0;                // keys of the block that this row sees
+            const int limit = min(seen, (int)keys) - key0;  // keys of the block that this row sees
             const float *ks = scales + (g % kStages) * S::kScaleFloats, *vs = ks + kKeys;
             float alpha_new;
+            int e_new = -100;
             float2 sum = make_float2(0.f, 0.f);
             // (kEdge in the type: a select per score would be paid in every block)
             auto weights = [&](auto edge_tag) {
@@ -527,6 +557,20 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 m = m_new;
                 if (it) take_output(it - 1);
                 if (!ok) return;
+                float mul = 1.f;
+                if constexpr (kI8 && kEdge) {  // (a scale that this row does not see must not push its own out of float16's range)
+                    float most = 0.f;
+#pragma unroll 4
+                    for (int at = 0; at < (int)kKeys; at += 4) {
+                        const float4 v4 = *reinterpret_cast<const float4 *>(vs + at);
+                        most = fmaxf(most, fmaxf(fmaxf(at < limit ? fabsf(v4.x) : 0.f, at + 1 < limit ? fabsf(v4.y) : 0.f),
+                                                 fmaxf(at + 2 < limit ? fabsf(v4.z) : 0.f, at + 3 < limit ? fabsf(v4.w) : 0.f)));
+                    }
+                    e_new = max(e_here, exponent_of(__float_as_uint(most)));
+                    mul = pow2(-1 - e_new) * kWeightScale;
+                } else if constexpr (kI8) {
+                    e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
+                }
                 const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
 #pragma unroll
                 for (int part = 0; part < 4; ++part) {
@@ -546,7 +590,9 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         x = make_float2(ex2(x.x), ex2(x.y));
                         sum = __fadd2_rn(sum, x);
                         if constexpr (kI8) {
-                            x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(vs + at));
+                            float2 v2 = *reinterpret_cast<const float2 *>(vs + at);
+                            if constexpr (kEdge) v2 = __fmul2_rn(v2, make_float2(mul, mul));
+                            x = __fmul2_rn(x, v2);
                             if constexpr (kEdge) {  // (a key that this row does not see may have the scale NaN)
                                 x.x = at < limit ? x.x : 0.f;
                                 x.y = at + 1 < limit ? x.y : 0.f;
@@ -561,13 +607,12 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(cols + S::weight_col(n, part), t[n]);
                 }
             };
-            if (edge) weights(std::true_type{});
+            if (at_edge(g)) weights(std::true_type{});
             else weights(std::false_type{});
             if (!ok) break;
             l = fmaf(l, alpha_new, sum.x + sum.y);
             alpha = alpha_new;
             if constexpr (kI8) {
-                const int e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
                 alpha *= pow2(max(-126, e_here - e_new));
                 e_here = e_new;
             }
@@ -577,6 +622,33 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             if (lane == 0) mbar_arrive(p_full + u);
         }
         if (ok && it) take_output(it - 1);
+        if constexpr (!kI8) {  // infinities and NaNs that the loaders took out, to the rows that see their keys
+#pragma unroll 1
+            for (uint32_t e = 0; ok && a.causal && e < min(kEdges, n_blocks); ++e) {
+                const uint32_t g = n_blocks - 1 - e;
+                if (g % 2 != u) continue;  // (the other unit's block)
+#pragma unroll 1
+                for (uint32_t half = 0; half < 2; ++half) {
+                    uint32_t marked = spoilt[2 * e + half];
+#pragma unroll 1
+                    for (; marked; marked &= marked - 1) {
+                        const uint32_t key = g * kKeys + 32 * half + __ffs(marked) - 1;
+                        if ((int)key >= seen) break;
+                        const uint4 *v = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(c.v) + (line0 + key) * (2 * D));
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) {
+                            const uint4 w = __ldg(v + i);
+                            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if ((x[j] & 0x7f80u) == 0x7f80u) o[8 * i + 2 * j] += __uint_as_float(x[j] << 16);
+                                if ((x[j] & 0x7f800000u) == 0x7f800000u) o[8 * i + 2 * j + 1] += __uint_as_float(x[j] & 0xffff0000u);
+                            }
+                        }
+                    }
+                }
+            }
+        }
         if (!ok) *abort_flag = 1;
         // ---- the units join: each finishes half of the channels and hands the others over, through the ring (every
         // product has been read out, every block consumed once both units are here)

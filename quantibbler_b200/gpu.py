@@ -58,7 +58,7 @@ class GpuContext:
         self._h = handle
         self.device_index = int(device_index)
         self._stream_handle = None   # (known once asked for; set_stream is the only way to change it)
-        self.workspaces = []         # device memory of eager calls (cache.workspace)
+        self.workspaces = {}         # stream -> device memory of eager calls (cache.workspace)
 
     @classmethod
     def init_at(cls, device_index: int) -> "GpuContext":
@@ -107,8 +107,10 @@ class GpuContext:
             handle = 0
         else:
             handle = int(cuda_stream) or 1
-        self._stream_handle = None
-        check(_lib.lib().qk_gpu_set_stream(self._h, ctypes.c_void_p(handle)))
+        try:
+            check(_lib.lib().qk_gpu_set_stream(self._h, ctypes.c_void_p(handle)))
+        finally:
+            self._stream_handle = None
 
     def container_to_rows(self, stream, n_rows: int, r: int, transposed: bool = False) -> np.ndarray:
         """The container repack of engine/mod.rs:258-289 run by the device's kernels (the ones

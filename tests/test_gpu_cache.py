@@ -144,9 +144,83 @@ def test_portion(gpu_ctx, dtype, d, heads, kv, tokens, first, prefix):
         near(got[t], want, bound)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (8, 2)])
+@pytest.mark.parametrize("tokens,first,at", [(200, 100, 150), (200, 100, 299), (130, 0, 127), (40, 4000, 4020), (5, 60, 63)])
+@pytest.mark.parametrize("spoilt", ["nan", "inf", "1e30"])
+def test_a_portion_s_own_rows_stay_behind_their_token(gpu_ctx, dtype, d, heads, kv, tokens, first, at, spoilt):
+    """An infinity, NaN or very large value in the rows of one token of a portion: tokens before it do not see it, it and
+    those after do."""
+    g = gen(tokens + at)
+    c, (k, v) = make(gpu_ctx, g, dtype, 1, kv, first + tokens, d)
+    q = randn(g, tokens, heads, d)
+    value = float(spoilt)
+    if dtype == "int8":
+        c.v_scale[0, 0, at] = value
+        v[0, 0, at] = c.v[0, 0, at].double() * value
+        places = torch.arange(d, device="cuda")
+    else:
+        places = torch.tensor([5, d - 2], device="cuda")
+        c.v[0, 0, at, places] = value
+        v[0, 0, at, places] = c.v[0, 0, at, places].double()
+    got = c.portion(q, 0, first)
+    gpu_ctx.synchronize()
+    group = heads // kv
+    for t in range(tokens):
+        n = first + t + 1
+        want, bound = attention64(q[t], k[0, :, :n], v[0, :, :n])
+        here = got[t]
+        if n > at and spoilt != "1e30":
+            lost = torch.isnan(want[:group, places]) | torch.isinf(want[:group, places])
+            assert not torch.isfinite(here[:group, places][lost]).any()
+            clean = v.clone()
+            clean[0, 0, at, places] = 0.0
+            want, bound = attention64(q[t], k[0, :, :n], clean[0, :, :n])
+            here = here.clone()
+            here[:group, places] = want[:group, places].float()
+        near(here, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+def test_the_last_slot_of_more_than_4_gb(gpu_ctx, dtype):
+    """Appending to, reading and attending a slot whose rows lie behind 2^32 values."""
+    from quantibbler_b200.cache import KvCache
+    n_seq, kv, rows, d, heads = 9, 8, 500_000, 128, 32
+    c = KvCache.empty(gpu_ctx, n_seq, kv, rows, d, dtype)
+    g = gen(8)
+    tokens, n = 300, rows
+    cs = table(rows, d)
+    q, k, v = (randn(g, tokens, h, d) for h in (heads, kv, kv))
+    pos = torch.arange(rows - tokens, rows, device="cuda", dtype=torch.int32)
+    slots = torch.full_like(pos, n_seq - 1)
+    q = c.append(k, v, cs, pos, slots, q=q)
+    k_back, v_back = c.read(pos, slots)
+    for want, back in ((rotated64(k, cs[pos.long()]), k_back), (v.double(), v_back)):
+        # (half a code, or half a bfloat16 step, of the row's largest; its scale's rounding)
+        step = want.abs().amax(-1, keepdim=True) * (0.5 / 127 * (1 + 2.0 ** -12) if dtype == "int8" else 2.0 ** -8)
+        assert ((back.double() - want).abs() <= step).all()
+    assert not c.v[:n_seq - 1, :, -tokens:].any()
+    # (all rows before the appended ones are zeros: scores of 0)
+    got = c.portion(q, n_seq - 1, rows - tokens)
+    lens = torch.tensor([0] * (n_seq - 1) + [rows], dtype=torch.int32, device="cuda")
+    step_got = c.attend(q[-1:].expand(n_seq, heads, d).contiguous(), lens)
+    gpu_ctx.synchronize()
+    kd, vd = c.k[-1].double(), c.v[-1].double()
+    if dtype == "int8":
+        kd, vd = kd * c.k_scale[-1].double()[..., None], vd * c.v_scale[-1].double()[..., None]
+    for t in (0, 128, tokens - 1):
+        n = rows - tokens + t + 1
+        for h in (0, 7):
+            want, bound = attention64(q[t, 4 * h:4 * h + 4], kd[h:h + 1, :n], vd[h:h + 1, :n])
+            near(got[t, 4 * h:4 * h + 4], want, bound)
+            if t == tokens - 1:
+                near(step_got[-1, 4 * h:4 * h + 4], want, bound)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
 def test_attend_over_a_long_cache(gpu_ctx, dtype):
-    """Rows beyond 2^31 bytes of the first, and more than the kernels' splits hold evenly."""
+    """More rows than the kernels' splits hold evenly."""
     g = gen(3)
     rows, kv, d = 300_017, 8, 128
     c, (k, v) = make(gpu_ctx, g, dtype, 2, kv, rows, d, spread=False)
@@ -364,6 +438,28 @@ def test_the_last_token_of_a_row_stays(gpu_ctx, dtype):
     gpu_ctx.synchronize()
     for a, b in ((c.k, one.k), (c.v, one.v), (c.k_scale, one.k_scale), (c.v_scale, one.v_scale)):
         assert a is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("d", [16, 128])
+def test_a_long_append_with_rows_named_again(gpu_ctx, dtype, d):
+    """More tokens than one launch takes: the last token of a row stays, wherever the launches part."""
+    from quantibbler_b200.cache import KvCache
+    g = gen(10)
+    n, rows = 20_001, 9_000
+    k, v, q = randn(g, n, 2, d), randn(g, n, 2, d), randn(g, n, 2, d)
+    positions = torch.randint(0, rows, (n,), device="cuda", generator=g, dtype=torch.int32)
+    seq = torch.zeros_like(positions)
+    cs = table(rows, d)
+    c, one = (KvCache.empty(gpu_ctx, 1, 2, rows, d, dtype=dtype) for _ in range(2))
+    turned = c.append(k, v, cs, positions, seq, q=q)
+    last = torch.full((rows,), -1, device="cuda").scatter_reduce(0, positions.long(), torch.arange(n, device="cuda"), "amax")
+    last = last[last >= 0]
+    one.append(k[last], v[last], cs, positions[last].contiguous(), seq[last].contiguous())
+    gpu_ctx.synchronize()
+    for a, b in ((c.k, one.k), (c.v, one.v), (c.k_scale, one.k_scale), (c.v_scale, one.v_scale)):
+        assert a is None or torch.equal(a, b)
+    assert (turned.double() - rotated64(q, cs[positions.long()])).abs().max() <= 2.0 ** -22 * q.abs().max()
 
 
 def test_tokens_outside_the_cache_are_skipped_and_reported(gpu_ctx):

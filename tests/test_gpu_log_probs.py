@@ -74,6 +74,17 @@ def test_orders_and_ties(gpu_ctx, vocab):
     check(gpu_ctx, x, targets, 32, log_probs(gpu_ctx, x, targets, 32))
 
 
+@pytest.mark.parametrize("top", [0, 3])
+def test_rows_behind_4_gb_of_logits(gpu_ctx, top):
+    from quantibbler_b200.scoring import log_probs
+    n, vocab = 40_000, 110_001
+    x = torch.zeros(n, vocab, device="cuda")
+    x[-3:] = torch.randn(3, vocab, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    targets = torch.full((n,), 7, device="cuda", dtype=torch.int32)
+    got = log_probs(gpu_ctx, x, targets, top)
+    check(gpu_ctx, x[-3:], targets[-3:], top, type(got)(*(None if t is None else t[-3:] for t in got)))
+
+
 def test_masked_and_spoiled_rows(gpu_ctx):
     from quantibbler_b200.scoring import log_probs
     vocab = 3001
