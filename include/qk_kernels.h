@@ -834,15 +834,17 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
  * prefix_len rows of slot prefix_seq of `prefix`, which are read once for all sequences.  The two caches agree
  * in dtype, kv heads and head_dim; `prefix` may be the same cache.  A sequence that sees no row gets zeros.
  * q [batch][n_heads][head_dim] (already rotated) and out, batch rows q_stride and out_stride values apart.
- * scratch: qk_cache_attend_scratch bytes, nothing kept in it between calls; calls that may overlap on the
- * device need one each.  head_dim up to 256; head_dim 64 and 128 with 16-byte aligned rows run on the tensor
+ * out may be q itself, but may not overlap it otherwise.
+ * scratch: qk_cache_attend_scratch bytes on a 16-byte boundary (null where that is 0), nothing kept in it between
+ * calls; calls that may overlap on the device need one each.  head_dim up to 256; head_dim 64 and 128 with 16-byte aligned rows run on the tensor
  * cores (all but float32 caches), others take a plain kernel. */
 qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, size_t prefix_seq,
                           size_t prefix_len, const float *q, size_t q_stride, const int32_t *kv_len, size_t batch,
                           size_t n_heads, void *scratch, float *out, size_t out_stride);
 size_t qk_cache_attend_scratch(const qk_kv_cache *cache, size_t prefix_len, size_t batch, size_t n_heads);
 /* The same for n_tokens consecutive tokens of one sequence whose rows first_row .. first_row + n_tokens - 1 have
- * been appended: token t sees rows 0 .. first_row + t of slot seq, and the prefix. */
+ * been appended: token t sees rows 0 .. first_row + t of slot seq, and the prefix.  What the rows of later tokens
+ * hold, infinities and NaNs too, does not reach it. */
 qk_status qk_cache_portion(qk_ctx *ctx, const qk_kv_cache *cache, size_t seq, size_t first_row, const qk_kv_cache *prefix,
                            size_t prefix_seq, size_t prefix_len, const float *q, size_t q_stride, size_t n_tokens,
                            size_t n_heads, void *scratch, float *out, size_t out_stride);
@@ -855,7 +857,7 @@ size_t qk_cache_portion_scratch(const qk_kv_cache *cache, size_t first_row, size
  * -infinity has probability 0 and adds nothing to the entropy.  A row whose largest entry is -infinity or
  * +infinity, or that holds a NaN, gives NaN throughout (its top_ids: -1).  targets may be null (no logprob);
  * a negative target marks a row without a token: its logprob is 0; a target >= vocab gives NaN.  Any output
- * may be null.  scratch: qk_log_probs_scratch bytes, nothing kept in it between calls. */
+ * may be null.  scratch: qk_log_probs_scratch bytes on a 16-byte boundary, nothing kept in it between calls. */
 qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t vocab, size_t stride,
                        const int32_t *targets, size_t n_top, void *scratch, float *lse, float *logprob, float *entropy,
                        float *top_logprob, int32_t *top_ids);

@@ -241,7 +241,7 @@ class KvCache:
         """softmax(q k^T / sqrt(head_dim)) v with one query per sequence: ``q`` ``[batch, heads, head_dim]``
         (rotated), sequence b sees the first ``kv_len[b]`` rows of slot b (int32, on the device) and the first
         ``prefix_len`` rows of slot ``prefix_seq`` of ``prefix``, a cache of the same kind.  A sequence that sees
-        nothing gets zeros.  Returns ``out`` (default: a new tensor)."""
+        nothing gets zeros.  Returns ``out`` (default: a new tensor; ``q`` itself is allowed)."""
         n, q_stride = self._rows("q", q, None)
         heads = q.shape[1]
         check_tensor("kv_len", kv_len, self._i32, self.device, (n,))

@@ -1072,10 +1072,12 @@ class Decoder(SlotDecoder):
         if self.prefix_len:
             self.positions.clamp_(min=self.prefix_len)
             self.kv_len.clamp_(min=1)
-        super().capture()
-        self.positions.copy_(saved[0])
-        self.kv_len.copy_(saved[1])
-        self.torch.cuda.synchronize()
+        try:
+            super().capture()
+        finally:
+            self.positions.copy_(saved[0])
+            self.kv_len.copy_(saved[1])
+            self.torch.cuda.synchronize()
 
     def start(self, token_ids, positions) -> None:
         if self.prefix_len and len(positions) and min(int(p) for p in positions) < self.prefix_len:

@@ -312,6 +312,24 @@ def test_rows_that_lie_apart_or_off_16_bytes(gpu_ctx, dtype, d):
         near(far[b], want, bound)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "int8"])
+@pytest.mark.parametrize("prefix", [0, 70, 9000])
+def test_out_in_the_place_of_q(gpu_ctx, dtype, prefix):
+    """The same bits as into a tensor of its own, from one launch or several."""
+    g = gen(11)
+    c, _ = make(gpu_ctx, g, dtype, 20, 2, 500, 64, first_position=prefix)
+    p, _ = make(gpu_ctx, g, dtype, 1, 2, max(prefix, 1), 64)
+    shared = dict(prefix=p, prefix_len=prefix) if prefix else {}
+    lens = torch.randint(0, 501, (20,), device="cuda", generator=g, dtype=torch.int32)
+    for n, call in ((1, lambda q, out: c.attend(q, lens[:1], out=out, **shared)),
+                    (20, lambda q, out: c.attend(q, lens, out=out, **shared)),
+                    (150, lambda q, out: c.portion(q, 3, prefix + 300, out=out, **shared))):
+        q = randn(g, n, 40, 64)
+        want = call(q, None)
+        assert torch.equal(call(q, q), want)
+    gpu_ctx.synchronize()
+
+
 # ---------------------------------------------------------------------- appending and reading
 def rotated64(x, cs):
     a, b = x.double().chunk(2, -1)
