@@ -37,7 +37,6 @@ constexpr uint32_t kThreads = 512, kLoaders = 96, kKeyWarp = 8, kValueWarp = 11,
 constexpr int kUnitRegs = 184, kOtherRegs = 72, kLaunchRegs = 128;
 static_assert(256 * kUnitRegs + 256 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kAhead = 2;  // a block's scores are formed when the product of the unit's block before is under way
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;
 constexpr uint32_t kWaitLimit = 1u << 22;
@@ -59,9 +58,8 @@ struct TileShape {
     // block), a unit's scores, over which its weights lie (16 columns of scores become eight of either term), its
     // outputs.  bfloat16, whose terms are three, has q in shared memory and the first two terms of the weights behind
     // the scores, the third over scores that have been read.
-    static constexpr bool kQInTmem = kI8;
-    __device__ static constexpr uint32_t q_col(uint32_t term) { return 64 * term; }
-    __device__ static constexpr uint32_t score_col(uint32_t u) { return kI8 ? 128 + 64 * u : 256 * u; }
+    static constexpr uint32_t kAhead = kI8 ? 4 : 2;  // blocks whose scores are formed ahead: block g's lie in place g % kAhead
+    __device__ static constexpr uint32_t score_col(uint32_t at) { return (kI8 ? 64 : 256) * at; }
     __device__ static constexpr uint32_t out_col(uint32_t u) { return kI8 ? 256 + 128 * u : 256 * u + 128; }
     __device__ static constexpr uint32_t weight_col(uint32_t term, uint32_t step) {  // of a step of 16 keys, from score_col
         return kI8 ? 16 * step + 8 * term : (term == 2 ? 0 : 64 + 32 * term) + 8 * step;
@@ -142,7 +140,7 @@ template <bool kI8, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tile_kernel(CacheView c, TileArgs a) {
     using S = TileShape<kI8, D>;
-    constexpr uint32_t kTerms = S::kTerms, kChunks = S::kChunks, kStages = S::kStages;
+    constexpr uint32_t kTerms = S::kTerms, kChunks = S::kChunks, kStages = S::kStages, kAhead = S::kAhead;
     qk::pdl_launch();
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *qs = raw_smem + (-smem_u32(raw_smem) & 1023u);  // (an offset: the compiler still sees shared memory)
@@ -152,7 +150,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     float *row_factor = scales + kStages * S::kScaleFloats;                     // [128]
     uint64_t *q_full = reinterpret_cast<uint64_t *>(row_factor + 128);
     uint64_t *k_full = q_full + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages, *v_empty = v_full + kStages;
-    uint64_t *s_full = v_empty + kStages, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint64_t *s_full = v_empty + kStages, *p_full = s_full + kAhead, *o_full = p_full + 2;
     uint64_t *drain = o_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -175,8 +173,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             mbar_init(v_full + s, kLoaders / 32 + (kI8 ? 1 : 0));
             mbar_init(v_empty + s, 1);
         }
+        for (uint32_t i = 0; i < kAhead; ++i) mbar_init(s_full + i, 1);
         for (int u = 0; u < 2; ++u) {
-            mbar_init(s_full + u, 1);
             mbar_init(p_full + u, 4);
             mbar_init(o_full + u, 1);
         }
@@ -359,24 +357,21 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const uint64_t v_desc = umma_desc(smem_u32(v_ring)) | ((uint64_t)(S::kChunkBytes >> 4) << 16);
             auto scores = [&](uint32_t g) {  // (one lane) small terms first
                 const uint64_t kd = k_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
-                const uint32_t dst = tmem + S::score_col(g & 1);
+                const uint32_t dst = tmem + S::score_col(g % kAhead);
 #pragma unroll
                 for (uint32_t i = 0; i < kTerms; ++i)
 #pragma unroll
                     for (uint32_t k = 0; k < 4 * kChunks; ++k) {
                         const uint64_t kk = kd + ((k / 4 * S::kChunkBytes + k % 4 * 32) >> 4);
-                        if constexpr (S::kQInTmem)
-                            mma_ts(dst, tmem + S::q_col(kTerms - 1 - i) + 8 * k, kk, idesc_s, i + k != 0);
-                        else
-                            mma_ss(dst, q_desc + (((kTerms - 1 - i) * S::kQTermBytes + k / 4 * S::kQChunkBytes + k % 4 * 32) >> 4),
-                                   kk, idesc_s, i + k != 0);
+                        mma_ss(dst, q_desc + (((kTerms - 1 - i) * S::kQTermBytes + k / 4 * S::kQChunkBytes + k % 4 * 32) >> 4), kk,
+                               idesc_s, i + k != 0);
                     }
                 umma_commit(k_empty + g % kStages);
-                umma_commit(s_full + (g & 1));
+                umma_commit(s_full + g % kAhead);
             };
             auto values = [&](uint32_t g) {  // (one lane)
                 const uint64_t vd = v_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
-                const uint32_t weights = tmem + S::score_col(g & 1), dst = tmem + S::out_col(g & 1);
+                const uint32_t weights = tmem + S::score_col(g % kAhead), dst = tmem + S::out_col(g & 1);
 #pragma unroll
                 for (uint32_t i = 0; i < kTerms; ++i)
 #pragma unroll
@@ -454,31 +449,12 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 for (uint32_t n = 0; n < kTerms; ++n) *reinterpret_cast<uint2 *>(to + n * S::kQTermBytes) = make_uint2(t0[n], t1[n]);
                 if (lane % kLanes == 0) row_factor[at] = factor;
             }
-            if constexpr (!S::kQInTmem) {
-                fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
-            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
             asm volatile("bar.sync 3, 256;" ::: "memory");
-            if constexpr (S::kQInTmem) {  // a unit takes one term, a thread its row
-                static_assert(kTerms == 2, "a term for each unit");
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * kChunks; ++i) {  // sixteen channels: eight columns
-                    uint32_t w[8];
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h)
-                        *reinterpret_cast<uint4 *>(w + 4 * h) = *reinterpret_cast<const uint4 *>(
-                            qs + u * S::kQTermBytes + i / 4 * S::kQChunkBytes + r * 128 + (((2 * (i % 4) + h) ^ (r & 7)) << 4));
-                    tmem_st8(tmem + S::q_col(u) + 8 * i + (((warp % 4) * 32) << 16), w);
-                }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
-            }
         }
         const float f = row_factor[r];
-        const uint32_t cols = tmem + S::score_col(u) + (((warp % 4) * 32) << 16);  // scores and weights
         const uint32_t outs = tmem + S::out_col(u) + (((warp % 4) * 32) << 16);
         // keys of this CTA that this row sees
         const int seen = a.causal ? (int)(a.first_row + query) + 1 - (int)(block0 * kKeys) : (int)keys;
@@ -511,9 +487,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         uint32_t it = 0;
         for (uint32_t g = u; g < n_blocks; g += 2, ++it) {
             const int key0 = (int)(g * kKeys);
+            const uint32_t cols = tmem + S::score_col(g % kAhead) + (((warp % 4) * 32) << 16);  // scores and weights
             // (the scales come with the values, most often before the scores)
             if (kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
-            ok = ok && mbar_wait(s_full + u, it & 1, abort_flag, a.wait_limit);
+            ok = ok && mbar_wait(s_full + g % kAhead, (g / kAhead) & 1, abort_flag, a.wait_limit);
             if (!ok) break;  // (a warp at a time: the others' waits end with the flag below)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int limit = min(seen, (int)keys) - key0;  // keys of the block that this row sees
