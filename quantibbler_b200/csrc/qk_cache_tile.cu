@@ -133,6 +133,37 @@ __device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint3
     hi = __byte_perm(u, 0x64646464u, 0x4342);
     asm("{\n .reg .b32 c;\n mov.b32 c, 0x64806480;\n sub.rn.f16x2 %0, %0, c;\n sub.rn.f16x2 %1, %1, c;\n}" : "+r"(lo), "+r"(hi));
 }
+// Waits for the loads of tensor memory, v's the last of them (which nothing may use before).
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                   "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+// n times sixteen columns of tensor memory to use(i, values), each load under way while the values before are used.
+template <int kN, typename Use>
+__device__ __forceinline__ void each16(uint32_t taddr, Use use) {
+    uint32_t v[2][16];
+    tmem_ld16(taddr, v[0]);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        tmem_ld_wait(v[i % 2]);
+        if (i + 1 < kN) tmem_ld16(taddr + 16 * (i + 1), v[(i + 1) % 2]);
+        use(i, v[i % 2]);
+    }
+}
+// Whether both barriers have completed their phases: the usual case of two waits, for the price of one.
+__device__ __forceinline__ bool both_ready(uint64_t *bar1, uint32_t parity1, uint64_t *bar2, uint32_t parity2) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p, q;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n and.pred p, p, q;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_u32(bar1)), "r"(parity1), "r"(smem_u32(bar2)), "r"(parity2)
+        : "memory");
+    return __all_sync(0xffffffffu, done) != 0;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Grid (kv heads x tiles of 128 rows, splits of the keys); late tiles see most keys: they go first.
@@ -470,18 +501,14 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             ok = mbar_wait(o_full + u, done & 1, abort_flag, a.wait_limit);
             if (!ok) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            each16<D / 16>(outs, [&](int part, const uint32_t (&w)[16]) {
 #pragma unroll
-            for (int part = 0; part < D / 32; ++part) {
-                uint32_t w[32];
-                tmem_ld32(outs + 32 * part, w);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = __ffma2_rn(make_float2(o[32 * part + i], o[32 * part + i + 1]), make_float2(alpha, alpha),
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 x = __ffma2_rn(make_float2(o[16 * part + i], o[16 * part + i + 1]), make_float2(alpha, alpha),
                                                 make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])));
-                    o[32 * part + i] = x.x, o[32 * part + i + 1] = x.y;
+                    o[16 * part + i] = x.x, o[16 * part + i + 1] = x.y;
                 }
-            }
+            });
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         };
         uint32_t it = 0;
@@ -489,8 +516,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const int key0 = (int)(g * kKeys);
             const uint32_t cols = tmem + S::score_col(g % kAhead) + (((warp % 4) * 32) << 16);  // scores and weights
             // (the scales come with the values, most often before the scores)
-            if (kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
-            ok = ok && mbar_wait(s_full + g % kAhead, (g / kAhead) & 1, abort_flag, a.wait_limit);
+            if (!kI8 || !both_ready(v_full + g % kStages, (g / kStages) & 1, s_full + g % kAhead, (g / kAhead) & 1)) {
+                if (kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                ok = ok && mbar_wait(s_full + g % kAhead, (g / kAhead) & 1, abort_flag, a.wait_limit);
+            }
             if (!ok) break;  // (a warp at a time: the others' waits end with the flag below)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int limit = min(seen, (int)keys) - key0;  // keys of the block that this row sees
@@ -501,33 +530,29 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             // (kEdge in the type: a select per score would be paid in every block)
             auto weights = [&](auto edge_tag) {
                 constexpr bool kEdge = decltype(edge_tag)::value;
-                float top = -INFINITY;
+                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                each16<kKeys / 16>(cols, [&](int part, const uint32_t (&s)[16]) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    uint32_t s[32];
-                    tmem_ld32(cols + 32 * part, s);
-                    tmem_ld_wait();
-                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
+                    for (int e = 0; e < 16; e += 4) {
+                        const int at = 16 * part + e;
                         float4 x = make_float4(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]),
                                                __uint_as_float(s[e + 3]));
                         if constexpr (kI8) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * part + e);
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + at);
                             const float2 lo = __fmul2_rn(make_float2(x.x, x.y), make_float2(k4.x, k4.y));
                             const float2 hi = __fmul2_rn(make_float2(x.z, x.w), make_float2(k4.z, k4.w));
                             x = make_float4(lo.x, lo.y, hi.x, hi.y);
                         }
                         if constexpr (kEdge) {
-                            x.x = 32 * part + e < limit ? x.x : -INFINITY;
-                            x.y = 32 * part + e + 1 < limit ? x.y : -INFINITY;
-                            x.z = 32 * part + e + 2 < limit ? x.z : -INFINITY;
-                            x.w = 32 * part + e + 3 < limit ? x.w : -INFINITY;
+                            x.x = at < limit ? x.x : -INFINITY;
+                            x.y = at + 1 < limit ? x.y : -INFINITY;
+                            x.z = at + 2 < limit ? x.z : -INFINITY;
+                            x.w = at + 3 < limit ? x.w : -INFINITY;
                         }
                         t4[0] = fmaxf(t4[0], x.x), t4[1] = fmaxf(t4[1], x.y), t4[2] = fmaxf(t4[2], x.z), t4[3] = fmaxf(t4[3], x.w);
                     }
-                    top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
-                }
+                });
+                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                 const float m_new = fmaxf(m, top * f);
                 const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
                 alpha_new = ex2(m - base);
@@ -549,11 +574,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
                 }
                 const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
-#pragma unroll
-                for (int part = 0; part < 4; ++part) {
-                    uint32_t s[16], t[kTerms][8];
-                    tmem_ld16(cols + 16 * part, s);
-                    tmem_ld_wait();
+                each16<kKeys / 16>(cols, [&](int part, const uint32_t (&s)[16]) {
+                    uint32_t t[kTerms][8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
@@ -582,7 +604,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     }
 #pragma unroll
                     for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(cols + S::weight_col(n, part), t[n]);
-                }
+                });
             };
             if (at_edge(g)) weights(std::true_type{});
             else weights(std::false_type{});
