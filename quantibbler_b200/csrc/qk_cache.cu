@@ -133,7 +133,8 @@ append_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t
 
 // Head sizes 64 kGroups on 16-byte boundaries: eight lanes to a row, four rows to a warp at once (what a row
 // costs beside its entries - the reductions, the division that gives the scale - is paid once for four), kGroups vectors
-// of four pairs a lane.  2048 tokens, 32 / 8 heads of 128: 26 us with a row to a warp, most of it issue.
+// of four pairs a lane.  2048 tokens, 32 / 8 heads of 128: 20 us, 4.4 TB/s (issue and the latency of one round of loads a
+// block; 26 us with a row to a warp, most of it issue).
 template <typename KV, int kGroups>
 __global__ void __launch_bounds__(128, kGroups == 4 ? 4 : 8)
 append_wide_kernel(CacheView c, const float *q, size_t q_stride, float *q_out, size_t q_out_stride, uint32_t n_heads,
@@ -300,7 +301,8 @@ template <> __device__ __forceinline__ float value_at<int8_t>(const int8_t *p, s
     return (float)p[i] * scale;
 }
 
-// A warp per row.  kVec: head sizes of whole groups of four values per lane, on 16-byte boundaries.
+// A warp per row.  kVec: head sizes of whole groups of four values per lane, on 16-byte boundaries.  2048 INT8 tokens of 8
+// heads of 128 as float32: 6.6 us, 3.2 TB/s (one round of loads a warp).
 template <typename KV, typename Out, bool kVec>
 __global__ void __launch_bounds__(256)
 read_kernel(CacheView c, const int32_t *__restrict__ positions, const int32_t *__restrict__ seq_index, uint32_t first_position,
@@ -667,7 +669,7 @@ size_t tiles_of(const qk_kv_cache *c, size_t queries, size_t n_heads) {
 // Whether the query rows on a prefix go eight at a time through attend_rows_kernel, or 128 at a time through the tile
 // kernel.  A block of the former costs the same for one row as for eight, 16 keys of a kv head about 0.7 ns of the whole
 // device; one of the latter costs 64 keys 9 ns whatever its rows, and the launch 10 us more.  Eight sequences of four rows
-// behind 4001 INT8 rows: 21 against 25 us; 64 of them behind 8192 bfloat16 rows: 131 against 49.
+// behind 4001 INT8 rows: 21 against 25 us; 64 of them behind 8192 bfloat16 rows: 131 against 50.
 bool prefix_by_rows(const qk_kv_cache *c, size_t rows, size_t prefix_len) {
     return rows <= 16 || qk::ceil_div(rows, 8) * prefix_len * c->n_kv_heads <= (1u << 18);
 }

@@ -4,10 +4,10 @@
 // The queries that read one kv head are the rows of one product: row r is query r / group, head r % group of the kv
 // head, 128 rows to a CTA, which takes a range of keys 64 at a time.  Two units of four warps take the key blocks in
 // turn, a thread owns a row (no shuffles): running maximum, sum and output in registers, the two units joined at the
-// end.  While one unit is at its exponentials the tensor core works for the other; a block's output is read out when
-// the maximum of the unit's next block is known.  The weights go back to tensor
-// memory as the A operand; v is read as it lies (MN-major B).  Three warps bring the
-// key blocks in, three the value blocks.
+// end.  While one unit is at its exponentials the tensor core works for the other; INT8 scores are formed four blocks
+// ahead, and a block's output is read out when the maximum of the unit's next block is known.  The weights go back to
+// tensor memory, over their scores, as the A operand; v is read as it lies (MN-major B).  Three warps bring the key blocks
+// in, three the value blocks.
 //
 // Exactness.  INT8 rows: codes as float16 are exact (three warps convert them on their way into shared memory); q is
 // two float16 terms after scaling by a power of two per row (22 bits), and so are the weights times the value scales,
@@ -16,7 +16,13 @@
 // they are; q and the weights are three bfloat16 terms.  A block's product with v starts from zero and is added to the
 // row's output in registers, in float32: the tensor core truncates.
 //
-// What bounds it: shared memory (the tensor core reads q anew for every block) and the instructions per score.
+// What bounds it: a unit's chain for a block of 64 keys, 4200 cycles (waits 500, maxima 850, the output's turn 850,
+// exponentials, weights and their terms 1900), of which two run side by side, and 16000 cycles of a CTA before its first
+// block (q) and behind its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 99 us, 0.35
+// PFLOP/s of the formula's operations, 0.69 of the tensor core's (29 % of its cycles).  64 x 32 / 8 heads behind 8192
+// bfloat16 rows: 35 us.  Slower, us for the INT8 portion: INT8 q in tensor memory with scores two blocks ahead (110), q's
+// loads in front of the barriers' setup (101.6), rows written out by bulk copies (99.9).  bfloat16: 200 registers a
+// thread for the units (+ 1.4), scores three blocks ahead (+ 0.4).
 #include <cuda_fp16.h>
 
 #include <algorithm>
