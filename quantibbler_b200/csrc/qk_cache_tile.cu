@@ -60,10 +60,9 @@ struct TileShape {
     static constexpr uint32_t kRingBytes = 2 * kStages * kTileBytes;
     static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 512;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
-    // Tensor memory.  INT8: q's terms (the A operand of the scores, so that shared memory is not read for them in every
-    // block), a unit's scores, over which its weights lie (16 columns of scores become eight of either term), its
-    // outputs.  bfloat16, whose terms are three, has q in shared memory and the first two terms of the weights behind
-    // the scores, the third over scores that have been read.
+    // Tensor memory.  INT8: the scores of four blocks, over which their weights lie (16 columns of scores become eight of
+    // either term), the units' outputs.  bfloat16, whose terms are three: a unit's scores, behind them the first two terms
+    // of its weights, the third over scores that have been read, its output.
     static constexpr uint32_t kAhead = kI8 ? 4 : 2;  // blocks whose scores are formed ahead: block g's lie in place g % kAhead
     __device__ static constexpr uint32_t score_col(uint32_t at) { return (kI8 ? 64 : 256) * at; }
     __device__ static constexpr uint32_t out_col(uint32_t u) { return kI8 ? 256 + 128 * u : 256 * u + 128; }

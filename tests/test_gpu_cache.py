@@ -744,6 +744,28 @@ def test_decoder_behind_a_shared_prefix(gpu_ctx, kv_dtype, graph):
             call()
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_greedy_decode_behind_a_prefix(gpu_ctx, graph):
+    """set_prefix, advance, decode: every slot goes on greedily (a token's logit is as near the largest as the logits
+    are to the reference's)."""
+    from quantibbler_b200.decoder import Decoder
+    cfg, weights = small(kv_dtype="float32", max_prefix=20)
+    dec = Decoder(gpu_ctx, cfg, weights)
+    prefix = np.random.default_rng(5).integers(0, cfg.vocab, 17).tolist()
+    dec.set_prefix(prefix)
+    if graph:
+        dec.capture()
+    first = dec.best_idx.cpu().numpy().copy()
+    dec.advance()
+    ids = dec.decode(3)
+    assert (ids == ids[:, :1]).all() and (first == first[0]).all()
+    tokens = prefix + [int(first[0])] + ids[:, 0].tolist()
+    want = reference_logits(cfg, weights, tokens[:-1])
+    scale = np.abs(want).max()
+    for i in range(len(prefix), len(tokens)):
+        assert want[i - 1].max() - want[i - 1][tokens[i]] <= 2 * TOL["float32"] * scale
+
+
 @pytest.mark.parametrize("kv_dtype", ["bfloat16", "int8"])
 def test_prompts_behind_a_prefix_and_a_second_prefix(gpu_ctx, kv_dtype):
     """Prompts of unequal length in portions behind a prefix; then another prefix with the same decoder."""
