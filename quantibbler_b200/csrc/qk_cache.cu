@@ -667,12 +667,19 @@ size_t tiles_of(const qk_kv_cache *c, size_t queries, size_t n_heads) {
     return qk::ceil_div(queries * (n_heads / c->n_kv_heads), 128) * c->n_kv_heads;
 }
 // Whether the query rows on a prefix go eight at a time through attend_rows_kernel, or 128 at a time through the tile
-// kernel.  A block of the former costs the same for one row as for eight, 16 keys of a kv head about 0.7 ns of the whole
-// device; one of the latter costs 64 keys 9 ns whatever its rows, and the launch 10 us more.  Eight sequences of four rows
-// behind 4001 INT8 rows: 21 against 25 us; 64 of them behind 8192 bfloat16 rows: 131 against 50.
+// kernel.  A block of the former costs the same for one row as for eight; one of the latter whatever its rows, and 10 us
+// are spent before its first keys and behind its last.  Heads 32 / 8 of 128, by rows against by tiles, us: 8 sequences
+// behind 6000 INT8 rows 22.7, 28.2; 12 behind 4000 22.1, 22.2; 16 behind 4000 29.1, 22.3; behind bfloat16 rows 16 and 1500
+// 18.5, 19.3; 24 and 1300 22.0, 19.5; 40 and 800 25.5, 19.9.
 bool prefix_by_rows(const qk_kv_cache *c, size_t rows, size_t prefix_len) {
-    return rows <= 16 || qk::ceil_div(rows, 8) * prefix_len * c->n_kv_heads <= (1u << 18);
+    return rows <= 16 || qk::ceil_div(rows, 8) * prefix_len * c->n_kv_heads <= (c->dtype == QK_I8 ? 12u << 14 : 7u << 14);
 }
+
+// The most query rows that a block of the call has, and how many blocks of the kernel for it an SM holds.
+uint32_t most_rows(const Plan &pl, bool prefix, size_t prefix_rows) {
+    return prefix ? std::max(pl.own_rows, (uint32_t)std::min<size_t>(8, prefix_rows)) : pl.own_rows;
+}
+size_t blocks_an_sm(const qk_kv_cache *c, uint32_t rows) { return (c->dtype == QK_I8 ? 4 : 3) - (rows > 4); }
 
 Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_heads) {
     Plan pl{};
@@ -686,6 +693,14 @@ Plan plan_rows(const qk_kv_cache *c, size_t prefix_len, size_t batch, size_t n_h
     pl.prefix_subs = (uint32_t)qk::ceil_div(batch * group, 8);
     const size_t own_blocks = batch * c->n_kv_heads * pl.own_subs, pre_blocks = by_rows ? pl.prefix_subs * c->n_kv_heads : 0;
     size_t own = splits(own_blocks, c->rows), pre = by_rows ? splits(pre_blocks, prefix_len) : 1;
+    // Fewer splits where all blocks then fit the device at once and last no longer than two rounds would.  Eight sequences
+    // behind 4001 INT8 rows: 19.5 -> 15.1 us; 14 of 2048 INT8 rows: 19.5 -> 17.4, 10 of bfloat16 22.8 -> 19.1.
+    const size_t slots = 148 * blocks_an_sm(c, most_rows(pl, by_rows, batch * group));
+    if (own_blocks * own + pre_blocks * pre > slots) {
+        const size_t fit = by_rows ? (slots - std::min(slots, own_blocks * own)) / pre_blocks : slots / own_blocks;
+        size_t &cut = by_rows ? pre : own;
+        if (2 * fit > cut) cut = fit;
+    }
     // While all blocks are resident at once, the splits are the blocks of a cluster (up to 32 of them become eight), and
     // there is no second launch: one sequence of 2048 INT8 rows, 32 heads: 14 -> 11.6 us a call on the host, the device's
     // time the same.  Where blocks queue, clusters make them wait for one another: 64 sequences 42 -> 47 us.
@@ -764,8 +779,9 @@ qk_status launch_rows(qk_ctx *c, const CacheView &own, const CacheView &pre, con
         qk_status st = prefix_tiles(c, pre, a, pl.prefix_slots, pl.n_slots);
         if (st != QK_OK) return st;
     }
-    const uint32_t rows = pl.prefix_blocks ? std::max(pl.own_rows, std::min(8u, a.n_queries * (a.n_heads / own.n_kv))) : pl.own_rows;
-    return rows > 4 ? launch_rows<kI8, D, 2>(c, own, pre, a, pl) : launch_rows<kI8, D, 1>(c, own, pre, a, pl);
+    return most_rows(pl, pl.prefix_blocks != 0, (size_t)a.n_queries * (a.n_heads / own.n_kv)) > 4
+               ? launch_rows<kI8, D, 2>(c, own, pre, a, pl)
+               : launch_rows<kI8, D, 1>(c, own, pre, a, pl);
 }
 
 qk_status attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, const qk::AttendArgs &a) {

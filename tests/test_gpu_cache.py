@@ -123,6 +123,29 @@ def test_attend_behind_a_prefix(gpu_ctx, dtype, d, heads, kv, batch, prefix):
         near(got[b], want, bound)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv,batch", [(8, 2, 6), (8, 2, 33), (32, 8, 40), (40, 2, 20)])
+@pytest.mark.parametrize("prefix", [4097, 6000])
+def test_attend_behind_a_long_prefix(gpu_ctx, dtype, d, heads, kv, batch, prefix):
+    """By eight rows a block in several splits, and by 128 rows."""
+    g = gen(prefix + heads)
+    c, (k, v) = make(gpu_ctx, g, dtype, batch, kv, 70, d, first_position=prefix)
+    p, (pk, pv) = make(gpu_ctx, g, dtype, 2, kv, prefix + 3, d)
+    lens = torch.randint(0, 71, (batch,), device="cuda", generator=g, dtype=torch.int32)
+    for b in range(batch):
+        spoil(c, b, int(lens[b]))
+    spoil(p, 1, prefix)
+    q = randn(g, batch, heads, d)
+    got = c.attend(q, lens, prefix=p, prefix_len=prefix, prefix_seq=1)
+    gpu_ctx.synchronize()
+    for b in range(batch):
+        n = int(lens[b])
+        want, bound = attention64(q[b], torch.cat([pk[1, :, :prefix], k[b, :, :n]], 1),
+                                  torch.cat([pv[1, :, :prefix], v[b, :, :n]], 1))
+        near(got[b], want, bound)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "int8"])
 @pytest.mark.parametrize("d", [16, 64, 128, 256])
 @pytest.mark.parametrize("heads,kv", [(4, 4), (8, 2), (6, 2), (18, 1)])
