@@ -20,7 +20,7 @@
 // exponentials, weights and their terms 1900), of which two run side by side, and 16000 cycles of a CTA before its first
 // block (q) and behind its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 99 us, 0.35
 // PFLOP/s of the formula's operations, 0.69 of the tensor core's (29 % of its cycles).  64 x 32 / 8 heads behind 8192
-// bfloat16 rows: 35 us.  Slower, us for the INT8 portion: INT8 q in tensor memory with scores two blocks ahead (110), q's
+// bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion: INT8 q in tensor memory with scores two blocks ahead (110), q's
 // loads in front of the barriers' setup (101.6), rows written out by bulk copies (99.9).  bfloat16: 200 registers a
 // thread for the units (+ 1.4), scores three blocks ahead (+ 0.4).
 #include <cuda_fp16.h>
