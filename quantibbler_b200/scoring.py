@@ -45,9 +45,9 @@ def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
         check_tensor("targets", targets, torch.int32, dev, (n,))
         if not targets.is_contiguous():
             raise KernelError("targets must be contiguous")
-    lse, entropy, logprob = logits.new_empty((3, n)).unbind(0)
-    top_logprob = logits.new_empty((n, top))
-    top_ids = torch.empty((n, top), dtype=torch.int32, device=dev)
+    new = logits.new_empty    # (cheaper than views of one tensor)
+    lse, entropy, logprob, top_logprob = new(n), new(n), None if targets is None else new(n), new((n, top))
+    top_ids = torch.empty((n, top), dtype=torch.int32, device=dev) if targets is None else targets.new_empty((n, top))
     lib = _lib.lib()
     if n:
         scratch = workspace(ctx, lib.qk_log_probs_scratch(n, vocab, top), dev)
@@ -55,6 +55,6 @@ def log_probs(ctx: GpuContext, logits, targets=None, top: int = 0) -> LogProbs:
             check(lib.qk_log_probs(ctx.handle, logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab,
                                    None if targets is None else targets.data_ptr(), top,
                                    None if scratch is None else scratch.data_ptr(), lse.data_ptr(),
-                                   None if targets is None else logprob.data_ptr(), entropy.data_ptr(),
+                                   None if logprob is None else logprob.data_ptr(), entropy.data_ptr(),
                                    top_logprob.data_ptr() if top else None, top_ids.data_ptr() if top else None))
-    return LogProbs(lse, None if targets is None else logprob, entropy, top_logprob, top_ids)
+    return LogProbs(lse, logprob, entropy, top_logprob, top_ids)
