@@ -336,6 +336,38 @@ def test_rows_that_lie_apart_or_off_16_bytes(gpu_ctx, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 50, 9000])
+@pytest.mark.parametrize("value", [NAN, float("inf"), 3e38])
+def test_a_query_of_infinities_stays_alone(gpu_ctx, dtype, d, prefix, value):
+    """One head's query holds an infinity, a NaN or a value whose scores overflow: the other heads of its kv head and the
+    other queries keep their results; lengths outside the cache are clamped."""
+    g = gen(12)
+    c, (k, v) = make(gpu_ctx, g, dtype, 30, 2, 90, d, first_position=prefix)
+    p, (pk, pv) = make(gpu_ctx, g, dtype, 1, 2, max(prefix, 1), d)
+    shared = dict(prefix=p, prefix_len=prefix) if prefix else {}
+    lens = [90] * 28 + [1_000_000, -7]
+    for n in (30, 75):
+        q = randn(g, n, 10, d)
+        q[3, 2, 5], q[20, 9, d - 1] = value, -value
+        if n == 30:
+            got = c.attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"), **shared)
+        else:
+            got = c.portion(q, 4, prefix + 15, **shared)
+        gpu_ctx.synchronize()
+        for t in range(n):
+            b, rows = (t, max(0, min(90, lens[t]))) if n == 30 else (4, 15 + t + 1)
+            want, bound = attention64(q[t], torch.cat([pk[0, :, :prefix], k[b, :, :rows]], 1),
+                                      torch.cat([pv[0, :, :prefix], v[b, :, :rows]], 1))
+            clean = torch.ones(10, dtype=torch.bool, device="cuda")
+            if t in (3, 20):
+                clean[2 if t == 3 else 9] = False
+                if abs(value) > 1e38 and value != 3e38:
+                    assert torch.isnan(got[t][~clean]).all()
+            near(got[t][clean], want[clean], bound[clean])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "int8"])
 @pytest.mark.parametrize("prefix", [0, 70, 9000])
 def test_out_in_the_place_of_q(gpu_ctx, dtype, prefix):
     """The same bits as into a tensor of its own, from one launch or several."""
