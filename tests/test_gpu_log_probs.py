@@ -74,6 +74,29 @@ def test_orders_and_ties(gpu_ctx, vocab):
     check(gpu_ctx, x, targets, 32, log_probs(gpu_ctx, x, targets, 32))
 
 
+@pytest.mark.parametrize("n,vocab", [(1, 32768), (1, 128256), (3, 50_003), (64, 40_001), (500, 9001)])
+@pytest.mark.parametrize("top", [0, 1, 20])
+def test_masks_that_leave_few_entries(gpu_ctx, n, vocab, top):
+    """All but a few entries -infinity, those in the first, a middle or the last slice; one entry alone; whole slices of
+    equal values; in one launch of clusters and in two."""
+    from quantibbler_b200.scoring import log_probs
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.full((n, vocab), -INF, device="cuda")
+    for row in range(n):
+        kind = row % 4 if n > 1 else top % 4
+        if kind == 0:
+            at = torch.randint(0, vocab, (7,), device="cuda", generator=g)
+            x[row, at] = torch.randn(7, device="cuda", generator=g)
+        elif kind == 1:
+            x[row, vocab - 1] = -3.0
+        elif kind == 2:
+            x[row, :vocab // 2] = 2.5
+        else:
+            x[row, vocab // 3:vocab // 3 + 40] = torch.randn(40, device="cuda", generator=g) * 1e3
+    targets = torch.argmax(x, -1).int()
+    check(gpu_ctx, x, targets, top, log_probs(gpu_ctx, x, targets, top))
+
+
 @pytest.mark.parametrize("top", [0, 3])
 def test_rows_behind_4_gb_of_logits(gpu_ctx, top):
     from quantibbler_b200.scoring import log_probs
