@@ -404,13 +404,10 @@ struct Plan {
     uint32_t prefix_slots, n_slots;           // partial results per (query, head); n_slots 1: none, the output is written
 };
 
-// kMost: column tiles of four query rows that a block needs at most.
-template <bool kI8, int D, int kMost>
-__global__ void __launch_bounds__(128, kI8 ? (kMost == 1 ? 4 : 3) : (kMost == 1 ? 3 : 2))
-attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
-    qk::pdl_launch();
-    qk::pdl_wait();
-    extern __shared__ __align__(16) uint8_t attend_smem[];
+// A block's work; its answer is attend_span's.  kMost: column tiles of four query rows that a block needs at most.
+template <bool kI8, int D, int kMost, bool kWide>
+__device__ __forceinline__ bool attend_block(const CacheView &c, const CacheView &p, const qk::AttendArgs &a, const Plan &pl,
+                                             uint8_t *smem) {
     const uint32_t group = a.n_heads / c.n_kv, row_bytes = kI8 ? D : 2 * D;
     Span s;
     uint32_t id = blockIdx.x, kvh;
@@ -451,12 +448,30 @@ attend_rows_kernel(CacheView c, CacheView p, qk::AttendArgs a, Plan pl) {
     s.k_scale = kI8 ? src->k_scale + line : nullptr;
     s.v_scale = kI8 ? src->v_scale + line : nullptr;
     if constexpr (kMost > 1) {
-        if (s.n_rows > 4) {
-            attend_span<kI8, D, 2>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, attend_smem);
-            return;
-        }
+        if (s.n_rows > 4) return attend_span<kI8, D, 2, kWide>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, smem);
     }
-    attend_span<kI8, D, 1>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, attend_smem);
+    return attend_span<kI8, D, 1, kWide>(s, a, kvh, c.n_kv, pl.n_slots, pl.cluster, smem);
+}
+template <int D, int kMost>
+__device__ __noinline__ void attend_block_wide(const CacheView &c, const CacheView &p, const qk::AttendArgs &a, const Plan &pl,
+                                               uint8_t *smem) {
+    attend_block<true, D, kMost, true>(c, p, a, pl, smem);
+}
+
+template <bool kI8, int D, int kMost>
+__global__ void __launch_bounds__(128, kI8 ? (kMost == 1 ? 4 : 3) : (kMost == 1 ? 3 : 2))
+attend_rows_kernel(const __grid_constant__ CacheView c, const __grid_constant__ CacheView p,
+                   const __grid_constant__ qk::AttendArgs a, const __grid_constant__ Plan pl) {
+    qk::pdl_launch();
+    qk::pdl_wait();
+    extern __shared__ __align__(16) uint8_t attend_smem[];
+    if constexpr (kI8) {
+        // Value scales that lie too far apart are seldom, and told at the end: the block then begins again.  (With the other
+        // form in the loop a look at every step costs a tenth of the time; inlined here, the registers that it takes do.)
+        if (!attend_block<true, D, kMost, false>(c, p, a, pl, attend_smem)) attend_block_wide<D, kMost>(c, p, a, pl, attend_smem);
+    } else {
+        attend_block<false, D, kMost, true>(c, p, a, pl, attend_smem);
+    }
 }
 
 // Partial results of a (query, head) joined: outputs [slot][D], then {maximum (log2 units), sum} [slot] of all rows.

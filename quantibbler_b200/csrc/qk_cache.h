@@ -26,6 +26,18 @@ struct AttendArgs {
     float *scratch;
 };
 
+// INT8: weights times value scales go into the products as two float16 terms, scaled so that 2^14 stands for a weight of one
+// times 2^(e_max + 1), e_max the exponent of the largest value scale so far; the second term is held 2^11 times larger.  A
+// weight times its scale that is 2^-27 of that or more is held to 2^-22 of itself, a smaller one to 2^-50 of that, which is
+// 2^-33 of the key's own scale or less while the scales lie within 2^kScaleSpread of one another.  Where they do not (a row
+// of zeros, whose scale is one, among small ones; an outlier that nearly nobody attends to), or are near the ends of
+// float32's range, three bfloat16 terms take over, which hold any to 2^-24 of itself.  (`least`: the bits, less one, of the
+// smallest scale that is not zero, so that zeros, whose rows add nothing, are the largest.)
+constexpr int kScaleSpread = 16;
+__device__ __forceinline__ bool scales_apart(int e_max, uint32_t least) {
+    return e_max >= 120 || (least != 0xffffffffu && e_max - ((int)((least + 1) >> 23) - 127) > kScaleSpread);
+}
+
 // One launch of the tile kernel (qk_cache_tile.cu): all queries against rows of one slot.
 struct TileArgs {
     const float *q;

@@ -9,10 +9,11 @@
 //
 // Exactness.  INT8: the codes are the A operand of the integer product as they lie; q is 23-bit fixed point in
 // three 8-bit digits, so a score is exact but for q's rounding (2^-22 of its largest entry) and one float32
-// rounding.  The weights times the value scales are two float16 terms (22 bits), scaled to 2^14; codes as float16
-// are exact.  The scales are taken relative to a power of two at their running maximum E, so nothing leaves
-// float16's range.  bfloat16: q and the weights are three bfloat16 terms.  A step's output product starts from
-// zero and is added to the running sum by float32 arithmetic: the tensor core truncates.
+// rounding.  The weights times the value scales are two float16 terms, relative to a power of two at the scales' running
+// maximum E (the bound stands at qk::scales_apart); codes as float16 are exact.  A block in whose span the value scales lie
+// too far apart for that begins again with three bfloat16 terms, and codes in bfloat16, in true units.  bfloat16: q and the
+// weights are three bfloat16 terms.  A step's output product starts from zero and is added to the running sum by float32
+// arithmetic: the tensor core truncates.
 //
 // What bounds it: issue (0.59 of the slots: the codes' conversion to float16, legacy products) and the loads' latency, short
 // of the cache's bytes.  INT8, 32 / 8 heads of 128: two sequences of 65536 rows 49.5 us (4.9 TB/s, join included), 64 of 1
@@ -28,6 +29,7 @@ using qk::CacheView;
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;  // weights enter the float16 product times this
+constexpr float kLowScale = 2048.f;      // and their second terms times this too
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -80,14 +82,14 @@ __device__ __forceinline__ void copy16_to(uint32_t smem, const void *gmem) {
 __device__ __forceinline__ void copy16_some(uint32_t smem, const void *gmem, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
 }
-// {hi, lo} of a weight as two float16 in one word, hi below.
+// {hi, lo 2^11} of a weight as two float16 in one word, hi below: lo loses nothing to float16's smallest numbers.
 __device__ __forceinline__ uint32_t weight_terms(float w) {
     uint32_t hi, r;
     float back;
     asm("{\n .reg .b16 h;\n cvt.rn.f16.f32 h, %2;\n cvt.f32.f16 %1, h;\n mov.b32 %0, {h, h};\n}" : "=r"(hi), "=f"(back) : "f"(w));
     asm("{\n .reg .b16 l, h, x;\n mov.b32 {h, x}, %1;\n cvt.rn.f16.f32 l, %2;\n mov.b32 %0, {h, l};\n}"
         : "=r"(r)
-        : "r"(hi), "f"(w - back));
+        : "r"(hi), "f"((w - back) * kLowScale));
     return r;
 }
 // Codes of byte `i` of two words (biased by 128) as a pair of float16: 1024 + u is the bit pattern 0x6400 | u.
@@ -96,6 +98,14 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b, int i) {
     w = __byte_perm(w, 0x64646464u, 0x4140);
     uint32_t r;
     asm("{\n .reg .b32 c;\n mov.b32 c, 0x64806480;\n sub.rn.f16x2 %0, %1, c;\n}" : "=r"(r) : "r"(w));
+    return r;
+}
+// The same as a pair of bfloat16, of codes as they are: with the low seven bits u of a code 0x4300 | u is 128 + u, with its
+// sign bit 0x4300 | 0x80 is 256 and 0x4300 is 128; the code is the difference.
+__device__ __forceinline__ uint32_t code_pair_bf16(uint32_t a, uint32_t b, int i) {
+    const uint32_t w = __byte_perm(a, b, (4 + i) << 8 | i);
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x007f007fu) | 0x43004300u), "r"((w & 0x00800080u) | 0x43004300u));
     return r;
 }
 
@@ -144,9 +154,10 @@ struct AttendShape {
     }
 };
 
-// kTiles: column tiles of query rows, four rows each.
-template <bool kI8, int D, int kTiles>
-__device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &a, uint32_t kvh, uint32_t n_kv, uint32_t n_slots,
+// kTiles: column tiles of query rows, four rows each.  kWide: weights as three bfloat16 terms; else as two of float16, unless
+// value scales of the block's lie too far apart for them: then nothing is written, and the answer is false to all threads.
+template <bool kI8, int D, int kTiles, bool kWide>
+__device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &a, uint32_t kvh, uint32_t n_kv, uint32_t n_slots,
                                             uint32_t n_cluster, uint8_t *smem) {
     using Shape = AttendShape<kI8, D>;
     constexpr int kRowBytes = Shape::kRowBytes, kPieces = Shape::kPieces, kStages = Shape::kStages;
@@ -268,7 +279,8 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
 #pragma unroll
         for (int i = 0; i < kOut; ++i) o[n][i][0] = o[n][i][1] = 0.f;
     }
-    int e_max = -100;  // exponent of the largest value scale so far
+    int e_max = -100;              // exponent of the largest value scale so far
+    uint32_t least = 0xffffffffu;  // bits, less one, of the smallest that is not zero (of this lane's)
 
     int stage = 0;
     for (int j = j_first; j < s.end; j += kStride, stage = stage + 1 == kStages ? 0 : stage + 1) {
@@ -343,17 +355,18 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                     if (j + (int)g + 8 * h >= s.end) x[n][h] = -INFINITY;
         }
         // ---- the value scales' common power of two
-        float shrink = 1.f, vmul = 1.f;
-        if (kI8) {
-            const uint32_t bits = max(__float_as_uint(fabsf(vs[0])), __float_as_uint(fabsf(vs[1])));
-            const int e_new = max(e_max, min(125, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, bits)))));
+        float shrink = 1.f;
+        if constexpr (!kWide) {
+            const uint32_t b0 = __float_as_uint(fabsf(vs[0])), b1 = __float_as_uint(fabsf(vs[1]));
+            const int e_new = max(e_max, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, max(b0, b1)))));
+            least = min(least, min(b0 - 1u, b1 - 1u));
             shrink = pow2(max(-126, e_max - e_new));
             e_max = e_new;
-            vmul = pow2(-1 - e_new);
+            const float vmul = pow2(-1 - e_new) * kWeightScale;
             vs[0] *= vmul, vs[1] *= vmul;
         }
         // ---- running maximum and sum, weights as terms
-        uint32_t pf[kI8 ? kTiles : kQTiles][2];
+        uint32_t pf[kQTiles][2], last[kTiles];
         float alpha[kTiles];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
@@ -367,23 +380,34 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
             const float p0 = ex2(x[n][0] - base), p1 = ex2(x[n][1] - base);
             l[n] = fmaf(l[n], alpha[n], p0 + p1);
             alpha[n] *= shrink;
-            if (kI8) {
-                pf[n][0] = transposed(weight_terms(p0 * vs[0] * kWeightScale));
-                pf[n][1] = transposed(weight_terms(p1 * vs[1] * kWeightScale));
-            } else {
+            if constexpr (kWide) {
                 uint32_t w[3];
-                split3(p0, p1, w);  // (key g below, key g + 8 above)
+                split3(p0 * vs[0], p1 * vs[1], w);  // (key g below, key g + 8 above)
                 pf[n][0] = transposed(__byte_perm(w[0], w[1], 0x5410));
                 pf[n][1] = transposed(__byte_perm(w[0], w[1], 0x7632));
-                if (n == 0) x[0][0] = __uint_as_float(w[2]);
-                else x[0][1] = __uint_as_float(w[2]);
+                last[n] = w[2];
+            } else {
+                pf[n][0] = transposed(weight_terms(p0 * vs[0]));
+                pf[n][1] = transposed(weight_terms(p1 * vs[1]));
             }
         }
-        if (!kI8) {  // thirds of rows t and 4 + t side by side
-            const uint32_t w0 = __float_as_uint(x[0][0]), w1 = kTiles > 1 ? __float_as_uint(x[0][1]) : 0u;
-            pf[kQTiles - 1][0] = transposed(__byte_perm(w0, w1, 0x5410));
-            pf[kQTiles - 1][1] = transposed(__byte_perm(w0, w1, 0x7632));
+        if constexpr (kWide) {  // thirds of rows t and 4 + t side by side
+            const uint32_t w0 = last[0], w1 = kTiles > 1 ? last[kTiles - 1] : 0u;
+            pf[kTiles][0] = transposed(__byte_perm(w0, w1, 0x5410));
+            pf[kTiles][1] = transposed(__byte_perm(w0, w1, 0x7632));
         }
+        // A channel tile's product in three terms joins the output.
+        auto add_wide = [&](int i, const uint32_t (&af)[4]) {
+            float third[4];
+            mma_bf16_first(third, af, pf[kTiles][0], pf[kTiles][1]);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                float c[4];
+                mma_bf16_first(c, af, pf[n][0], pf[n][1]);
+                o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + (c[1] + third[n]));
+                o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + (c[3] + third[2 + n]));
+            }
+        };
         // ---- output: channels are the M side
         if (kI8) {
             uint32_t vw[4][D / 32];  // keys 2t, 2t + 1, 2t + 8, 2t + 9: channels (D / 8) g ..
@@ -397,20 +421,29 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                     const uint2 v2 = *reinterpret_cast<const uint2 *>(vt + Shape::swizzle(key, g / 2) + 8 * (g % 2));
                     vw[r][0] = v2.x, vw[r][1] = v2.y;
                 }
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) vw[r][i] ^= 0x80808080u;
             }
+            if constexpr (!kWide)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) vw[r][i] ^= 0x80808080u;
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {  // rows g, g + 8 of tile i: channels (D / 8) g + 2 i, + 1
                 const int w = i / 2, b = 2 * (i % 2);
-                const uint32_t af[4] = {code_pair(vw[0][w], vw[1][w], b), code_pair(vw[0][w], vw[1][w], b + 1),
-                                        code_pair(vw[2][w], vw[3][w], b), code_pair(vw[2][w], vw[3][w], b + 1)};
+                auto pair = [&](int r, int b) {
+                    return kWide ? code_pair_bf16(vw[r][w], vw[r + 1][w], b) : code_pair(vw[r][w], vw[r + 1][w], b);
+                };
+                const uint32_t af[4] = {pair(0, b), pair(0, b + 1), pair(2, b), pair(2, b + 1)};
+                if constexpr (kWide) {
+                    add_wide(i, af);
+                } else {
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
-                    float c[4];
-                    mma_f16_first(c, af, pf[n][0], pf[n][1]);
-                    o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + c[1]);
-                    o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + c[3]);
+                    for (int n = 0; n < kTiles; ++n) {
+                        float c[4];
+                        mma_f16_first(c, af, pf[n][0], pf[n][1]);
+                        o[n][i][0] = fmaf(o[n][i][0], alpha[n], fmaf(c[1], 1.f / kLowScale, c[0]));
+                        o[n][i][1] = fmaf(o[n][i][1], alpha[n], fmaf(c[3], 1.f / kLowScale, c[2]));
+                    }
                 }
             }
         } else {
@@ -420,22 +453,14 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
                 uint32_t af[4];
                 const uint32_t key = (lane & 7) + 8 * (lane >> 4), piece = 2 * i + ((lane >> 3) & 1);
                 ldsm4_trans(af, v_addr + Shape::swizzle(key, piece));
-                float third[4];
-                mma_bf16_first(third, af, pf[kQTiles - 1][0], pf[kQTiles - 1][1]);
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
-                    float c[4];
-                    mma_bf16_first(c, af, pf[n][0], pf[n][1]);
-                    o[n][i][0] = fmaf(o[n][i][0], alpha[n], c[0] + (c[1] + third[n]));
-                    o[n][i][1] = fmaf(o[n][i][1], alpha[n], c[2] + (c[3] + third[2 + n]));
-                }
+                add_wide(i, af);
             }
         }
         __syncwarp();  // the stage may be filled again
     }
 
     // ---- the block's warps join: [row][D] outputs, then maxima and sums, each in its warp's ring
-    const float undo = kI8 ? pow2(min(127, e_max + 1)) * (1.f / kWeightScale) : 1.f;
+    const float undo = kWide ? 1.f : pow2(min(127, e_max + 1)) * (1.f / kWeightScale);
     float *mine = reinterpret_cast<float *>(ring);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -450,7 +475,11 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
             for (int h = 0; h < 2; ++h)
                 mine[r * D + (kI8 ? (D / 8) * g + 2 * i + h : 16 * i + 8 * h + g)] = o[n][i][h] * undo;
     }
-    __syncthreads();
+    if constexpr (kWide) {
+        __syncthreads();
+    } else if (__syncthreads_or(qk::scales_apart(e_max, __reduce_min_sync(0xffffffffu, least)))) {
+        return false;
+    }
     const bool alone = n_cluster == 1;
     float *result = reinterpret_cast<float *>(q_lines);  // [8][D] outputs, [8] maxima, [8] sums: for the cluster's blocks
     auto put = [&](uint32_t r, uint32_t c, float top, float sum, float val) {
@@ -489,7 +518,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
             if (c == 0) result[8 * D + r] = top, result[8 * D + 8 + r] = sum;
         }
     }
-    if (alone) return;
+    if (alone) return true;
     // ---- the splits of a cluster join through distributed shared memory, every block a part of the outputs
     cluster_sync();
     uint32_t rank;
@@ -521,6 +550,7 @@ __device__ __forceinline__ void attend_span(const Span s, const qk::AttendArgs &
         put(r, c, top, sum, val);
     }
     cluster_sync();  // (no block ends while another reads its results)
+    return true;
 }
 
 }  // namespace

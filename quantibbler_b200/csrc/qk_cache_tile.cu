@@ -4,25 +4,27 @@
 // The queries that read one kv head are the rows of one product: row r is query r / group, head r % group of the kv
 // head, 128 rows to a CTA, which takes a range of keys 64 at a time.  Two units of four warps take the key blocks in
 // turn, a thread owns a row (no shuffles): running maximum, sum and output in registers, the two units joined at the
-// end.  While one unit is at its exponentials the tensor core works for the other; INT8 scores are formed four blocks
+// end.  While one unit is at its exponentials the tensor core works for the other; INT8 scores are formed three blocks
 // ahead, and a block's output is read out when the maximum of the unit's next block is known.  The weights go back to
 // tensor memory, over their scores, as the A operand; v is read as it lies (MN-major B).  Three warps bring the key blocks
 // in, three the value blocks.
 //
 // Exactness.  INT8 rows: codes as float16 are exact (three warps convert them on their way into shared memory); q is
 // two float16 terms after scaling by a power of two per row (22 bits), and so are the weights times the value scales,
-// which are taken relative to a power of two at their running maximum E and scaled to 2^14 (in blocks that some row does
-// not see whole, at the row's own maximum).  bfloat16 rows go in as
-// they are; q and the weights are three bfloat16 terms.  A block's product with v starts from zero and is added to the
-// row's output in registers, in float32: the tensor core truncates.
+// relative to a power of two at the scales' running maximum E (the bound stands at qk::scales_apart).  Where value scales
+// lie too far apart for that, and in blocks that some row does not see whole, the weights are "wide": three bfloat16 terms
+// times codes in bfloat16, in true units.  bfloat16 rows go in as they are; q and the weights are three bfloat16 terms.  A
+// block's product with v starts from zero and is added to the row's output in registers, in float32: the tensor core
+// truncates.
 //
-// What bounds it: a unit's chain for a block of 64 keys, 4200 cycles (waits 500, maxima 850, the output's turn 850,
-// exponentials, weights and their terms 1900), of which two run side by side, and 16000 cycles of a CTA before its first
-// block (q) and behind its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 99 us, 0.35
-// PFLOP/s of the formula's operations, 0.69 of the tensor core's (29 % of its cycles).  64 x 32 / 8 heads behind 8192
-// bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion: INT8 q in tensor memory with scores two blocks ahead (110), q's
-// loads in front of the barriers' setup (101.6), rows written out by bulk copies (99.9).  bfloat16: 200 registers a
-// thread for the units (+ 1.4), scores three blocks ahead (+ 0.4).
+// What bounds it: a unit's chain for a block of 64 keys, 4300 cycles (waits, maxima, the output's turn, exponentials,
+// weights and their terms), of which two run side by side, and 16000 cycles of a CTA before its first
+// block (q) and behind its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 104 us, 0.33
+// PFLOP/s of the formula's operations.  64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for
+// the INT8 portion: wide weights throughout (115), a branch on the form for every word that is converted (111.5), both
+// forms in one loop of the warp that issues the products (104.6), its look at the form a block ahead (106.2), 192 registers
+// a thread for the units and 64 for the rest (112.5), 176 and 80 (106.5).  Faster by 1: scores four blocks ahead, which
+// leaves no place for a third term.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -44,30 +46,33 @@ constexpr int kUnitRegs = 184, kOtherRegs = 72, kLaunchRegs = 128;
 static_assert(256 * kUnitRegs + 256 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr float kWeightScale = 16384.f;
+constexpr float kWeightScale = 16384.f;  // float16 weights enter the product times this, their second terms times
+constexpr uint32_t kLowBits = 11;        // 2^11 more (of wide weights too), which the product takes off again
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kEdges = 4;  // causal: the blocks that some row of a tile does not see whole are among the last four
 
 template <bool kI8, int D>
 struct TileShape {
-    static constexpr uint32_t kTerms = kI8 ? 2 : 3;                    // of q and of the weights
+    static constexpr uint32_t kTerms = kI8 ? 2 : 3;                    // of q
     static constexpr uint32_t kChunks = D / 64;                        // of 64 channels, rows of 128 bytes
     static constexpr uint32_t kChunkBytes = kKeys * 128, kTileBytes = kChunks * kChunkBytes;
     static constexpr uint32_t kQChunkBytes = kRows * 128, kQTermBytes = kChunks * kQChunkBytes;
     static constexpr uint32_t kStages = kI8 || D == 64 ? 4 : 3;        // of the keys' ring, and of the values'
-    static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a block's key and value scales, and E
+    static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a block's key and value scales, E, and whether its weights are wide
     static constexpr uint32_t kRingBytes = 2 * kStages * kTileBytes;
     static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 512;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
-    // Tensor memory.  INT8: the scores of four blocks, over which their weights lie (16 columns of scores become eight of
-    // either term), the units' outputs.  bfloat16, whose terms are three: a unit's scores, behind them the first two terms
-    // of its weights, the third over scores that have been read, its output.
-    static constexpr uint32_t kAhead = kI8 ? 4 : 2;  // blocks whose scores are formed ahead: block g's lie in place g % kAhead
-    __device__ static constexpr uint32_t score_col(uint32_t at) { return (kI8 ? 64 : 256) * at; }
+    // Tensor memory.  INT8: the scores of three blocks, over which the first two terms of their weights lie (16 columns of
+    // scores become eight of either term), a third term's place for either unit, the units' outputs.  (Scores of four blocks:
+    // 1 % faster.)  bfloat16, whose terms are three: a unit's scores, behind them the first two terms of its weights, the
+    // third over scores that have been read, its output.
+    static constexpr uint32_t kAhead = kI8 ? 3 : 2;  // blocks whose scores are formed ahead: block g's lie in place g % kAhead
+    __device__ static constexpr uint32_t score_col(uint32_t g) { return (kI8 ? 64 : 256) * (g % kAhead); }
     __device__ static constexpr uint32_t out_col(uint32_t u) { return kI8 ? 256 + 128 * u : 256 * u + 128; }
-    __device__ static constexpr uint32_t weight_col(uint32_t term, uint32_t step) {  // of a step of 16 keys, from score_col
-        return kI8 ? 16 * step + 8 * term : (term == 2 ? 0 : 64 + 32 * term) + 8 * step;
+    __device__ static constexpr uint32_t weight_col(uint32_t g, uint32_t term, uint32_t step) {  // of a step of 16 keys
+        return !kI8 ? score_col(g) + (term == 2 ? 0 : 64 + 32 * term) + 8 * step
+                    : term == 2 ? 192 + 32 * (g & 1) + 8 * step : score_col(g) + 16 * step + 8 * term;
     }
     static_assert(kRingBytes >= (D * kRows + 5 * kRows) * 4, "the units' exchange lies in the ring");
 };
@@ -102,6 +107,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uin
         "r"(at), "l"(bd), "r"(idesc), "r"((uint32_t)add)
         : "memory");
 }
+// The same where d counts for 2^-kLowBits of itself.
+__device__ __forceinline__ void mma_ts_above(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.eq.b32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %4;\n}" ::"r"(d),
+        "r"(at), "l"(bd), "r"(idesc), "n"(kLowBits)
+        : "memory");
+}
 // Barrier `id` of n threads; true when all of them say so.
 template <int kId, int kN>
 __device__ __forceinline__ bool vote(bool ok) {
@@ -118,18 +130,18 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two values as their terms, float16 or bfloat16 pairs; t[0] the leading one.
-template <bool kI8>
-__device__ __forceinline__ void terms_of(float a, float b, uint32_t *t) {
-    if constexpr (kI8) {
-        t[0] = pack_f16x2(a, b);
-        const float2 h = __half22float2(*reinterpret_cast<__half2 *>(&t[0]));
-        t[1] = pack_f16x2(a - h.x, b - h.y);
-    } else {
-        uint32_t w[3];
-        split3(a, b, w);
-        t[0] = w[0], t[1] = w[1], t[2] = w[2];
-    }
+// Two values as their terms, t[0] the leading one: two of float16 or three of bfloat16, all but the first `times` larger.
+__device__ __forceinline__ void terms_f16(float a, float b, float times, uint32_t *t) {
+    t[0] = pack_f16x2(a, b);
+    float2 r = __ffma2_rn(__half22float2(*reinterpret_cast<__half2 *>(&t[0])), make_float2(-1.f, -1.f), make_float2(a, b));
+    r = __fmul2_rn(r, make_float2(times, times));
+    t[1] = pack_f16x2(r.x, r.y);
+}
+__device__ __forceinline__ void terms_bf16(float a, float b, float times, uint32_t *t) {
+    t[0] = bf16_pair(a, b);
+    a = (a - __uint_as_float(t[0] << 16)) * times, b = (b - __uint_as_float(t[0] & 0xffff0000u)) * times;
+    t[1] = bf16_pair(a, b);
+    t[2] = bf16_pair(a - __uint_as_float(t[1] << 16), b - __uint_as_float(t[1] & 0xffff0000u));
 }
 // Four codes as float16: 1024 + u is the bit pattern 0x6400 | u, u = code + 128.
 __device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
@@ -137,6 +149,13 @@ __device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint3
     lo = __byte_perm(u, 0x64646464u, 0x4140);
     hi = __byte_perm(u, 0x64646464u, 0x4342);
     asm("{\n .reg .b32 c;\n mov.b32 c, 0x64806480;\n sub.rn.f16x2 %0, %0, c;\n sub.rn.f16x2 %1, %1, c;\n}" : "+r"(lo), "+r"(hi));
+}
+// Four codes as bfloat16: with the low seven bits u of a code 0x4300 | u is 128 + u, with its sign bit 0x4300 | 0x80 is 256
+// and 0x4300 is 128; the code is the difference.
+__device__ __forceinline__ void codes_to_bf16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    const uint32_t a = __byte_perm(codes, 0u, 0x4140), b = __byte_perm(codes, 0u, 0x4342);
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"((a & 0x007f007fu) | 0x43004300u), "r"((a & 0x00800080u) | 0x43004300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"((b & 0x007f007fu) | 0x43004300u), "r"((b & 0x00800080u) | 0x43004300u));
 }
 // Waits for the loads of tensor memory, v's the last of them (which nothing may use before).
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16]) {
@@ -236,6 +255,21 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     // keys that every row of the tile sees: the blocks past them (at the end) are edges
     const int seen0 = min((int)keys, a.causal ? (int)(a.first_row + row0 / group) + 1 - (int)(block0 * kKeys) : (int)keys);
     auto at_edge = [&](uint32_t g) { return (int)((g + 1) * kKeys) > seen0; };
+    // INT8: whether block g's weights are wide, three bfloat16 terms (else two of float16): at an edge, where scales that some
+    // row does not see must not count, and from the first block on up to which the value scales lie too far apart.  s0, s1:
+    // the block's, two a lane; every warp that asks for all blocks in turn comes to the same answers.
+    struct Scales {
+        int e_max = -100;              // exponent of the largest so far
+        uint32_t least = 0xffffffffu;  // bits, less one, of the smallest but zero
+        bool wide = false;
+    };
+    auto look = [&](Scales &st, uint32_t g, float s0, float s1) {
+        const uint32_t b0 = __float_as_uint(fabsf(s0)), b1 = __float_as_uint(fabsf(s1));
+        const int e = max(st.e_max, exponent_of(__reduce_max_sync(0xffffffffu, max(b0, b1))));
+        st.least = min(st.least, __reduce_min_sync(0xffffffffu, min(b0 - 1u, b1 - 1u)));
+        st.wide = st.wide || at_edge(g) || qk::scales_apart(e, st.least);
+        if (!st.wide) st.e_max = e;
+    };
 
     if (warp >= kKeyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -260,7 +294,12 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             };
             if constexpr (kI8) {
                 uint4 held[kPasses];  // the next block's, on their way while this one is converted
+                float s0 = 0.f, s1 = 0.f;  // its value scales
                 auto load = [&](uint32_t g) {
+                    if (is_v) {
+                        const uint32_t key = g * kKeys + lane;
+                        s0 = key < keys ? c.v_scale[line0 + key] : 0.f, s1 = key + 32 < keys ? c.v_scale[line0 + key + 32] : 0.f;
+                    }
 #pragma unroll
                     for (uint32_t i = 0; i < kPasses; ++i) {
                         const uint32_t row = first + i * kStep, key = g * kKeys + row;
@@ -268,26 +307,32 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                                                             : make_uint4(0u, 0u, 0u, 0u);
                     }
                 };
+                Scales st;
                 load(0);
                 for (uint32_t g = 0; g < n_blocks; ++g) {
                     const uint32_t s = g % kStages;
+                    if (is_v) look(st, g, s0, s1);
                     ok = mbar_wait(empties + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
                     if (!ok) break;
                     uint8_t *tile_at = tiles + s * S::kTileBytes + piece / 4 * S::kChunkBytes;
+                    auto store = [&](auto convert) {
 #pragma unroll
-                    for (uint32_t i = 0; i < kPasses; ++i) {  // sixteen codes: two pieces of eight float16
-                        const uint32_t row = first + i * kStep;
-                        if (row >= kKeys) break;
-                        uint32_t w[8];
-                        codes_to_f16(held[i].x, w[0], w[1]);
-                        codes_to_f16(held[i].y, w[2], w[3]);
-                        codes_to_f16(held[i].z, w[4], w[5]);
-                        codes_to_f16(held[i].w, w[6], w[7]);
-                        const uint32_t at = 2 * (piece % 4);
-                        *reinterpret_cast<uint4 *>(tile_at + row * 128 + ((at ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4 *>(tile_at + row * 128 + (((at + 1) ^ (row & 7)) << 4)) =
-                            make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+                        for (uint32_t i = 0; i < kPasses; ++i) {  // sixteen codes: two pieces of eight values
+                            const uint32_t row = first + i * kStep;
+                            if (row >= kKeys) break;
+                            uint32_t w[8];
+                            convert(held[i].x, w[0], w[1]);
+                            convert(held[i].y, w[2], w[3]);
+                            convert(held[i].z, w[4], w[5]);
+                            convert(held[i].w, w[6], w[7]);
+                            const uint32_t at = 2 * (piece % 4);
+                            *reinterpret_cast<uint4 *>(tile_at + row * 128 + ((at ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4 *>(tile_at + row * 128 + (((at + 1) ^ (row & 7)) << 4)) =
+                                make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    };
+                    if (st.wide) store([](uint32_t codes, uint32_t &lo, uint32_t &hi) { codes_to_bf16(codes, lo, hi); });
+                    else store([](uint32_t codes, uint32_t &lo, uint32_t &hi) { codes_to_f16(codes, lo, hi); });
                     load(g + 1);
                     hand_over(fulls + s);
                 }
@@ -352,8 +397,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                                                                   (size_t)(kvh2 * group + which % group) * D + i % (D / 32) * 32));
                 }
             }
-            // ---- INT8: the scales, those of the values relative to the running maximum's power of two; at an edge, where the
-            // maximum is a row's own affair, as they are
+            // ---- INT8: the scales, those of the values relative to the running maximum's power of two, or (wide weights) as
+            // they are, which is what relative to 2^13 would be
             if constexpr (kI8) {
                 float sc[4];  // key and value scales of keys lane, lane + 32 of the next block
                 auto load = [&](uint32_t g) {
@@ -363,21 +408,20 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         sc[i] = key < keys ? c.k_scale[line0 + key] : 0.f, sc[2 + i] = key < keys ? c.v_scale[line0 + key] : 0.f;
                     }
                 };
-                int e_max = -100;
+                Scales st;
                 bool ok = true;
                 load(0);
                 for (uint32_t g = 0; g < n_blocks; ++g) {
                     const uint32_t s = g % kStages;
-                    const uint32_t top = __reduce_max_sync(0xffffffffu,
-                                                           max(__float_as_uint(fabsf(sc[2])), __float_as_uint(fabsf(sc[3]))));
-                    e_max = max(e_max, exponent_of(top));
-                    const float mul = at_edge(g) ? 1.f : pow2(-1 - e_max) * kWeightScale;
+                    look(st, g, sc[2], sc[3]);
+                    const int e = st.wide ? 13 : st.e_max;
+                    const float mul = st.wide ? 1.f : pow2(-1 - e) * kWeightScale;
                     ok = mbar_wait(v_empty + s, ((g / kStages) & 1) ^ 1, abort_flag, a.wait_limit);
                     if (!ok) break;
                     float *dst = scales + s * S::kScaleFloats;
                     dst[lane] = sc[0], dst[32 + lane] = sc[1];
                     dst[kKeys + lane] = sc[2] * mul, dst[kKeys + 32 + lane] = sc[3] * mul;
-                    if (lane == 0) reinterpret_cast<int *>(dst)[2 * kKeys] = e_max;
+                    if (lane == 0) *reinterpret_cast<int2 *>(dst + 2 * kKeys) = make_int2(e, st.wide);
                     load(g + 1);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(v_full + s);
@@ -387,13 +431,13 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         } else {
             // ---- products
             constexpr uint32_t kind = kI8 ? 0 : 1;
-            const uint32_t idesc_s = instruction(kKeys, 0, kind), idesc_o = instruction(D, 1, kind);
+            const uint32_t idesc_s = instruction(kKeys, 0, kind), idesc_o = instruction(D, 1, kind), idesc_wide = instruction(D, 1, 1);
             const uint64_t q_desc = umma_desc(smem_u32(qs)), k_desc = umma_desc(smem_u32(ring));
             // (MN-major: chunks of 64 channels kChunkBytes apart)
             const uint64_t v_desc = umma_desc(smem_u32(v_ring)) | ((uint64_t)(S::kChunkBytes >> 4) << 16);
             auto scores = [&](uint32_t g) {  // (one lane) small terms first
                 const uint64_t kd = k_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
-                const uint32_t dst = tmem + S::score_col(g % kAhead);
+                const uint32_t dst = tmem + S::score_col(g);
 #pragma unroll
                 for (uint32_t i = 0; i < kTerms; ++i)
 #pragma unroll
@@ -405,15 +449,21 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 umma_commit(k_empty + g % kStages);
                 umma_commit(s_full + g % kAhead);
             };
-            auto values = [&](uint32_t g) {  // (one lane)
+            auto values = [&](uint32_t g, bool wide) {  // (one lane) small terms first
                 const uint64_t vd = v_desc + (uint64_t)((g % kStages) * (S::kTileBytes >> 4));
-                const uint32_t weights = tmem + S::score_col(g % kAhead), dst = tmem + S::out_col(g & 1);
-#pragma unroll
-                for (uint32_t i = 0; i < kTerms; ++i)
+                const uint32_t dst = tmem + S::out_col(g & 1), idesc = wide ? idesc_wide : idesc_o;
+                if (wide)
 #pragma unroll
                     for (uint32_t k = 0; k < kKeys / 16; ++k)
-                        mma_ts(dst, weights + S::weight_col(kTerms - 1 - i, k), vd + ((k * 2048) >> 4), idesc_o,
-                               i + k != 0);
+                        mma_ts(dst, tmem + S::weight_col(g, 2, k), vd + ((k * 2048) >> 4), idesc, k != 0);
+#pragma unroll
+                for (uint32_t k = 0; k < kKeys / 16; ++k)
+                    mma_ts(dst, tmem + S::weight_col(g, 1, k), vd + ((k * 2048) >> 4), idesc, wide || k != 0);
+                if constexpr (kI8) mma_ts_above(dst, tmem + S::weight_col(g, 0, 0), vd, idesc);
+                else mma_ts(dst, tmem + S::weight_col(g, 0, 0), vd, idesc, true);
+#pragma unroll
+                for (uint32_t k = 1; k < kKeys / 16; ++k)
+                    mma_ts(dst, tmem + S::weight_col(g, 0, k), vd + ((k * 2048) >> 4), idesc, true);
                 umma_commit(v_empty + g % kStages);
                 umma_commit(o_full + (g & 1));
             };
@@ -425,20 +475,31 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 if (elect_one()) scores(g);
                 __syncwarp();
             }
-            for (uint32_t g = 0; g < n_blocks && ok; ++g) {
+            uint32_t g = 0;
+            auto issue = [&](auto wide_tag) {  // block g; false: the weights are of the other form, or a wait ran out
+                constexpr bool kWide = decltype(wide_tag)::value;
                 const bool more = g + kAhead < n_blocks;
                 // (what the loaders bring is there, most often, before the weights are)
                 ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                if constexpr (!kWide) {
+                    const int wide = reinterpret_cast<const int *>(scales + (g % kStages) * S::kScaleFloats)[2 * kKeys + 1];
+                    if (__any_sync(0xffffffffu, wide)) return false;
+                }
                 if (ok && more) ok = mbar_wait(k_full + (g + kAhead) % kStages, ((g + kAhead) / kStages) & 1, abort_flag, a.wait_limit);
                 if (ok) ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
-                if (!ok) break;
+                if (!ok) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
-                    values(g);
+                    values(g, kWide);
                     if (more) scores(g + kAhead);  // (over columns whose weights the product before reads first)
                 }
                 __syncwarp();
-            }
+                ++g;
+                return true;
+            };
+            if constexpr (kI8)
+                while (g < n_blocks && ok && issue(std::false_type{})) {}
+            while (g < n_blocks && ok && issue(std::true_type{})) {}
             if (!ok) *abort_flag = 1;
         }
     } else {
@@ -478,8 +539,13 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     factor = top < 0x7f800000u ? factor * pow2(e - 14) : __int_as_float(0x7fffffff);
                 }
                 uint32_t t0[3], t1[3];
-                terms_of<kI8>(x.x * mul, x.y * mul, t0);
-                terms_of<kI8>(x.z * mul, x.w * mul, t1);
+                if constexpr (kI8) {
+                    terms_f16(x.x * mul, x.y * mul, 1.f, t0);
+                    terms_f16(x.z * mul, x.w * mul, 1.f, t1);
+                } else {
+                    split3(x.x, x.y, t0);
+                    split3(x.z, x.w, t1);
+                }
                 uint8_t *to = qs + ch / 64 * S::kQChunkBytes + at * 128 + (((ch % 64 / 8) ^ (at & 7)) << 4) + ch % 8 * 2;
 #pragma unroll
                 for (uint32_t n = 0; n < kTerms; ++n) *reinterpret_cast<uint2 *>(to + n * S::kQTermBytes) = make_uint2(t0[n], t1[n]);
@@ -519,7 +585,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
         uint32_t it = 0;
         for (uint32_t g = u; g < n_blocks; g += 2, ++it) {
             const int key0 = (int)(g * kKeys);
-            const uint32_t cols = tmem + S::score_col(g % kAhead) + (((warp % 4) * 32) << 16);  // scores and weights
+            const uint32_t lanes = tmem + (((warp % 4) * 32) << 16), cols = lanes + S::score_col(g);
             // (the scales come with the values, most often before the scores)
             if (!kI8 || !both_ready(v_full + g % kStages, (g / kStages) & 1, s_full + g % kAhead, (g / kAhead) & 1)) {
                 if (kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
@@ -530,11 +596,11 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             const int limit = min(seen, (int)keys) - key0;  // keys of the block that this row sees
             const float *ks = scales + (g % kStages) * S::kScaleFloats, *vs = ks + kKeys;
             float alpha_new;
-            int e_new = -100;
             float2 sum = make_float2(0.f, 0.f);
-            // (kEdge in the type: a select per score would be paid in every block)
+            // (kEdge in the type: a select per score would be paid in every block.  INT8: wide weights, at edges or not.)
             auto weights = [&](auto edge_tag) {
                 constexpr bool kEdge = decltype(edge_tag)::value;
+                constexpr uint32_t kOfWeights = kI8 && !kEdge ? 2 : 3;
                 float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 each16<kKeys / 16>(cols, [&](int part, const uint32_t (&s)[16]) {
 #pragma unroll
@@ -564,23 +630,9 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 m = m_new;
                 if (it) take_output(it - 1);
                 if (!ok) return;
-                float mul = 1.f;
-                if constexpr (kI8 && kEdge) {  // (a scale that this row does not see must not push its own out of float16's range)
-                    float most = 0.f;
-#pragma unroll 4
-                    for (int at = 0; at < (int)kKeys; at += 4) {
-                        const float4 v4 = *reinterpret_cast<const float4 *>(vs + at);
-                        most = fmaxf(most, fmaxf(fmaxf(at < limit ? fabsf(v4.x) : 0.f, at + 1 < limit ? fabsf(v4.y) : 0.f),
-                                                 fmaxf(at + 2 < limit ? fabsf(v4.z) : 0.f, at + 3 < limit ? fabsf(v4.w) : 0.f)));
-                    }
-                    e_new = max(e_here, exponent_of(__float_as_uint(most)));
-                    mul = pow2(-1 - e_new) * kWeightScale;
-                } else if constexpr (kI8) {
-                    e_new = reinterpret_cast<const int *>(ks)[2 * kKeys];
-                }
                 const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
                 each16<kKeys / 16>(cols, [&](int part, const uint32_t (&s)[16]) {
-                    uint32_t t[kTerms][8];
+                    uint32_t t[kOfWeights][8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
@@ -594,31 +646,31 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         x = make_float2(ex2(x.x), ex2(x.y));
                         sum = __fadd2_rn(sum, x);
                         if constexpr (kI8) {
-                            float2 v2 = *reinterpret_cast<const float2 *>(vs + at);
-                            if constexpr (kEdge) v2 = __fmul2_rn(v2, make_float2(mul, mul));
-                            x = __fmul2_rn(x, v2);
+                            x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(vs + at));
                             if constexpr (kEdge) {  // (a key that this row does not see may have the scale NaN)
                                 x.x = at < limit ? x.x : 0.f;
                                 x.y = at + 1 < limit ? x.y : 0.f;
                             }
                         }
                         uint32_t w[3];
-                        terms_of<kI8>(x.x, x.y, w);
+                        if constexpr (kOfWeights == 2) terms_f16(x.x, x.y, (float)(1 << kLowBits), w);
+                        else terms_bf16(x.x, x.y, kI8 ? (float)(1 << kLowBits) : 1.f, w);
 #pragma unroll
-                        for (uint32_t n = 0; n < kTerms; ++n) t[n][e] = w[n];
+                        for (uint32_t n = 0; n < kOfWeights; ++n) t[n][e] = w[n];
                     }
 #pragma unroll
-                    for (uint32_t n = 0; n < kTerms; ++n) tmem_st8(cols + S::weight_col(n, part), t[n]);
+                    for (uint32_t n = 0; n < kOfWeights; ++n) tmem_st8(lanes + S::weight_col(g, n, part), t[n]);
                 });
             };
-            if (at_edge(g)) weights(std::true_type{});
+            const int2 form = kI8 ? *reinterpret_cast<const int2 *>(ks + 2 * kKeys) : make_int2(0, at_edge(g));  // E, wide
+            if (form.y) weights(std::true_type{});
             else weights(std::false_type{});
             if (!ok) break;
             l = fmaf(l, alpha_new, sum.x + sum.y);
             alpha = alpha_new;
             if constexpr (kI8) {
-                alpha *= pow2(max(-126, e_here - e_new));
-                e_here = e_new;
+                alpha *= pow2(max(-126, e_here - form.x));
+                e_here = form.x;
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
