@@ -806,7 +806,11 @@ qk_status qk_grouped_portion(qk_ctx *ctx, const qk_grouped_call *call);
  * QK_I8: a row x of head_dim values (a token's key, rotated, or value of one kv head) is held as
  * scale = float32(max|x| / 127), 1 where that is zero, and the codes clip(rint(x / scale), -127, 127), ties to
  * even, all in 64 bits.  A row that holds an infinity or NaN gets the scale NaN: what reads it is NaN, never a
- * wrong number.  The value is code * scale. */
+ * wrong number.  The value is code * scale.
+ *
+ * Attention holds a query of an INT8 cache to 2^-22 of its largest entry (head_dim 64 and 128), weights to 2^-22 of
+ * themselves or 2^-33 of a weight of one, and sums in float32: weights of at most one times values are added up before
+ * they are divided, so the sum of a sequence's weighted values has to lie in float32's range. */
 typedef struct qk_kv_cache {
     int32_t dtype;            /* QK_F32, QK_BF16 or QK_I8 */
     void *k, *v;              /* [n_seq][n_kv_heads][rows][head_dim] */

@@ -367,10 +367,10 @@ attend_plain_kernel(CacheView c, CacheView p, qk::AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t i = lane + 32 * e;
-                if (i < d) dot = fmaf(qv[e], value_at<KV>(kb, (size_t)j * d + i, 1.f), dot);
+                if (i < d) dot = fmaf(qv[e], value_at<KV>(kb, (size_t)j * d + i, ks), dot);
             }
             for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-            const float x = dot * ks, m_new = fmaxf(m, x), alpha = m_new == -INFINITY ? 1.f : expf(m - m_new);
+            const float x = dot, m_new = fmaxf(m, x), alpha = m_new == -INFINITY ? 1.f : expf(m - m_new);
             const float w = x == -INFINITY ? 0.f : expf(x - m_new);
             l = l * alpha + w;
 #pragma unroll

@@ -37,8 +37,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-__device__ __forceinline__ int exponent_of(float magnitude) {  // clamped to -100 .. 126
-    return min(126, max(-100, (int)(__float_as_uint(magnitude) >> 23) - 127));
+__device__ __forceinline__ int exponent_of(float magnitude) {  // clamped to -100 .. 127
+    return min(127, max(-100, (int)(__float_as_uint(magnitude) >> 23) - 127));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // an 8 x 8 matrix of 16-bit values
     uint32_t r;
@@ -142,7 +142,7 @@ struct AttendShape {
     static constexpr int kQPitch = kRowBytes + 16;                     // bytes of one term of a query row
     static constexpr int kQBytes = 8 * 3 * kQPitch, kResultBytes = (8 * D + 16) * 4;  // (the block's results follow q's terms)
     static constexpr int kTermBytes = kQBytes > kResultBytes ? kQBytes : kResultBytes;
-    static constexpr int kSmem = 4 * kWarpBytes + kTermBytes + 32;
+    static constexpr int kSmem = 4 * kWarpBytes + kTermBytes + 64;
     static_assert(kWarpBytes >= (8 * D + 16) * 4, "a warp's results lie in its ring");
     // (pieces of 16 bytes of a row change places so that fragment loads meet no bank twice)
     __device__ static uint32_t swizzle(uint32_t row, uint32_t piece) {
@@ -155,7 +155,8 @@ struct AttendShape {
 };
 
 // kTiles: column tiles of query rows, four rows each.  kWide: weights as three bfloat16 terms; else as two of float16, unless
-// value scales of the block's lie too far apart for them: then nothing is written, and the answer is false to all threads.
+// value scales of the block's lie too far apart for them, or a query is too small for its factor: then nothing is written,
+// and the answer is false to all threads.
 template <bool kI8, int D, int kTiles, bool kWide>
 __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &a, uint32_t kvh, uint32_t n_kv, uint32_t n_slots,
                                             uint32_t n_cluster, uint8_t *smem) {
@@ -211,7 +212,10 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
 
     // ---- q's terms, a warp per row: lines of [row][term] in shared memory
     uint8_t *q_lines = smem + 4 * Shape::kWarpBytes;
-    float *q_factor = reinterpret_cast<float *>(q_lines + Shape::kTermBytes);  // what turns a row's sums into log2 units
+    // What turns a row's sums into log2 units.  INT8, kWide: divided by a power of two that is given behind the eight factors,
+    // for the smallest queries' own is below float32's range.
+    float *q_factor = reinterpret_cast<float *>(q_lines + Shape::kTermBytes);
+    bool tiny = false;  // INT8: a row has such a query
     const float unit = kLog2E / sqrtf((float)D);
     for (uint32_t r = warp; r < 4 * kTiles; r += 4) {
         constexpr uint32_t kLanes = D / 4;  // lanes with four channels each
@@ -225,7 +229,14 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
                                       max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
             const uint32_t peak = __reduce_max_sync(0xffffffffu, bits);  // (an infinity or NaN is larger than any number)
             const int e = exponent_of(__uint_as_float(peak));
-            const float mul = pow2(21 - e);
+            float mul = pow2(21 - e), more = 1.f;
+            if constexpr (kWide) {
+                const int down = (int)(peak >> 23) - 127 - e;  // (below zero for those alone)
+                more = down < 0 && peak ? pow2(max(-26, down)) : 1.f;
+                x.x /= more, x.y /= more, x.z /= more, x.w /= more;
+            } else {
+                tiny |= peak != 0 && (int)(peak >> 23) - 127 < e;
+            }
             const float v4[4] = {x.x, x.y, x.z, x.w};
             uint32_t word[3] = {0, 0, 0};
 #pragma unroll
@@ -240,7 +251,10 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
 #pragma unroll
                 for (int term = 0; term < 3; ++term) *reinterpret_cast<uint32_t *>(line + term * Shape::kQPitch + c) = word[term];
             }
-            if (lane == 0) q_factor[r] = peak < 0x7f800000u ? pow2(e - 21) * unit : __int_as_float(0x7fffffff);
+            if (lane == 0) {
+                q_factor[r] = peak < 0x7f800000u ? pow2(e - 21) * unit : __int_as_float(0x7fffffff);
+                if constexpr (kWide) q_factor[8 + r] = more;
+            }
         } else {
             uint32_t w0[3], w1[3];
             split3(x.x, x.y, w0);
@@ -257,7 +271,7 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
     // ---- as B fragments.  Column g of tile n: tile n < kTiles: row 4 n + g / 2, term g % 2; the last: third terms of
     // rows g / 2 and 4 + g / 2 side by side
     uint32_t qf[kQTiles][kSteps][2];
-    float f[kTiles];
+    float f[kTiles], f_more[kTiles];
 #pragma unroll
     for (int n = 0; n < kQTiles; ++n) {
         const uint32_t r = n >= kTiles ? 4 * (g % 2) + g / 2 : 4 * n + g / 2, term = n >= kTiles ? 2 : g % 2;
@@ -269,7 +283,7 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
             qf[n][2 * i][0] = w.x, qf[n][2 * i][1] = w.y;
             qf[n][2 * i + 1][0] = w.z, qf[n][2 * i + 1][1] = w.w;
         }
-        if (n < kTiles) f[n < kTiles ? n : 0] = q_factor[4 * n + t];
+        if (n < kTiles) f[n < kTiles ? n : 0] = q_factor[4 * n + t], f_more[n < kTiles ? n : 0] = kI8 && kWide ? q_factor[8 + 4 * n + t] : 1.f;
     }
 
     float o[kTiles][kOut][2], m[kTiles], l[kTiles];
@@ -323,7 +337,8 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
                 for (int h = 0; h < 2; ++h) {
                     // (thirds: columns 2 t and 2 t + 1 of the last tile are rows t and 4 + t)
                     const int low = acc[n][2 * h + 1] * 256 + acc[kTiles][2 * h + n];
-                    x[n][h] = fmaf((float)acc[n][2 * h], 65536.f, (float)low) * f[n] * sc[8 * h + g];
+                    x[n][h] = fmaf((float)acc[n][2 * h], 65536.f, (float)low) * (f[n] * sc[8 * h + g]);
+                    if constexpr (kWide) x[n][h] *= f_more[n];
                 }
         } else {
             float acc[kQTiles][4];
@@ -358,7 +373,7 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
         float shrink = 1.f;
         if constexpr (!kWide) {
             const uint32_t b0 = __float_as_uint(fabsf(vs[0])), b1 = __float_as_uint(fabsf(vs[1]));
-            const int e_new = max(e_max, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, max(b0, b1)))));
+            const int e_new = max(e_max, min(125, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, max(b0, b1))))));
             least = min(least, min(b0 - 1u, b1 - 1u));
             shrink = pow2(max(-126, e_max - e_new));
             e_max = e_new;
@@ -460,7 +475,7 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
     }
 
     // ---- the block's warps join: [row][D] outputs, then maxima and sums, each in its warp's ring
-    const float undo = kWide ? 1.f : pow2(min(127, e_max + 1)) * (1.f / kWeightScale);
+    const float undo = kWide ? 1.f : pow2(e_max + 1) * (1.f / kWeightScale);
     float *mine = reinterpret_cast<float *>(ring);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -477,7 +492,7 @@ __device__ __forceinline__ bool attend_span(const Span s, const qk::AttendArgs &
     }
     if constexpr (kWide) {
         __syncthreads();
-    } else if (__syncthreads_or(qk::scales_apart(e_max, __reduce_min_sync(0xffffffffu, least)))) {
+    } else if (__syncthreads_or(tiny || qk::scales_apart(e_max, __reduce_min_sync(0xffffffffu, least)))) {
         return false;
     }
     const bool alone = n_cluster == 1;

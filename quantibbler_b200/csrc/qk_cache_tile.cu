@@ -48,6 +48,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;  // float16 weights enter the product times this, their second terms times
 constexpr uint32_t kLowBits = 11;        // 2^11 more (of wide weights too), which the product takes off again
+constexpr float kKeyShrink = 0x1p-30f;   // of the key scales that maxima are formed with, see below
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kEdges = 4;  // causal: the blocks that some row of a tile does not see whole are among the last four
@@ -59,7 +60,8 @@ struct TileShape {
     static constexpr uint32_t kChunkBytes = kKeys * 128, kTileBytes = kChunks * kChunkBytes;
     static constexpr uint32_t kQChunkBytes = kRows * 128, kQTermBytes = kChunks * kQChunkBytes;
     static constexpr uint32_t kStages = kI8 || D == 64 ? 4 : 3;        // of the keys' ring, and of the values'
-    static constexpr uint32_t kScaleFloats = kI8 ? 2 * kKeys + 4 : 0;  // a block's key and value scales, E, and whether its weights are wide
+    // Of a block: key scales, value scales, key scales times kKeyShrink, E, whether its weights are wide.
+    static constexpr uint32_t kScaleFloats = kI8 ? 3 * kKeys + 4 : 0;
     static constexpr uint32_t kRingBytes = 2 * kStages * kTileBytes;
     static constexpr uint32_t kSmem = 1024 + kTerms * kQTermBytes + kRingBytes + kStages * kScaleFloats * 4 + 512 + 512;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
@@ -83,8 +85,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-__device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {  // clamped to -100 .. 125
-    return min(125, max(-100, (int)(magnitude_bits >> 23) - 127));
+__device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {  // clamped to -110 .. 127
+    return min(127, max(-110, (int)(magnitude_bits >> 23) - 127));
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
@@ -259,7 +261,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     // row does not see must not count, and from the first block on up to which the value scales lie too far apart.  s0, s1:
     // the block's, two a lane; every warp that asks for all blocks in turn comes to the same answers.
     struct Scales {
-        int e_max = -100;              // exponent of the largest so far
+        int e_max = -110;              // exponent of the largest so far
         uint32_t least = 0xffffffffu;  // bits, less one, of the smallest but zero
         bool wide = false;
     };
@@ -420,8 +422,9 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     if (!ok) break;
                     float *dst = scales + s * S::kScaleFloats;
                     dst[lane] = sc[0], dst[32 + lane] = sc[1];
+                    dst[2 * kKeys + lane] = sc[0] * kKeyShrink, dst[2 * kKeys + 32 + lane] = sc[1] * kKeyShrink;
                     dst[kKeys + lane] = sc[2] * mul, dst[kKeys + 32 + lane] = sc[3] * mul;
-                    if (lane == 0) *reinterpret_cast<int2 *>(dst + 2 * kKeys) = make_int2(e, st.wide);
+                    if (lane == 0) *reinterpret_cast<int2 *>(dst + 3 * kKeys) = make_int2(e, st.wide);
                     load(g + 1);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(v_full + s);
@@ -482,7 +485,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                 // (what the loaders bring is there, most often, before the weights are)
                 ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
                 if constexpr (!kWide) {
-                    const int wide = reinterpret_cast<const int *>(scales + (g % kStages) * S::kScaleFloats)[2 * kKeys + 1];
+                    const int wide = reinterpret_cast<const int *>(scales + (g % kStages) * S::kScaleFloats)[3 * kKeys + 1];
                     if (__any_sync(0xffffffffu, wide)) return false;
                 }
                 if (ok && more) ok = mbar_wait(k_full + (g + kAhead) % kStages, ((g + kAhead) / kStages) & 1, abort_flag, a.wait_limit);
@@ -557,11 +560,17 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             asm volatile("bar.sync 3, 256;" ::: "memory");
         }
         const float f = row_factor[r];
+        // A raw score is below 2^29, and times its key's scale it may leave float32's range although f brings it back.  So the
+        // weights' exponents are formed with scale times f, and the maxima, which come first, with scales that are 2^30
+        // smaller (what these lose of scales below 2^-96 is nothing after f) unless f is so large that nothing comes back.
+        const bool large = f >= 0x1p43f;  // (a query of 2^60 or more)
+        const uint32_t of_maxima = large ? 0 : 2 * kKeys;
+        const float f_maxima = large ? f : f * (1.f / kKeyShrink);
         const uint32_t outs = tmem + S::out_col(u) + (((warp % 4) * 32) << 16);
         // keys of this CTA that this row sees
         const int seen = a.causal ? (int)(a.first_row + query) + 1 - (int)(block0 * kKeys) : (int)keys;
         float m = -INFINITY, l = 0.f;
-        int e_here = -100;
+        int e_here = -110;
         float o[D];
 #pragma unroll
         for (int i = 0; i < D; ++i) o[i] = 0.f;
@@ -609,7 +618,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         float4 x = make_float4(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]),
                                                __uint_as_float(s[e + 3]));
                         if constexpr (kI8) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + at);
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + of_maxima + at);
                             const float2 lo = __fmul2_rn(make_float2(x.x, x.y), make_float2(k4.x, k4.y));
                             const float2 hi = __fmul2_rn(make_float2(x.z, x.w), make_float2(k4.z, k4.w));
                             x = make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -624,7 +633,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     }
                 });
                 const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                const float m_new = fmaxf(m, top * f);
+                const float m_new = fmaxf(m, top * (kI8 ? f_maxima : f));
                 const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
                 alpha_new = ex2(m - base);
                 m = m_new;
@@ -637,8 +646,8 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     for (int e = 0; e < 8; ++e) {
                         float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
                         const int at = 16 * part + 2 * e;
-                        if constexpr (kI8) x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(ks + at));
-                        x = __ffma2_rn(x, f2, base2);
+                        if constexpr (kI8) x = __ffma2_rn(x, __fmul2_rn(*reinterpret_cast<const float2 *>(ks + at), f2), base2);
+                        else x = __ffma2_rn(x, f2, base2);
                         if constexpr (kEdge) {
                             x.x = at < limit ? x.x : -INFINITY;
                             x.y = at + 1 < limit ? x.y : -INFINITY;
@@ -662,7 +671,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     for (uint32_t n = 0; n < kOfWeights; ++n) tmem_st8(lanes + S::weight_col(g, n, part), t[n]);
                 });
             };
-            const int2 form = kI8 ? *reinterpret_cast<const int2 *>(ks + 2 * kKeys) : make_int2(0, at_edge(g));  // E, wide
+            const int2 form = kI8 ? *reinterpret_cast<const int2 *>(ks + 3 * kKeys) : make_int2(0, at_edge(g));  // E, wide
             if (form.y) weights(std::true_type{});
             else weights(std::false_type{});
             if (!ok) break;

@@ -136,3 +136,40 @@ def test_a_row_of_zeros_that_was_appended(gpu_ctx, small):
     near(step[0], *attention64(q[-1], *rows))
     for t in (1, 63, 64, 200, n - 1):
         near(portion[t], *attention64(q[t], rows[0][:, :t + 1], rows[1][:, :t + 1]))
+
+
+@pytest.mark.parametrize("size", ["largest queries", "largest keys"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_queries_and_keys_at_the_end_of_the_range(gpu_ctx, size, d):
+    """Entries up to the largest float32 in one head's query (or keys of 1e35), with keys (queries) so small that the scores
+    are ordinary ones: by rows, behind a prefix by tiles, and in a portion.  (The heads beside the large query see scores of
+    zero.)  The query's entries are of one magnitude, so that a rounding relative to the largest is one relative to each."""
+    from quantibbler_b200.cache import KvCache
+    g = torch.Generator(device="cuda").manual_seed(d)
+    heads, kv, rows, batch = 8, 2, 150, 70
+    ks = 1e-40 if size == "largest queries" else 1e35 / 127
+
+    def filled(n_seq):
+        shape = (n_seq, kv, rows, d)
+        codes = [torch.randint(-127, 128, shape, device="cuda", generator=g, dtype=torch.int8) for _ in range(2)]
+        scales = [torch.full(shape[:3], s, device="cuda") for s in (ks, 0.01)]
+        return KvCache(gpu_ctx, *codes, *scales), [x.double() * s.double()[..., None] for x, s in zip(codes, scales)]
+
+    c, (k, v) = filled(batch)
+    p, (pk, pv) = filled(1)
+    q = torch.rand(batch, heads, d, device="cuda", generator=g) * 0.5 + 0.5
+    q *= torch.randint(0, 2, q.shape, device="cuda", generator=g) * 2.0 - 1.0
+    if size == "largest queries":
+        top = torch.finfo(torch.float32).max
+        q[:, 1::2] *= top
+        q[:, 1::2, 3], q[:, 3::4, 3] = top, -top
+    else:
+        q *= 1e-34
+    lens = torch.full((batch,), rows, dtype=torch.int32, device="cuda")
+    steps, behind = c.attend(q, lens), c.attend(q, lens, prefix=p, prefix_len=rows)
+    portion = c.portion(q, 2, 60)
+    gpu_ctx.synchronize()
+    for b in range(batch):
+        near(steps[b], *attention64(q[b], k[b], v[b]))
+        near(behind[b], *attention64(q[b], torch.cat([pk[0], k[b]], 1), torch.cat([pv[0], v[b]], 1)))
+        near(portion[b], *attention64(q[b], k[2, :, :61 + b], v[2, :, :61 + b]))
