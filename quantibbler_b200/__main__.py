@@ -41,19 +41,22 @@ def main(argv=None) -> int:
     sub.add_parser("trace", help="replay a trace of token ids (see bin/trace_run)")
     a = ap.parse_args(argv)
     from .gpu import GpuContext
-    from .registry import load_decoder
+    from .registry import UnknownSetting, load_decoder
     prompt = [int(t) for t in a.prompt.split(",")]
     settings = {} if a.dtype is None else {"serving": a.dtype}
     if a.kv_dtype is not None:
         settings["kv_dtype"] = a.kv_dtype
     if a.command == "score":
         conts = [[int(t) for t in c.split(",")] for c in a.continuation]
-        decoder = load_decoder(GpuContext.init(), a.model, max_batch=len(conts), max_prefix=len(prompt),
-                               max_seq=max(len(c) for c in conts), **settings)
-        print(json.dumps(decoder.score(prompt, conts, a.top)))
-        return 0
-    decoder = load_decoder(GpuContext.init(), a.model, max_seq=len(prompt) + max(a.max_tokens, 1), **settings)
-    print(json.dumps(decoder.generate(prompt, a.max_tokens, a.eos)))
+        settings.update(max_batch=len(conts), max_prefix=len(prompt), max_seq=max(len(c) for c in conts))
+    else:
+        settings["max_seq"] = len(prompt) + max(a.max_tokens, 1)
+    try:
+        decoder = load_decoder(GpuContext.init(), a.model, **settings)
+    except UnknownSetting as e:   # (--kv-dtype or score with a model of another kind)
+        ap.error(str(e))
+    print(json.dumps(decoder.score(prompt, conts, a.top) if a.command == "score" else
+                     decoder.generate(prompt, a.max_tokens, a.eos)))
     return 0
 
 
