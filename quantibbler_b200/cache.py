@@ -28,11 +28,15 @@ class KvCacheStruct(ctypes.Structure):
                 ("n_kv_heads", ctypes.c_size_t), ("rows", ctypes.c_size_t), ("head_dim", ctypes.c_size_t)]
 
 
+def _stream_of(torch, handle, device):
+    """The stream ``handle`` as torch knows it."""
+    return torch.cuda.ExternalStream(handle, device=device) if handle > 2 else torch.cuda.default_stream(device)
+
+
 @contextlib.contextmanager
 def _joined(torch, handle, current):
     """Orders the context's stream ``handle`` behind torch's ``current`` stream, and that behind it."""
-    stream = torch.cuda.ExternalStream(handle, device=current.device) if handle > 2 else \
-        torch.cuda.default_stream(current.device)
+    stream = _stream_of(torch, handle, current.device)
     stream.wait_stream(current)
     try:
         yield
@@ -72,8 +76,10 @@ def workspace(ctx: GpuContext, size: int, device):
     if not kept or kept[-1].numel() < size:
         with _growing:
             if not kept or kept[-1].numel() < size:
-                grown = torch.empty(max(size, 1 << 20, 2 * kept[-1].numel() if kept else 0), dtype=torch.uint8, device=device)
-                kept.append(grown)
+                # (of that stream's own memory: another thread's call may use it before this one has ordered the streams)
+                with torch.cuda.stream(_stream_of(torch, ctx.stream_handle, device)):
+                    kept.append(torch.empty(max(size, 1 << 20, 2 * kept[-1].numel() if kept else 0), dtype=torch.uint8,
+                                            device=device))
     return kept[-1]
 
 
