@@ -18,13 +18,13 @@
 // truncates.
 //
 // What bounds it: a unit's chain for a block of 64 keys, 4300 cycles (waits, maxima, the output's turn, exponentials,
-// weights and their terms), of which two run side by side, and 16000 cycles of a CTA before its first
-// block (q) and behind its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 104 us, 0.33
-// PFLOP/s of the formula's operations.  64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for
-// the INT8 portion: wide weights throughout (115), a branch on the form for every word that is converted (111.5), both
-// forms in one loop of the warp that issues the products (104.6), its look at the form a block ahead (106.2), 192 registers
-// a thread for the units and 64 for the rest (112.5), 176 and 80 (106.5).  Faster by 1: scores four blocks ahead, which
-// leaves no place for a third term.
+// weights and their terms), of which two run side by side, and 16000 cycles of a CTA before its first block (q) and behind
+// its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 104.7 us, 0.33 PFLOP/s of the
+// formula's operations.  64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion:
+// wide weights throughout (115), a branch on the form for every word that is converted (111.5), both forms in one loop of
+// the warp that issues the products (+ 0.5), its look at the form a block ahead (+ 2), 184 registers a thread for the units
+// and 72 for the rest (105.5), 192 and 64 (113.7).  Faster by 1: scores four blocks ahead, which leaves no place for a third
+// term.  bfloat16: 200 registers for the units (+ 1.4), scores three blocks ahead (+ 0.4).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -42,13 +42,12 @@ using qk::TileArgs;
 
 constexpr uint32_t kRows = 128, kKeys = 64;  // query rows of a CTA, keys of a block
 constexpr uint32_t kThreads = 512, kLoaders = 96, kKeyWarp = 8, kValueWarp = 11, kScaleWarp = 14, kMmaWarp = 15;  // three warps a loader
-constexpr int kUnitRegs = 184, kOtherRegs = 72, kLaunchRegs = 128;
-static_assert(256 * kUnitRegs + 256 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
+constexpr int kLaunchRegs = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kWeightScale = 16384.f;  // float16 weights enter the product times this, their second terms times
 constexpr uint32_t kLowBits = 11;        // 2^11 more (of wide weights too), which the product takes off again
-constexpr float kKeyShrink = 0x1p-30f;   // of the key scales that maxima are formed with, see below
+constexpr float kKeyShrink = 0x1p-30f;   // of the second set of a block's key scales, see below
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kEdges = 4;  // causal: the blocks that some row of a tile does not see whole are among the last four
@@ -56,6 +55,8 @@ constexpr uint32_t kEdges = 4;  // causal: the blocks that some row of a tile do
 template <bool kI8, int D>
 struct TileShape {
     static constexpr uint32_t kTerms = kI8 ? 2 : 3;                    // of q
+    static constexpr int kUnitRegs = kI8 ? 200 : 184, kOtherRegs = kI8 ? 56 : 72;
+    static_assert(256 * kUnitRegs + 256 * kOtherRegs <= (int)kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
     static constexpr uint32_t kChunks = D / 64;                        // of 64 channels, rows of 128 bytes
     static constexpr uint32_t kChunkBytes = kKeys * 128, kTileBytes = kChunks * kChunkBytes;
     static constexpr uint32_t kQChunkBytes = kRows * 128, kQTermBytes = kChunks * kQChunkBytes;
@@ -274,7 +275,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
     };
 
     if (warp >= kKeyWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
         if (warp < kScaleWarp) {
             // ---- key blocks into their ring, value blocks into theirs; rows past the end are zeros
             const bool is_v = warp >= kValueWarp;
@@ -506,7 +507,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             if (!ok) *abort_flag = 1;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUnitRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kUnitRegs));
         const uint32_t u = warp / 4, r = threadIdx.x % 128;
         const uint32_t query = min(row0 + r, n_rows - 1) / group;
         // q: a warp takes sixteen rows, D / 4 lanes a row
@@ -525,8 +526,10 @@ attend_tile_kernel(CacheView c, TileArgs a) {
 #pragma unroll
             for (uint32_t i = 0; i < kTurns; ++i) {
                 const uint32_t at = warp * 16 + i * kSide + lane / kLanes;
-                const float4 x = held[i];
-                float factor = unit_scale, mul = 1.f;  // factor: what turns a raw score into log2 units
+                // In log2 units from here on: what is left to do to a raw score is a power of two, so that its product with that
+                // is exact and the largest score less the maximum is zero, however large it is.
+                const float4 x = make_float4(held[i].x * unit_scale, held[i].y * unit_scale, held[i].z * unit_scale, held[i].w * unit_scale);
+                float factor = 1.f, mul = 1.f;
                 if constexpr (kI8) {
                     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
                                        max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
@@ -539,7 +542,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     const int e = exponent_of(top);
                     mul = pow2(14 - e);
                     // (an infinity or NaN: the row is NaN)
-                    factor = top < 0x7f800000u ? factor * pow2(e - 14) : __int_as_float(0x7fffffff);
+                    factor = top < 0x7f800000u ? pow2(e - 14) : __int_as_float(0x7fffffff);
                 }
                 uint32_t t0[3], t1[3];
                 if constexpr (kI8) {
@@ -559,13 +562,13 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             if (lane == 0) mbar_arrive(q_full);
             asm volatile("bar.sync 3, 256;" ::: "memory");
         }
-        const float f = row_factor[r];
-        // A raw score is below 2^29, and times its key's scale it may leave float32's range although f brings it back.  So the
-        // weights' exponents are formed with scale times f, and the maxima, which come first, with scales that are 2^30
-        // smaller (what these lose of scales below 2^-96 is nothing after f) unless f is so large that nothing comes back.
-        const bool large = f >= 0x1p43f;  // (a query of 2^60 or more)
-        const uint32_t of_maxima = large ? 0 : 2 * kKeys;
-        const float f_maxima = large ? f : f * (1.f / kKeyShrink);
+        const float f = kI8 ? row_factor[r] : 1.f;
+        // A raw score is below 2^29, and times its key's scale it may leave float32's range although f brings it back: unless
+        // f is so large that nothing comes back, scales are taken that are 2^30 smaller (what these lose of scales below 2^-96
+        // is nothing after f).
+        const bool large = f >= 0x1p46f;  // (a query of 2^60 or more)
+        const uint32_t which_scales = large ? 0 : 2 * kKeys;
+        const float to_log2 = !kI8 || large ? f : f * (1.f / kKeyShrink);
         const uint32_t outs = tmem + S::out_col(u) + (((warp % 4) * 32) << 16);
         // keys of this CTA that this row sees
         const int seen = a.causal ? (int)(a.first_row + query) + 1 - (int)(block0 * kKeys) : (int)keys;
@@ -618,7 +621,7 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                         float4 x = make_float4(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]),
                                                __uint_as_float(s[e + 3]));
                         if constexpr (kI8) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + of_maxima + at);
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + which_scales + at);
                             const float2 lo = __fmul2_rn(make_float2(x.x, x.y), make_float2(k4.x, k4.y));
                             const float2 hi = __fmul2_rn(make_float2(x.z, x.w), make_float2(k4.z, k4.w));
                             x = make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -633,21 +636,22 @@ attend_tile_kernel(CacheView c, TileArgs a) {
                     }
                 });
                 const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                const float m_new = fmaxf(m, top * (kI8 ? f_maxima : f));
+                const float m_new = fmaxf(m, top * to_log2);
                 const float base = m_new == -INFINITY ? 0.f : m_new;  // (nothing seen yet: every weight is zero)
                 alpha_new = ex2(m - base);
                 m = m_new;
                 if (it) take_output(it - 1);
                 if (!ok) return;
-                const float2 f2 = make_float2(f, f), base2 = make_float2(-base, -base);
+                const float2 f2 = make_float2(to_log2, to_log2), base2 = make_float2(-base, -base);
                 each16<kKeys / 16>(cols, [&](int part, const uint32_t (&s)[16]) {
                     uint32_t t[kOfWeights][8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float2 x = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
                         const int at = 16 * part + 2 * e;
-                        if constexpr (kI8) x = __ffma2_rn(x, __fmul2_rn(*reinterpret_cast<const float2 *>(ks + at), f2), base2);
-                        else x = __ffma2_rn(x, f2, base2);
+                        // (to_log2 is a power of two: this is the difference of what the maximum was formed from)
+                        if constexpr (kI8) x = __fmul2_rn(x, *reinterpret_cast<const float2 *>(ks + which_scales + at));
+                        x = __ffma2_rn(x, f2, base2);
                         if constexpr (kEdge) {
                             x.x = at < limit ? x.x : -INFINITY;
                             x.y = at + 1 < limit ? x.y : -INFINITY;
