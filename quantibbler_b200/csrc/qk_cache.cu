@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <initializer_list>
 #include <type_traits>
 
 #include "qk_cache.h"
@@ -582,6 +583,10 @@ join_few_kernel(qk::AttendArgs a, uint32_t n_slots) {
 // ------------------------------------------------------------------ host side
 using qk::DeviceGuard;
 
+bool on(size_t bytes, std::initializer_list<const void *> pointers) {  // all on boundaries of so many bytes
+    return std::all_of(pointers.begin(), pointers.end(), [&](const void *p) { return (uintptr_t)p % bytes == 0; });
+}
+
 qk_status check_cache(const qk_kv_cache *c, const char *what) {
     if (!c) return qk::fail(QK_ERR_VALUE, "%s is null", what);
     if (c->dtype != QK_F32 && c->dtype != QK_BF16 && c->dtype != QK_I8)
@@ -597,6 +602,9 @@ qk_status check_cache(const qk_kv_cache *c, const char *what) {
     if (!c->k || !c->v) return qk::fail(QK_ERR_VALUE, "%s: k or v is null", what);
     if (c->dtype == QK_I8 && (!c->k_scale || !c->v_scale))
         return qk::fail(QK_ERR_VALUE, "%s: an int8 cache needs k_scale and v_scale", what);
+    if (!on(c->dtype == QK_F32 ? 4 : c->dtype == QK_BF16 ? 2 : 1, {c->k, c->v}) ||
+        (c->dtype == QK_I8 && !on(4, {c->k_scale, c->v_scale})))
+        return qk::fail(QK_ERR_VALUE, "%s: rows or scales lie on no boundary of their type", what);
     return QK_OK;
 }
 
@@ -635,6 +643,7 @@ qk_status check_heads(const qk_kv_cache *c, size_t n_heads, size_t n_tokens) {
 // A token's row of `width` values, `stride` to the next.
 qk_status check_rows(const char *what, const void *p, size_t stride, size_t width) {
     if (!p) return qk::fail(QK_ERR_VALUE, "%s is null", what);
+    if (!on(4, {p})) return qk::fail(QK_ERR_VALUE, "%s lies on no float boundary", what);
     if (stride < width) return qk::fail(QK_ERR_VALUE, "%s: rows of %zu values cannot be %zu apart", what, width, stride);
     return QK_OK;
 }
@@ -862,6 +871,8 @@ qk_status qk_cache_append(qk_ctx *ctx, const qk_kv_cache *cache, const float *q,
     if ((st = check_rows("k", k, k_stride, kv_width)) != QK_OK) return st;
     if ((st = check_rows("v", v, v_stride, kv_width)) != QK_OK) return st;
     if (!cos_sin || !positions || !seq_index) return qk::fail(QK_ERR_VALUE, "cos_sin, positions or seq_index is null");
+    if (!on(4, {cos_sin, positions, seq_index}))
+        return qk::fail(QK_ERR_VALUE, "cos_sin, positions or seq_index lies on no boundary of its type");
     if (first_position > 0x7fffffffull || n_positions > 0x7fffffffull)
         return qk::fail(QK_ERR_VALUE, "positions are 32-bit: first_position %zu, n_positions %zu", first_position, n_positions);
     qk_ctx *c;
@@ -913,6 +924,8 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
     if ((st = check_heads(cache, cache->n_kv_heads, n_tokens)) != QK_OK) return st;
     if (!positions || !seq_index || !k_out || !v_out)
         return qk::fail(QK_ERR_VALUE, "positions, seq_index, k_out or v_out is null");
+    if (!on(4, {positions, seq_index}) || !on(out_dtype == QK_F32 ? 4 : 2, {k_out, v_out}))
+        return qk::fail(QK_ERR_VALUE, "positions, seq_index, k_out or v_out lies on no boundary of its type");
     if (out_dtype != QK_F32 && out_dtype != QK_BF16)
         return qk::fail(QK_ERR_VALUE, "rows are read as float32 or bfloat16, got tag %d", out_dtype);
     if (first_position > 0x7fffffffull) return qk::fail(QK_ERR_VALUE, "positions are 32-bit: first_position %zu", first_position);
@@ -967,6 +980,7 @@ qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cac
     if ((st = check_rows("q", q, q_stride, n_heads * cache->head_dim)) != QK_OK) return st;
     if ((st = check_rows("out", out, out_stride, n_heads * cache->head_dim)) != QK_OK) return st;
     if (!kv_len) return qk::fail(QK_ERR_VALUE, "kv_len is null");
+    if (!on(4, {kv_len})) return qk::fail(QK_ERR_VALUE, "kv_len lies on no boundary of its type");
     if ((st = check_scratch(scratch, qk_cache_attend_scratch(cache, prefix_len, batch, n_heads))) != QK_OK) return st;
     if (batch == 0) return QK_OK;
     qk::AttendArgs a{};

@@ -511,6 +511,9 @@ qk_status qk_log_probs(qk_ctx *ctx, const float *logits, size_t n_tokens, size_t
     if (!logits) return qk::fail(QK_ERR_VALUE, "logits is null");
     if ((uintptr_t)logits % sizeof(float)) return qk::fail(QK_ERR_VALUE, "logits lie on no float boundary");
     if (logprob && !targets) return qk::fail(QK_ERR_VALUE, "logprob needs targets");
+    for (const void *p : {(const void *)targets, (const void *)lse, (const void *)logprob, (const void *)entropy,
+                          (const void *)top_logprob, (const void *)top_ids})
+        if ((uintptr_t)p % 4) return qk::fail(QK_ERR_VALUE, "targets or an output lies on no boundary of its type");
     const size_t need = qk_log_probs_scratch(n_tokens, vocab, n_top);
     if (need && (!scratch || (uintptr_t)scratch % 16)) return qk::fail(QK_ERR_VALUE, "scratch is null or on no 16-byte boundary");
     if (n_tokens == 0) return QK_OK;
