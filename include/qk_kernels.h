@@ -835,13 +835,15 @@ qk_status qk_cache_read(qk_ctx *ctx, const qk_kv_cache *cache, const int32_t *po
                         size_t first_position, size_t n_tokens, int32_t out_dtype, void *k_out, void *v_out);
 /* softmax(q k^T / sqrt(head_dim)) v for one query per sequence: sequence b (of batch <= cache->n_seq) sees
  * rows 0 .. kv_len[b] - 1 of its slot (kv_len is clamped to 0 .. rows) and, with prefix_len > 0, the first
- * prefix_len rows of slot prefix_seq of `prefix`, which are read once for all sequences.  The two caches agree
- * in dtype, kv heads and head_dim; `prefix` may be the same cache.  A sequence that sees no row gets zeros.
+ * prefix_len rows of slot prefix_seq of `prefix`, which the tensor-core kernels below read once for all sequences (the
+ * plain one once per sequence and head).  The two caches agree in dtype, kv heads and head_dim; `prefix` may be the same cache.  A sequence that sees no row gets zeros.
  * q [batch][n_heads][head_dim] (already rotated) and out, batch rows q_stride and out_stride values apart.
  * out may be q itself, but may not overlap it otherwise.
  * scratch: qk_cache_attend_scratch bytes on a 16-byte boundary (null where that is 0), nothing kept in it between
- * calls; calls that may overlap on the device need one each.  head_dim up to 256; head_dim 64 and 128 with 16-byte aligned rows run on the tensor
- * cores (all but float32 caches), others take a plain kernel. */
+ * calls; calls that may overlap on the device need one each.  head_dim up to 256.  INT8 and bfloat16 caches of head_dim 64
+ * and 128 run on the tensor cores where k, v and q lie on 16-byte boundaries and q_stride is a multiple of four values.
+ * All else, float32 caches among it, takes a plain kernel, a warp to a query's head, which is 80 to 380 times slower: a q
+ * that lies off 16 bytes is better copied first. */
 qk_status qk_cache_attend(qk_ctx *ctx, const qk_kv_cache *cache, const qk_kv_cache *prefix, size_t prefix_seq,
                           size_t prefix_len, const float *q, size_t q_stride, const int32_t *kv_len, size_t batch,
                           size_t n_heads, void *scratch, float *out, size_t out_stride);

@@ -37,7 +37,7 @@ def main(argv=None) -> int:
     sc.add_argument("--top", type=int, default=0, help="most probable alternatives to print at each place")
     sc.add_argument("--dtype", choices=("bfloat16", "float32"), default=None, help="default: the model's own")
     sc.add_argument("--kv-dtype", choices=("bfloat16", "float32", "int8"), default=None,
-                    help="storage of the key/value cache")
+                    help="storage of the key/value cache (default: float32, the slowest by far)")
     sub.add_parser("trace", help="replay a trace of token ids (see bin/trace_run)")
     a = ap.parse_args(argv)
     from .gpu import GpuContext

@@ -97,7 +97,10 @@ class KvCache:
 
     ``k`` and ``v`` are contiguous float32, bfloat16 or int8 tensors; int8 caches come with ``k_scale`` and
     ``v_scale`` ``[slots, kv heads, rows]`` (float32).  Row r of a slot holds the position
-    ``first_position + r`` of its sequence (``first_position`` > 0: the rows behind a shared prefix)."""
+    ``first_position + r`` of its sequence (``first_position`` > 0: the rows behind a shared prefix).
+
+    Attention over bfloat16 and int8 rows of head_dim 64 and 128 runs on the tensor cores where k, v and q lie on
+    16-byte boundaries; other caches, and a q off them, take a plain kernel that is a hundred times slower."""
 
     def __init__(self, ctx: GpuContext, k, v, k_scale=None, v_scale=None, first_position: int = 0):
         import torch

@@ -339,7 +339,9 @@ read_kernel(CacheView c, const int32_t *__restrict__ positions, const int32_t *_
 
 // ------------------------------------------------------------------ attention, plain form
 // Any dtype and head size: a warp per (query row, head), the lanes share the channels, one pass with the running
-// maximum and sum.  What the fast kernels cannot hold runs here.
+// maximum and sum.  What the fast kernels cannot hold runs here, bound by the chain of a key: loads, the lanes' sum, two
+// exponentials; keys are not split and rows not shared.  32 / 8 heads, float32 rows of 128: one sequence of 2048 rows
+// 2180 us, 64 of 1 to 2048 4930, a portion of 2048 tokens 14800, 64 behind 8192 shared rows 12000.
 template <typename KV>
 __global__ void __launch_bounds__(128)
 attend_plain_kernel(CacheView c, CacheView p, qk::AttendArgs a) {

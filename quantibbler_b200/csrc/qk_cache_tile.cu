@@ -20,7 +20,8 @@
 // What bounds it: a unit's chain for a block of 64 keys, 4300 cycles (waits, maxima, the output's turn, exponentials,
 // weights and their terms), of which two run side by side, and 16000 cycles of a CTA before its first block (q) and behind
 // its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 104.7 us, 0.33 PFLOP/s of the
-// formula's operations.  64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion:
+// formula's operations (in a program where it took 110, a first value scale that made all weights wide: 133).
+// 64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion:
 // wide weights throughout (115), a branch on the form for every word that is converted (111.5), both forms in one loop of
 // the warp that issues the products (+ 0.5), its look at the form a block ahead (+ 2), 184 registers a thread for the units
 // and 72 for the rest (105.5), 192 and 64 (113.7).  Faster by 1: scores four blocks ahead, which leaves no place for a third

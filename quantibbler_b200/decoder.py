@@ -46,7 +46,8 @@ class DecoderConfig:
     kv_dtype: str = "bfloat16"
     max_seq: int = 4096
     # > 0: room for a prefix of so many tokens that all sequences share (set_prefix): it is stored once and read once
-    # a step for the whole batch; max_seq is then what every sequence may have behind it
+    # a step for the whole batch (bfloat16 and int8, head sizes 64 and 128; else once per sequence and head, by a plain
+    # kernel that is a hundred times slower); max_seq is then what every sequence may have behind it
     max_prefix: int = 0
     max_batch: int = 1
     n_splits: int = 0              # key splits of the decode attention (0 = choose)
