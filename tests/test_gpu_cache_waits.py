@@ -23,7 +23,7 @@ def gives_up(ctx, call) -> bool:
     (a poll itself waits for a while)."""
     side, (a, b) = torch.cuda.Stream(), (torch.empty(1 << 28, dtype=torch.uint8, device="cuda") for _ in range(2))
     torch.cuda.synchronize()
-    for _ in range(60):
+    for _ in range(1000):   # (head size 64: one in twenty gives up)
         with torch.cuda.stream(side):
             for _ in range(3):
                 a.copy_(b)
