@@ -17,15 +17,15 @@
 // block's product with v starts from zero and is added to the row's output in registers, in float32: the tensor core
 // truncates.
 //
-// What bounds it: a unit's chain for a block of 64 keys, 4300 cycles (waits, maxima, the output's turn, exponentials,
+// What bounds it: a unit's chain for a block of 64 keys, 4200 cycles (waits, maxima, the output's turn, exponentials,
 // weights and their terms), of which two run side by side, and 16000 cycles of a CTA before its first block (q) and behind
-// its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 104.7 us, 0.33 PFLOP/s of the
-// formula's operations (in a program where it took 110, a first value scale that made all weights wide: 133).
-// 64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion:
-// wide weights throughout (115), a branch on the form for every word that is converted (111.5), both forms in one loop of
-// the warp that issues the products (+ 0.5), its look at the form a block ahead (+ 2), 184 registers a thread for the units
-// and 72 for the rest (105.5), 192 and 64 (113.7).  Faster by 1: scores four blocks ahead, which leaves no place for a third
-// term.  bfloat16: 200 registers for the units (+ 1.4), scores three blocks ahead (+ 0.4).
+// its last (the units' exchange).  INT8, 2048 tokens from position 0, 32 / 8 heads of 128: 99.9 us, 0.34 PFLOP/s of the
+// formula's operations.  64 x 32 / 8 heads behind 8192 bfloat16 rows: 35 us standing alone.  Slower, us for the INT8 portion:
+// wide weights throughout (115 when two terms took 104), a branch on the form for every word that is converted (+ 7), the
+// warp that issues the products waiting for what the units have waited for, and for the keys of later scores ahead of a
+// product (104.8), 184 registers a thread for the units and 72 for the rest (103.6), 192 and 64 (111.5), 208 and 48 (113).
+// Faster by 1: scores four blocks ahead, which leaves no place for a third term.  bfloat16: 200 registers for the units
+// (+ 1.4), scores three blocks ahead (+ 0.4).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -484,21 +484,23 @@ attend_tile_kernel(CacheView c, TileArgs a) {
             auto issue = [&](auto wide_tag) {  // block g; false: the weights are of the other form, or a wait ran out
                 constexpr bool kWide = decltype(wide_tag)::value;
                 const bool more = g + kAhead < n_blocks;
-                // (what the loaders bring is there, most often, before the weights are)
-                ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                // (INT8: the units have waited for the values' stage, whose scales they need, before they gave the weights)
+                if constexpr (!kI8) ok = mbar_wait(v_full + g % kStages, (g / kStages) & 1, abort_flag, a.wait_limit);
+                if (ok) ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
+                if (!ok) return false;
                 if constexpr (!kWide) {
                     const int wide = reinterpret_cast<const int *>(scales + (g % kStages) * S::kScaleFloats)[3 * kKeys + 1];
                     if (__any_sync(0xffffffffu, wide)) return false;
                 }
-                if (ok && more) ok = mbar_wait(k_full + (g + kAhead) % kStages, ((g + kAhead) / kStages) & 1, abort_flag, a.wait_limit);
-                if (ok) ok = mbar_wait(p_full + (g & 1), (g >> 1) & 1, abort_flag, a.wait_limit);
-                if (!ok) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) {
-                    values(g, kWide);
-                    if (more) scores(g + kAhead);  // (over columns whose weights the product before reads first)
-                }
+                if (elect_one()) values(g, kWide);
                 __syncwarp();
+                if (more) {
+                    ok = mbar_wait(k_full + (g + kAhead) % kStages, ((g + kAhead) / kStages) & 1, abort_flag, a.wait_limit);
+                    if (!ok) return false;
+                    if (elect_one()) scores(g + kAhead);  // (over columns whose weights the product before reads first)
+                    __syncwarp();
+                }
                 ++g;
                 return true;
             };
