@@ -16,8 +16,8 @@
 // arithmetic: the tensor core truncates.
 //
 // What bounds it: issue (0.59 of the slots: the codes' conversion to float16, legacy products) and the loads' latency, short
-// of the cache's bytes.  INT8, 32 / 8 heads of 128: two sequences of 65536 rows 49.8 us (4.9 TB/s, join included), 64 of 1
-// to 2048 rows 44.2 (4.8); the copy rate is 6.6.  Where every block begins again: 64 of 32 to 2048 rows 37 -> 69 us.
+// of the cache's bytes.  INT8, 32 / 8 heads of 128: two sequences of 65536 rows 49.9 us (4.9 TB/s, join included), 64 of 1
+// to 2048 rows 44.0 (4.8); the copy rate is 6.6.  Where every block begins again: 64 of 32 to 2048 rows 37 -> 69 us.
 #pragma once
 
 #include "qk_cache.h"

@@ -24,7 +24,8 @@
 // wide weights throughout (115 when two terms took 104), a branch on the form for every word that is converted (+ 7), the
 // warp that issues the products waiting for what the units have waited for, and for the keys of later scores ahead of a
 // product (104.8), 184 registers a thread for the units and 72 for the rest (103.6), 192 and 64 (111.5), 208 and 48 (113).
-// Faster by 1: scores four blocks ahead, which leaves no place for a third term.  bfloat16: 200 registers for the units
+// Where the first value scale makes all weights wide: 131.  Faster by 1: scores four blocks ahead, which leaves no place for
+// a third term.  bfloat16: 200 registers for the units
 // (+ 1.4), scores three blocks ahead (+ 0.4).
 #include <cuda_fp16.h>
 
